@@ -291,6 +291,127 @@ int pcb_pack_u8(const void* src, int64_t batch, int64_t rows, int64_t cols,
                 int64_t ssb, int64_t ssr, int64_t ssc,
                 void* dst, int64_t dsb, int64_t dsr, int64_t cols_padded, void* stream);
 
+/* Quantized output of pcb_rms_norm_fwd. */
+typedef enum pcb_norm_quant {
+  PCB_NORM_QUANT_NONE = 0,
+  PCB_NORM_QUANT_BLOCK = 1, /* 1x128 blocks: the scales of pcb_quant_per_block   */
+  PCB_NORM_QUANT_ROW = 2    /* one scale a row: the scales of pcb_quant_per_channel */
+} pcb_norm_quant;
+
+/*
+ * Root-mean-square norm with the residual's addition and an FP8 output (no
+ * counterpart in the reference, whose training linears quantize a norm's
+ * output in a pass of their own).  For each of `rows` rows of `dim` elements:
+ *   h = x + residual, rounded to x_dtype and written to h (residual NULL: h is
+ *       x, and the h argument is not used),
+ *   s = 1 / sqrt(mean(h^2) + eps), written to rstd[row],
+ *   y = h s weight, written to y in x_dtype unless y is NULL,
+ *   q = the FP8 quantization of the unrounded y (quant_mode), scale its
+ *       dequantization scales: scale[row*ssr + block*ssb], or scale[row*ssr].
+ * x, residual, h, y: x_dtype F32/F16/BF16, rows of contiguous elements, row
+ * strides sx, sr, sh, sy.  weight: [dim], contiguous, F32/F16/BF16 of its own.
+ * q: E4M3 or E5M2, row stride sq.  pow2_scales: the power-of-two scales of
+ * pcb_quant_per_block_pow2 (blocks only).  Outputs must not overlap inputs.
+ */
+int pcb_rms_norm_fwd(const void* x, int x_dtype, int64_t rows, int64_t dim, int64_t sx, const void* residual,
+                     int64_t sr, const void* weight, int w_dtype, float eps, void* h, int64_t sh, void* y, int64_t sy,
+                     void* q, int q_dtype, int64_t sq, float* scale, int64_t ssr, int64_t ssb, int quant_mode,
+                     int pow2_scales, float quant_eps, float* rstd, void* stream);
+
+/* Device workspace (bytes, 16-byte aligned) of pcb_rms_norm_bwd. */
+int64_t pcb_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
+
+/*
+ * Backward pass of pcb_rms_norm_fwd, from the h and rstd that it wrote:
+ *   n = h s, dx = s (weight dy - n mean(n weight dy)) + dh, dw = sum_rows dy n
+ * with dh the gradient of the h output (NULL: none).  dx is the gradient of x
+ * and of the residual alike.  dy, h, dh, dx: x_dtype, contiguous rows; weight
+ * and dw: [dim], w_dtype.  dw is summed in a fixed order.
+ */
+int pcb_rms_norm_bwd(const void* dy, int64_t sdy, const void* h, int64_t sh, int x_dtype, int64_t rows, int64_t dim,
+                     const void* dh, int64_t sdh, const void* weight, int w_dtype, const float* rstd, void* dx,
+                     int64_t sdx, void* dw, void* workspace, int64_t workspace_bytes, void* stream);
+
+typedef enum pcb_grad_norm_type {
+  PCB_GRAD_NORM_L2 = 0, /* sqrt of the sum of squares */
+  PCB_GRAD_NORM_MAX = 1 /* largest magnitude          */
+} pcb_grad_norm_type;
+
+/* Device workspace (bytes, 8-byte aligned) of pcb_grad_norm and pcb_grad_clip
+ * for `count` tensors. */
+int64_t pcb_grad_norm_workspace_bytes(int64_t count);
+
+/*
+ * Global norm over `count` gradient tensors (no counterpart in the reference):
+ * grads[i] is a device pointer to numel[i] contiguous elements of dtypes[i]
+ * (F32/F16/BF16; types may be mixed).  The four arrays are host memory and
+ * are read before the call returns.  *norm (device, fp32) gets the norm;
+ * squares are summed in fp32 runs of at most 32 and in fp64 from there on, in
+ * a fixed order.  No tensors, or only empty ones: 0.
+ */
+int pcb_grad_norm(const void* const* grads, const int64_t* numel, const int* dtypes, int64_t count, int norm_type,
+                  float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * pcb_grad_norm, then out[i] = grads[i] * min(1, max_norm / (norm + eps)),
+ * each product rounded once to the tensor's type.  out[i] may be grads[i];
+ * tensors must not overlap otherwise.  A NaN norm makes every output NaN.
+ */
+int pcb_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes, int64_t count,
+                  int norm_type, float max_norm, float eps, float* norm, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+
+/* The scaling of pcb_grad_clip alone, with the norm read from the device
+ * (a norm that several processes have joined, say). */
+int pcb_grad_scale(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes, int64_t count,
+                   const float* norm, float max_norm, float eps, void* stream);
+
+/* Reduction of pcb_linear_ce_*. */
+typedef enum pcb_reduction {
+  PCB_REDUCTION_NONE = 0,
+  PCB_REDUCTION_SUM = 1,
+  PCB_REDUCTION_MEAN = 2 /* over the tokens that are not left out */
+} pcb_reduction;
+
+/* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_fwd: the
+ * statistics of every 128 columns of every token, never the logits. */
+int64_t pcb_linear_ce_fwd_workspace_bytes(int64_t tokens, int64_t vocab);
+
+/*
+ * Softmax cross entropy of an output projection, without its logits (no
+ * counterpart in the reference):
+ *   l = x weight^T, lse_i = log sum_j exp(l_ij), loss_i = lse_i - l_i,target[i]
+ * x [tokens, dim] and weight [vocab, dim]: F16 or BF16, contiguous rows, row
+ * strides sx, sw that are multiples of 8, 16-byte aligned (PCB_ERR_LAYOUT
+ * otherwise).  target: int64 [tokens]; tokens whose target is ignore_index
+ * are left out (loss 0, no gradient).  A target outside [0, vocab) makes its
+ * token's loss and gradients NaN and is reported through
+ * pcb_get_device_error().  Logits, statistics and sums are fp32.
+ * Writes loss ([tokens], or one value: the sum, or the mean over the tokens
+ * that are not left out, NaN if there are none), lse [tokens] and count [1]
+ * (those tokens), which the backward pass reads.  tokens == 0 writes nothing.
+ */
+int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                      int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                      float* loss, float* lse, float* count, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_bwd; piece and
+ * want_dx as there. */
+int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx);
+
+/*
+ * Gradients of pcb_linear_ce_fwd: with G = (softmax(l) - onehot(target)) times
+ * the loss's gradient, dx = G weight and dw = G^T x (either may be NULL), in
+ * x's type.  dloss: [tokens] or [1], as loss.  The vocabulary is taken in
+ * pieces of `piece` columns (rounded down to a multiple of 256; <= 0: as many
+ * as keep G at 128 MiB, at least 2048), of which only one piece of G exists at
+ * a time.  Sums are taken in a fixed order.
+ */
+int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                      int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                      const float* lse, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
+                      int64_t sdw, int64_t piece, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,6 +119,40 @@ _SIGNATURES = {
          _vp, _i64, _i64, _i64,  # xs
          _i, _f, _vp],
     ),
+    "pcb_rms_norm_fwd": (
+        _i,
+        [_vp, _i, _i64, _i64, _i64,  # x, rows, dim, row stride
+         _vp, _i64, _vp, _i, _f,  # residual, weight, eps
+         _vp, _i64, _vp, _i64,  # h, y
+         _vp, _i, _i64, _vp, _i64, _i64, _i, _i, _f,  # q, scale, quant mode, pow2, quant eps
+         _vp, _vp],
+    ),
+    "pcb_rms_norm_bwd_workspace_bytes": (_i64, [_i64, _i64]),
+    "pcb_rms_norm_bwd": (
+        _i,
+        [_vp, _i64, _vp, _i64, _i, _i64, _i64,  # dy, h, dtype, rows, dim
+         _vp, _i64, _vp, _i, _vp,  # dh, weight, rstd
+         _vp, _i64, _vp, _vp, _i64, _vp],
+    ),
+    "pcb_grad_norm_workspace_bytes": (_i64, [_i64]),
+    "pcb_grad_norm": (_i, [_vp, _vp, _vp, _i64, _i, _vp, _vp, _i64, _vp]),
+    "pcb_grad_clip": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _f, _f, _vp, _vp, _i64, _vp]),
+    "pcb_grad_scale": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _f, _f, _vp]),
+    "pcb_linear_ce_fwd_workspace_bytes": (_i64, [_i64, _i64]),
+    "pcb_linear_ce_fwd": (
+        _i,
+        [_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64,  # x, weight, dtype, tokens, vocab, dim
+         _vp, _i64, _i, _vp, _vp, _vp,  # target, ignore index, reduction, loss, lse, count
+         _vp, _i64, _vp],
+    ),
+    "pcb_linear_ce_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i]),
+    "pcb_linear_ce_bwd": (
+        _i,
+        [_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64,  # x, weight, dtype, tokens, vocab, dim
+         _vp, _i64, _i, _vp, _vp, _vp,  # target, ignore index, reduction, lse, count, dloss
+         _vp, _i64, _vp, _i64, _i64,  # dx, dw, piece
+         _vp, _i64, _vp],
+    ),
     "pcb_pack_u8": (_i, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp]),
 }
 

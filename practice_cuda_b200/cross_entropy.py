@@ -1,0 +1,139 @@
+"""Softmax cross entropy of an output projection, without its logits.
+
+``linear_cross_entropy(x, weight, target)`` is
+``cross_entropy(x @ weight.T, target)`` with the projection and the loss in
+one: the logits leave the tensor cores as each token's softmax statistics, and
+the backward pass computes them again in pieces of the vocabulary, so that no
+more than one piece of their gradient exists at a time.  The reference computes
+the whole logits and their loss in torch
+(``fp8_training/fp8_bench/bench/bench_fsdp2.py:120-187``).
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_ALIGN = 8  # elements: 16 bytes
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with contiguous rows that start on 16-byte boundaries (a copy with
+    padded rows where they do not)."""
+    if t.stride(1) == 1 and t.stride(0) % _ALIGN == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    rows, cols = t.shape
+    padded = torch.empty((rows, -(-cols // _ALIGN) * _ALIGN), device=t.device, dtype=t.dtype)
+    view = padded[:, :cols]
+    view.copy_(t)
+    return view
+
+
+def _check(x, weight, target, reduction, piece):
+    what = "linear_cross_entropy"
+    _lib.require_cuda(x, "x")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what}: x must be bf16 or fp16, got {x.dtype}")
+    if weight.dtype != x.dtype:
+        raise ValueError(f"{what}: weight must have x's type {x.dtype}, got {weight.dtype}")
+    if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"{what}: x [..., dim] and weight [vocab, dim] do not fit: "
+                         f"{tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"{what}: weight has no elements: {tuple(weight.shape)}")
+    if target.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{what}: target must be int64 or int32, got {target.dtype}")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"{what}: target must have shape {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    if weight.device != x.device or target.device != x.device:
+        raise ValueError(f"{what}: x is on {x.device}, weight on {weight.device}, target on {target.device}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f'{what}: reduction must be "mean", "sum" or "none", got {reduction!r}')
+    if piece is not None and piece < 1:
+        raise ValueError(f"{what}: vocab_piece must be positive, got {piece}")
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, reduction, piece):
+        x2, w2 = _aligned_rows(x), _aligned_rows(weight)
+        tokens, dim = x.shape
+        vocab = weight.shape[0]
+        device = x.device
+        lib = _lib.lib()
+        with torch.cuda.device(device):
+            loss = torch.empty(tokens if reduction == 0 else (), device=device, dtype=torch.float32)
+            stats = torch.empty(tokens + 1, device=device, dtype=torch.float32)  # lse, count
+            if tokens == 0:
+                loss.fill_(float("nan") if reduction == 2 else 0.0)
+            nbytes = lib.pcb_linear_ce_fwd_workspace_bytes(tokens, vocab)
+            workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+            lse = stats.data_ptr()
+            status = lib.pcb_linear_ce_fwd(
+                x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x.dtype], tokens, vocab, dim,
+                target.data_ptr(), ignore_index, reduction, loss.data_ptr(), lse, lse + 4 * tokens,
+                workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
+            if status:
+                _lib.check(status, "pcb_linear_ce_fwd")
+        ctx.save_for_backward(x2, w2, target, stats)
+        ctx.args = (ignore_index, reduction, piece)
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        x2, w2, target, stats = ctx.saved_tensors
+        ignore_index, reduction, piece = ctx.args
+        tokens, dim = x2.shape
+        vocab = w2.shape[0]
+        device = x2.device
+        want_dx, want_dw = ctx.needs_input_grad[:2]
+        lib = _lib.lib()
+        with torch.cuda.device(device):
+            dloss = dloss.to(torch.float32).contiguous()
+            dx = torch.empty((tokens, dim), device=device, dtype=x2.dtype) if want_dx else None
+            dw = torch.empty((vocab, dim), device=device, dtype=x2.dtype) if want_dw else None
+            nbytes = lib.pcb_linear_ce_bwd_workspace_bytes(tokens, vocab, dim, piece, int(want_dx))
+            workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+            lse = stats.data_ptr()
+            status = lib.pcb_linear_ce_bwd(
+                x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x2.dtype], tokens, vocab, dim,
+                target.data_ptr(), ignore_index, reduction, lse, lse + 4 * tokens, dloss.data_ptr(),
+                dx.data_ptr() if want_dx else None, dim, dw.data_ptr() if want_dw else None, dim, piece,
+                workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
+            if status:
+                _lib.check(status, "pcb_linear_ce_bwd")
+        return dx, dw, None, None, None, None
+
+
+def linear_cross_entropy(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    target: torch.Tensor,
+    *,
+    reduction: str = "mean",
+    ignore_index: int = -100,
+    vocab_piece: Optional[int] = None,
+) -> torch.Tensor:
+    """Cross entropy of the logits ``x @ weight.T`` (x [..., dim], weight
+    [vocab, dim], both bf16 or both fp16) against ``target`` [...], in fp32.
+
+    ``reduction``, ``ignore_index`` and the mean over no token at all (NaN,
+    with zero gradients) are those of ``torch.nn.functional.cross_entropy``.
+    Differentiable in ``x`` and ``weight``; a gradient that is not needed is
+    not computed.  ``vocab_piece`` bounds the columns of the logits' gradient
+    that exist at a time in the backward pass (rounded down to a multiple of
+    256, at least 256; default: as many as fit 128 MiB, at least 2048).
+
+    A target outside the vocabulary that is not ``ignore_index`` makes its
+    loss NaN and sets the device error word (``_lib.device_error``).
+    """
+    _check(x, weight, target, reduction, vocab_piece)
+    shape = target.shape
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    t = target.reshape(-1).to(torch.int64).contiguous()
+    loss = _LinearCrossEntropy.apply(x2, weight, t, int(ignore_index), _REDUCTIONS[reduction], int(vocab_piece or 0))
+    return loss.view(shape) if reduction == "none" else loss

@@ -15,9 +15,10 @@ namespace pcb {
 
 // ----------------------------------------------------------------------------
 // Device error word: {code, site, info}.  The first failure sticks (CAS on
-// code); pcb_get_device_error() reads and clears it.
+// code); pcb_get_device_error() reads and clears it.  Each translation unit
+// has a word of its own.
 // ----------------------------------------------------------------------------
-__device__ unsigned int g_device_error[3];
+static __device__ unsigned int g_device_error[3];
 
 enum ErrorSite : int {
   SITE_GEMM_PRODUCER = 1,

@@ -1,0 +1,316 @@
+// C entry points of the output projection's cross entropy.
+#include <algorithm>
+
+#include "cross_entropy.cuh"
+#include "host.cuh"
+
+using namespace pcb;
+
+namespace {
+
+// 3-D map (inner, outer, 1) of 16-bit elements with 64-element rows in the
+// 128-byte swizzle.
+bool make_map(CUtensorMap* map, const void* base, int dt, int64_t inner, int64_t outer, int64_t stride, int box_outer,
+              CUtensorMapL2promotion promotion) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t row = (cuuint64_t)stride * 2;
+  const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)outer, 1};
+  const cuuint64_t strides[2] = {row, std::max<cuuint64_t>(16, (cuuint64_t)outer * row)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_outer, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, dt == PCB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool load_map(CUtensorMap* map, const void* base, int dt, int64_t inner, int64_t outer, int64_t stride, int box_outer) {
+  return make_map(map, base, dt, inner, outer, stride, box_outer, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+bool store_map(CUtensorMap* map, void* base, int dt, int64_t inner, int64_t outer, int64_t stride) {
+  return make_map(map, base, dt, inner, outer, stride, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE);
+}
+
+constexpr int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <int MODE>
+int launch_product(const loss::Params& p, cudaStream_t s) {
+  auto kernel = loss::vocab_product_kernel<MODE>;
+  ensure_smem_attr(kernel, loss::SMEM_ALLOC);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * std::min(p.num_tiles, device_info().sm_count / 2)), 1, 1);
+  cfg.blockDim = dim3(loss::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = loss::SMEM_ALLOC;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  // griddepcontrol.wait precedes every global access of the kernel.
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, p);
+  return check_launch("vocab_product_kernel");
+}
+
+template <typename K, typename... A>
+int launch_after(K kernel, const char* what, int64_t grid, int threads, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+  return check_launch(what);
+}
+
+// tile counts and K split of a problem
+void shape(loss::Problem& q, int64_t m, int64_t n, int64_t k, int splits) {
+  q.m = (int)m;
+  q.n = (int)n;
+  q.m_blocks = (int)up(m, loss::TILE);
+  q.n_blocks = (int)up(n, loss::TILE);
+  q.k_stages = (int)up(k, loss::BK);
+  q.split_stages = (int)up(q.k_stages, splits);
+  q.splits = (int)up(q.k_stages, q.split_stages);  // none of them empty
+  q.tiles = q.m_blocks * q.n_blocks * q.splits;
+}
+
+int check_shapes(int dtype, int64_t tokens, int64_t vocab, int64_t dim, int reduction) {
+  if (dtype != PCB_DTYPE_F16 && dtype != PCB_DTYPE_BF16)
+    return fail(PCB_ERR_INVALID, "linear cross entropy: x and weight must be F16 or BF16");
+  if (tokens < 0 || vocab <= 0 || dim <= 0)
+    return fail(PCB_ERR_INVALID, "linear cross entropy needs tokens >= 0, vocab > 0 and dim > 0");
+  if (reduction < loss::kNone || reduction > loss::kMean)
+    return fail(PCB_ERR_INVALID, "linear cross entropy: reduction must be 0 (none), 1 (sum) or 2 (mean)");
+  if (tokens > (1 << 26) || vocab > (1 << 26) || dim > (1 << 26))
+    return fail(PCB_ERR_UNSUPPORTED, "linear cross entropy: dimension too large");
+  if (up(tokens, loss::TILE) * up(vocab, loss::TILE) > (1 << 30))
+    return fail(PCB_ERR_UNSUPPORTED, "linear cross entropy: too many tiles");
+  return PCB_OK;
+}
+
+int check_operands(const void* x, int64_t sx, const void* w, int64_t sw) {
+  if (!x || !w) return fail(PCB_ERR_INVALID, "null pointer");
+  if (!aligned(x, 16) || !aligned(w, 16) || sx % 8 != 0 || sw % 8 != 0)
+    return fail(PCB_ERR_LAYOUT, "linear cross entropy: rows of x and weight must start on 16-byte boundaries");
+  if (device_info().major != 10) return fail(PCB_ERR_DEVICE, "linear cross entropy needs an sm_100 device");
+  return PCB_OK;
+}
+
+// A workspace cut into 256-byte aligned parts.
+struct Cut {
+  int64_t at = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t a = at;
+    at += up(bytes, 256) * 256;
+    return a;
+  }
+};
+
+struct FwdPlan {
+  int64_t partial, target_logit, sums, ticket, bytes;
+  FwdPlan(int64_t tokens, int64_t vocab) {
+    Cut c;
+    partial = c.take(up(vocab, loss::TILE) * 2 * tokens * 8);
+    target_logit = c.take(tokens * 4);
+    sums = c.take(up(tokens, 32) * 16);
+    ticket = c.take(4);
+    bytes = c.at;
+  }
+};
+
+struct BwdPlan {
+  int64_t cols, pieces, pitch;  // of G
+  int splits;                   // parts of K of dX
+  int64_t g, acc, weight, alpha, bytes;
+  BwdPlan(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, bool want_dx) {
+    // G of one piece takes 128 MiB at most (and is no narrower than 2048
+    // columns): pieces of even width, whole tiles each.
+    if (piece <= 0) piece = std::max<int64_t>(2048, ((int64_t)128 << 20) / 2 / tokens);
+    piece = std::max<int64_t>(loss::TILE, piece / loss::TILE * loss::TILE);
+    pieces = up(vocab, piece);
+    cols = up(up(vocab, pieces), loss::TILE) * loss::TILE;
+    pieces = up(vocab, cols);
+    pitch = std::min(cols, up(vocab, 64) * 64);
+    splits = 1;
+    const int64_t dx_tiles = up(tokens, loss::TILE) * up(dim, loss::TILE);
+    if (want_dx && pieces == 1) {
+      // dX's tiles are few and long where tokens are few: cut them along the
+      // vocabulary so that none is longer than a quarter of an SM pair's share.
+      const int64_t stages = up(vocab, loss::BK);
+      const int64_t all = dx_tiles * stages + up(vocab, loss::TILE) * up(dim, loss::TILE) * up(tokens, loss::BK);
+      const int64_t longest = std::max<int64_t>(16, all / (4 * std::max(1, device_info().sm_count / 2)));
+      splits = (int)std::min<int64_t>(std::max<int64_t>(1, stages / longest), 64);
+    }
+    Cut c;
+    g = c.take(tokens * pitch * 2);
+    acc = c.take(want_dx && (pieces > 1 || splits > 1) ? dx_tiles * splits * loss::TILE * loss::TILE * 4 : 0);
+    weight = c.take(tokens * 4);
+    alpha = c.take(4);
+    bytes = c.at;
+  }
+};
+
+loss::Params base_params(int dtype, int64_t vocab, const int64_t* target, int64_t ignore_index) {
+  loss::Params p;
+  std::memset(&p, 0, sizeof(p));
+  p.fmt = dtype == PCB_DTYPE_BF16 ? 1 : 0;
+  p.target = reinterpret_cast<const long long*>(target);
+  p.ignore_index = ignore_index;
+  p.vocab = vocab;
+  p.grad_scale = dtype == PCB_DTYPE_BF16 ? 1.f : 16384.f;
+  return p;
+}
+
+}  // namespace
+
+namespace pcb {
+// This translation unit's device error word, read and cleared (the device is idle).
+cudaError_t take_loss_device_error(unsigned int (&h)[3]) {
+  cudaError_t e = cudaMemcpyFromSymbol(h, g_device_error, sizeof(h));
+  const unsigned int zero[3] = {0, 0, 0};
+  return e != cudaSuccess ? e : cudaMemcpyToSymbol(g_device_error, zero, sizeof(zero));
+}
+}  // namespace pcb
+
+extern "C" {
+
+int64_t pcb_linear_ce_fwd_workspace_bytes(int64_t tokens, int64_t vocab) {
+  if (tokens <= 0 || vocab <= 0) return 0;
+  return FwdPlan(tokens, vocab).bytes;
+}
+
+int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                      int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                      float* loss_out, float* lse, float* count, void* workspace, int64_t workspace_bytes,
+                      void* stream) {
+  if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
+  if (tokens == 0) return PCB_OK;
+  if (!target || !loss_out || !lse || !count) return fail(PCB_ERR_INVALID, "null pointer");
+  const FwdPlan plan(tokens, vocab);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
+    return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
+  if (int st = check_operands(x, sx, weight, sw)) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  char* ws = static_cast<char*>(workspace);
+  loss::Params p = base_params(dtype, vocab, target, ignore_index);
+  loss::Problem& q = p.prob[0];
+  if (!load_map(&q.a, x, dtype, dim, tokens, sx, loss::BM) || !load_map(&q.b, weight, dtype, dim, vocab, sw, loss::TILE / 2))
+    return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
+  shape(q, tokens, vocab, dim, 1);
+  p.num_tiles = q.tiles;
+  p.partial = reinterpret_cast<float2*>(ws + plan.partial);
+  p.target_logit = reinterpret_cast<float*>(ws + plan.target_logit);
+  p.ticket = reinterpret_cast<unsigned*>(ws + plan.ticket);
+  if (int st = launch_product<loss::kStats>(p, s)) return st;
+  loss::RowArgs r{p.partial, p.target_logit, p.target, ignore_index, vocab, (int)tokens, 2 * q.n_blocks, reduction,
+                  lse, loss_out, count, reinterpret_cast<double*>(ws + plan.sums), p.ticket};
+  return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), 256, s, r);
+}
+
+int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx) {
+  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  return BwdPlan(tokens, vocab, dim, piece, want_dx != 0).bytes;
+}
+
+int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                      int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                      const float* lse, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
+                      int64_t sdw, int64_t piece, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (tokens == 0) {
+    if (dw && cudaMemset2DAsync(dw, (size_t)sdw * 2, 0, (size_t)dim * 2, (size_t)vocab, s) != cudaSuccess)
+      return check_launch("linear cross entropy dw");
+    return PCB_OK;
+  }
+  if (!dx && !dw) return PCB_OK;
+  if (!target || !lse || !count || !dloss) return fail(PCB_ERR_INVALID, "null pointer");
+  const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
+    return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
+  if (int st = check_operands(x, sx, weight, sw)) return st;
+  char* ws = static_cast<char*>(workspace);
+  void* g = ws + plan.g;
+  float4* acc = reinterpret_cast<float4*>(ws + plan.acc);
+  loss::Params base = base_params(dtype, vocab, target, ignore_index);
+  base.lse = lse;
+  if (reduction == loss::kNone) {
+    float* row_weight = reinterpret_cast<float*>(ws + plan.weight);
+    float* alpha = reinterpret_cast<float*>(ws + plan.alpha);
+    if (int st = launch_after(loss::loss_weights_kernel, "loss_weights_kernel", 1, 1024, s, dloss, base.target,
+                              (long long)ignore_index, (int)tokens, base.grad_scale, row_weight, alpha))
+      return st;
+    base.row_weight = row_weight;
+    base.alpha = alpha;
+  } else {
+    base.dloss = dloss;
+    base.count = reduction == loss::kMean ? count : nullptr;
+  }
+  for (int64_t i = 0; i < plan.pieces; ++i) {
+    const int64_t col0 = i * plan.cols, cols = std::min(plan.cols, vocab - col0);
+    const char* w = static_cast<const char*>(weight) + col0 * sw * 2;
+    bool ok = true;
+    loss::Params p = base;
+    p.col0 = (int)col0;
+    loss::Problem& q = p.prob[0];
+    ok &= load_map(&q.a, x, dtype, dim, tokens, sx, loss::BM);
+    ok &= load_map(&q.b, w, dtype, dim, cols, sw, loss::TILE / 2);
+    ok &= store_map(&q.c_box, g, dtype, cols, tokens, plan.pitch);
+    shape(q, tokens, cols, dim, 1);
+    q.c_tma = 1;
+    q.c = g;
+    q.scm = plan.pitch;
+    p.num_tiles = q.tiles;
+    if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
+    if (int st = launch_product<loss::kGradient>(p, s)) return st;
+
+    p = base;
+    int n = 0;
+    if (dx) {
+      loss::Problem& d = p.prob[n++];
+      ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, loss::BM);
+      ok &= load_map(&d.b, w, dtype, dim, cols, sw, loss::BK);
+      shape(d, tokens, dim, cols, plan.splits);
+      d.acc = acc;
+      if (plan.splits > 1) d.acc_mode = loss::kAccSlab;
+      else if (plan.pieces > 1) d.acc_mode = i == 0 ? loss::kAccWrite : i + 1 < plan.pieces ? loss::kAccAdd : loss::kAccLast;
+      d.c = dx;
+      d.scm = sdx;
+      d.c_tma = aligned(dx, 16) && sdx % 8 == 0;
+      if (d.c_tma) ok &= store_map(&d.c_box, dx, dtype, dim, tokens, sdx);
+    }
+    if (dw) {
+      loss::Problem& d = p.prob[n++];
+      ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, loss::BK);
+      ok &= load_map(&d.b, x, dtype, dim, tokens, sx, loss::BK);
+      shape(d, cols, dim, tokens, 1);
+      d.a_mn = 1;
+      char* out = static_cast<char*>(dw) + col0 * sdw * 2;
+      d.c = out;
+      d.scm = sdw;
+      d.c_tma = aligned(out, 16) && sdw % 8 == 0;
+      if (d.c_tma) ok &= store_map(&d.c_box, out, dtype, dim, cols, sdw);
+    }
+    if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
+    p.num_tiles = p.prob[0].tiles + (n > 1 ? p.prob[1].tiles : 0);
+    if (int st = launch_product<loss::kProducts>(p, s)) return st;
+    if (dx && plan.splits > 1) {
+      const loss::Problem& d = p.prob[0];
+      const loss::JoinArgs j{acc, d.m, d.n, d.m_blocks, d.n_blocks, d.splits, p.fmt, static_cast<uint16_t*>(dx), sdx};
+      if (int st = launch_after(loss::loss_join_kernel, "loss_join_kernel",
+                                (int64_t)d.m_blocks * d.n_blocks * 2 * loss::kAccVec, 256, s, j, p))
+        return st;
+    }
+  }
+  return PCB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,632 @@
+// Softmax cross entropy of an output projection without its logits.
+//
+//   l = X W^T (X [tokens, dim], W [vocab, dim]),  lse_i = log sum_j exp(l_ij),
+//   nll_i = lse_i - l_i,target
+//   G_ij = (exp(l_ij - lse_i) - [j = target_i]) w_i,  dX = a G W,  dW = a G^T X
+//
+// One tcgen05 product kernel in three forms:
+//   kStats     a tile of logits leaves the tensor memory as the maximum and the
+//              sum of exponentials of each row's 128 columns, and the target's
+//              logit; the logits are never written.
+//   kGradient  the logits of one piece of the vocabulary again, leaving as G in
+//              the operands' 16-bit type (the one rounding that a tensor-core
+//              product of G asks for; w_i and a are split so that it is of the
+//              order of 1 and the loss's scale stays in fp32).
+//   kProducts  dX += G W and dW = G^T X of that piece in one launch: the tiles
+//              of both share the grid, so neither leaves SMs idle at its end.
+// Logits, softmax statistics and every sum are fp32; tiles are 256 x 256 on a
+// CTA pair (cta_group::2), 64-deep stages of 128-byte swizzled operands by TMA,
+// two accumulators of 256 fp32 columns in tensor memory, so that a tile's
+// epilogue runs under the next tile's products.  Bound by the tensor cores.
+#pragma once
+
+#include "gemm_sm100.cuh"
+
+namespace pcb {
+namespace loss {
+
+enum Mode : int { kStats = 0, kGradient = 1, kProducts = 2 };
+enum Acc : int { kAccNone = 0, kAccWrite = 1, kAccAdd = 2, kAccLast = 3, kAccSlab = 4 };
+
+constexpr int BM = 128;            // rows of the tile per CTA
+constexpr int TILE = 256;          // tile rows of the pair, and tile columns
+constexpr int BK = 64;             // K elements of a stage: one 128-byte swizzle atom of 16-bit values
+constexpr int UMMA_K = 16;
+constexpr int STAGES = 6;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr int B_BYTES = TILE / 2 * BK * 2;  // each CTA stages half of the columns
+constexpr int SLAB = 64 * BK * 2;           // 64 MN elements x 64 K rows of an MN-major operand
+constexpr int NACC = 2;
+constexpr int kThreads = 384;
+constexpr int kEpiWarp0 = 4;
+constexpr int EPI_COLS = TILE / 2;  // columns of an epilogue thread
+constexpr int kGroupM = 16;         // tile rows that share the columns of W in L2
+constexpr int kAccVec = EPI_COLS / 4;  // float4s of an epilogue thread's share of a tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+constexpr int OFF_B = STAGES * A_BYTES;
+constexpr int OFF_CSTG = OFF_B + STAGES * B_BYTES;  // 4 KB per epilogue warp
+constexpr int OFF_BAR = OFF_CSTG + 8 * 4096;
+constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 2 * NACC) * 8;
+constexpr int SMEM_ALLOC = OFF_MISC + 16 + 1024;  // slack for the 1 KB alignment
+static_assert(SMEM_ALLOC <= 232448, "shared memory per CTA");
+
+enum Site : int { SITE_LOSS_PRODUCER = 16, SITE_LOSS_MMA = 17, SITE_LOSS_EPILOGUE = 18, SITE_LOSS_TARGET = 19 };
+
+// One matrix product C [m, n] = A B of a launch.
+struct Problem {
+  CUtensorMap a, b, c_box;
+  int m, n;
+  int m_blocks, n_blocks, splits;  // splits: parts of K, each a tile of its own
+  int tiles;                       // m_blocks * n_blocks * splits
+  int k_stages, split_stages;
+  int a_mn;   // A is M-major (kProducts)
+  int c_tma;  // C leaves through TMA stores
+  void* c;
+  long long scm;
+  float4* acc;  // fp32 accumulators in tile order, for the Acc modes
+  int acc_mode;
+};
+
+struct Params {
+  Problem prob[2];
+  int num_tiles;
+  int fmt;  // 0 fp16, 1 bf16
+  // rows
+  const long long* target;
+  long long ignore_index;
+  long long vocab;
+  const float* lse;
+  const float* row_weight;  // null: 1
+  float grad_scale;         // power of two that G carries
+  int col0;                 // first vocabulary column of the piece
+  float2* partial;          // [n_blocks * 2][m]: maximum and sum of exponentials
+  float* target_logit;      // [m]
+  unsigned* ticket;         // zeroed here for the kernel that follows
+  // alpha = *dloss / *count (or *dloss, or *alpha)
+  const float* dloss;
+  const float* count;
+  const float* alpha;
+};
+
+__device__ __forceinline__ float alpha_of(const Params& p) {
+  if (p.alpha) return *p.alpha;
+  float a = *p.dloss;
+  if (p.count) a = *p.count > 0.f ? __fdiv_rn(a, *p.count) : 0.f;
+  return a / p.grad_scale;
+}
+
+__device__ __forceinline__ void umma_f16_pair_elect(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                                    uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t.reg .b64 ad, bd;\n\t"
+      "mov.b64 ad, {%1, %2};\n\t"
+      "mov.b64 bd, {%3, %4};\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, int fmt) {
+  if (fmt) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct TileAt {
+  int prob, mb, nb, split, index;  // index: within its problem
+};
+// Tiles in groups of kGroupM tile rows, rows fastest: the tiles in flight share
+// few columns of B, and a group's rows of A stay in L2.
+__device__ __forceinline__ TileAt locate(const Params& p, int tile) {
+  TileAt t;
+  t.prob = tile >= p.prob[0].tiles ? 1 : 0;
+  const Problem& q = p.prob[t.prob];
+  int i = tile - (t.prob ? p.prob[0].tiles : 0);
+  t.index = i;
+  const int area = q.m_blocks * q.n_blocks;
+  t.split = i / area;
+  i -= t.split * area;
+  const int group = i / (kGroupM * q.n_blocks);
+  const int rows = min(kGroupM, q.m_blocks - group * kGroupM);
+  i -= group * kGroupM * q.n_blocks;
+  t.nb = i / rows;
+  t.mb = group * kGroupM + i - t.nb * rows;
+  return t;
+}
+
+// 64 columns of a warp's 32 rows: every lane packs its row's 128 bytes into the
+// warp's staging buffer (128-byte swizzle), from where one TMA store takes
+// the box, or, where C's rows do not suit TMA, the warp writes row by row.
+__device__ __forceinline__ void store_box(const Params& p, const Problem& q, const uint32_t (&w)[32], uint32_t stg,
+                                          int lane, int row0, int col) {
+  if (lane == 0) gemm::bulk_wait_read<0>();
+  __syncwarp();
+  const uint32_t swz = (uint32_t)(lane & 7);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const uint32_t dst = stg + (uint32_t)lane * 128u + (((uint32_t)c ^ swz) << 4);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[4 * c]), "r"(w[4 * c + 1]),
+                 "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
+                 : "memory");
+  }
+  if (q.c_tma) {
+    gemm::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && row0 < q.m && col < q.n) gemm::tma_store_3d(&q.c_box, stg, col, row0, 0);
+    return;
+  }
+  __syncwarp();
+  uint16_t* c = static_cast<uint16_t*>(q.c);
+  const int rows = min(32, q.m - row0);
+  for (int r = 0; r < rows; ++r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = h * 32 + lane;  // column within the box
+      uint16_t v;
+      const uint32_t src = stg + (uint32_t)r * 128u + ((((uint32_t)e >> 3) ^ ((uint32_t)r & 7u)) << 4) + ((uint32_t)e & 7u) * 2u;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
+      if (col + e < q.n) c[(long long)(row0 + r) * q.scm + col + e] = v;
+    }
+  }
+  __syncwarp();
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid_constant__ Params p) {
+  constexpr uint32_t STAGE_TX = 2 * (A_BYTES + B_BYTES);  // of both CTAs, on the leader's barrier
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t s_base = smem_u32(smem);
+  const uint32_t bar_full = s_base + OFF_BAR;         // [STAGES]
+  const uint32_t bar_empty = bar_full + 8 * STAGES;   // [STAGES]
+  const uint32_t bar_tfull = bar_empty + 8 * STAGES;  // [NACC]
+  const uint32_t bar_tempty = bar_tfull + 8 * NACC;   // [NACC]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = gemm::cluster_ctarank();
+  const bool leader = rank == 0;
+  const int first_tile = (int)(blockIdx.x >> 1);
+  const int tile_step = (int)(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int i = 0; i < NACC; ++i) {
+      mbar_init(bar_tfull + 8 * i, 1);
+      mbar_init(bar_tempty + 8 * i, 16);  // one arrive per epilogue warp of both CTAs
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    gemm::prefetch_tmap(&p.prob[0].a);
+    gemm::prefetch_tmap(&p.prob[0].b);
+  }
+  if (warp == 1) gemm::tmem_alloc_pair(smem_u32(tmem_slot), NACC * TILE);
+  gemm::tc_fence_before();
+  gemm::cluster_sync_all();  // both CTAs' barriers exist before any remote arrive / TMA
+  gemm::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // The set-up above overlaps the previous kernel's tail; nothing global is
+  // read or written before that kernel has completed.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer ------------------------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < p.num_tiles && ok; tile += tile_step) {
+        const TileAt t = locate(p, tile);
+        const Problem& q = p.prob[t.prob];
+        const int a_row = t.mb * TILE + (int)rank * BM;
+        const int b_col = t.nb * TILE + (int)rank * (TILE / 2);
+        const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
+        for (int ks = t.split * q.split_stages; ks < ks1; ++ks) {
+          if (!mbar_spin_bounded(bar_empty + 8 * stage, phase ^ 1, abort_flag, SITE_LOSS_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb = bar_full + 8 * stage;
+          const uint32_t a_dst = s_base + stage * A_BYTES;
+          const uint32_t b_dst = s_base + OFF_B + stage * B_BYTES;
+          if (leader) mbar_arrive_expect_tx(fb, STAGE_TX);
+          const uint32_t fbl = gemm::mapa_shared(fb, 0);
+          if (MODE == kProducts && q.a_mn) {
+            gemm::tma_load_3d_pair(a_dst, &q.a, fbl, a_row, ks * BK, 0);
+            gemm::tma_load_3d_pair(a_dst + SLAB, &q.a, fbl, a_row + 64, ks * BK, 0);
+          } else {
+            gemm::tma_load_3d_pair(a_dst, &q.a, fbl, ks * BK, a_row, 0);
+          }
+          if (MODE == kProducts) {
+            gemm::tma_load_3d_pair(b_dst, &q.b, fbl, b_col, ks * BK, 0);
+            gemm::tma_load_3d_pair(b_dst + SLAB, &q.b, fbl, b_col + 64, ks * BK, 0);
+          } else {
+            gemm::tma_load_3d_pair(b_dst, &q.b, fbl, ks * BK, b_col, 0);
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        // Let the copies already issued land before the CTA can exit.
+        for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(bar_full + 8 * s, 0, abort_flag, SITE_LOSS_PRODUCER);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer -------------------------------
+    if (leader) {
+      int stage = 0;
+      uint32_t phase = 0, acc_cnt = 0;
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        return mbar_spin_bounded_warp(bar, parity, abort_flag, SITE_LOSS_MMA);
+      };
+      const uint64_t k_desc = gemm::make_sw128_desc(s_base, 16u), mn_desc = gemm::make_sw128_desc(s_base, SLAB);
+      constexpr uint32_t K_STEP = UMMA_K * 2 >> 4;      // 32 bytes along a K-major row
+      constexpr uint32_t MN_STEP = UMMA_K * 128 >> 4;   // 16 K rows of an MN-major slab
+      constexpr uint32_t B_STEP = MODE == kProducts ? MN_STEP : K_STEP;
+      const uint64_t b_desc = MODE == kProducts ? mn_desc : k_desc;
+      for (int tile = first_tile; tile < p.num_tiles && ok; tile += tile_step, ++acc_cnt) {
+        const TileAt t = locate(p, tile);
+        const Problem& q = p.prob[t.prob];
+        const bool a_mn = MODE == kProducts && q.a_mn;
+        const uint64_t a_desc = a_mn ? mn_desc : k_desc;
+        const uint32_t a_step = a_mn ? MN_STEP : K_STEP;
+        const uint32_t idesc = gemm::make_idesc(TILE, p.fmt, p.fmt, a_mn ? 1 : 0, MODE == kProducts ? 1 : 0, 2 * BM);
+        const uint32_t abuf = acc_cnt % NACC, d_tmem = tmem_base + abuf * TILE;
+        if (!wait(bar_tempty + 8 * abuf, ((acc_cnt / NACC) & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        const int ks0 = t.split * q.split_stages, ks1 = min(q.k_stages, ks0 + q.split_stages);
+        for (int ks = ks0; ks < ks1; ++ks) {
+          if (!wait(bar_full + 8 * stage, phase)) {
+            ok = false;
+            break;
+          }
+          gemm::tc_fence_after();
+          const uint32_t a_lo = (uint32_t)a_desc + (uint32_t)(stage * A_BYTES >> 4);
+          const uint32_t b_lo = (uint32_t)b_desc + (uint32_t)((OFF_B + stage * B_BYTES) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            umma_f16_pair_elect(d_tmem, a_lo + kk * a_step, (uint32_t)(a_desc >> 32), b_lo + kk * B_STEP,
+                                (uint32_t)(b_desc >> 32), idesc, (kk > 0 || ks > ks0) ? 1u : 0u);
+          gemm::umma_commit_elect<true>(bar_empty + 8 * stage);  // stage (of both CTAs) free once these retire
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        gemm::umma_commit_elect<true>(bar_tfull + 8 * abuf);  // accumulator ready (both CTAs)
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // -------------------------------- epilogue --------------------------------
+    const int ew = warp - kEpiWarp0;  // 0..7
+    const int quarter = warp & 3;     // tensor-memory lanes 32 * quarter .. + 31
+    const int half = ew >> 2;         // column half
+    const uint32_t stg = s_base + OFF_CSTG + (uint32_t)ew * 4096u;
+    const uint32_t bar_tempty_l = gemm::mapa_shared(bar_tempty, 0);
+    uint32_t acc_cnt = 0;
+    const float alpha = MODE == kProducts ? alpha_of(p) : 1.f;
+    for (int tile = first_tile; tile < p.num_tiles; tile += tile_step, ++acc_cnt) {
+      const TileAt t = locate(p, tile);
+      const Problem& q = p.prob[t.prob];
+      const int row0 = t.mb * TILE + (int)rank * BM + quarter * 32;  // of the warp
+      const int row = row0 + lane;
+      const int col0 = t.nb * TILE + half * EPI_COLS;
+      const bool in = row < q.m;
+      // Row values are read before the wait, so their latency is hidden.
+      long long target = -1;
+      float lse = 0.f, weight = 0.f;
+      if (MODE != kProducts && in) {
+        target = p.target[row];
+        const bool valid = target != p.ignore_index;
+        if (MODE == kGradient && valid) {
+          lse = p.lse[row];
+          weight = p.grad_scale * (p.row_weight ? p.row_weight[row] : 1.f);
+          if (target < 0 || target >= p.vocab) weight = NAN;  // no such column
+        }
+        target = valid ? target - p.col0 : -1;
+      }
+      const uint32_t abuf = acc_cnt % NACC;
+      if (!mbar_spin_bounded_warp(bar_tfull + 8 * abuf, (acc_cnt / NACC) & 1, abort_flag, SITE_LOSS_EPILOGUE)) break;
+      gemm::tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * TILE + half * EPI_COLS;
+      auto release = [&] {  // this warp has read its part of the accumulator
+        gemm::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) gemm::mbar_arrive_cluster(bar_tempty_l + 8 * abuf);
+      };
+      uint32_t v[2][32];
+      gemm::tmem_ld32_nowait(taddr, v[0]);
+      gemm::tmem_wait_ld();
+      gemm::tmem_regs_ready(v[0]);
+
+      if constexpr (MODE == kStats) {
+        float m = -INFINITY, s = 0.f, tl = 0.f;
+#pragma unroll
+        for (int c = 0; c < EPI_COLS / 32; ++c) {
+          if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
+          else release();
+          uint32_t(&u)[32] = v[c & 1];
+          const int cc = col0 + c * 32;
+          if (cc + 32 > q.n) {  // columns beyond the vocabulary
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (cc + i >= q.n) u[i] = 0xff800000u;
+          }
+          if (target >= cc && target < cc + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (target == cc + i) tl = __uint_as_float(u[i]);
+          }
+          float mc[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mc[i & 3] = fmaxf(mc[i & 3], __uint_as_float(u[i]));
+          const float mn = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
+          const float base = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: exp(-inf - 0) = 0
+          float sc[4] = {s * exp2_approx((m - base) * kLog2e), 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sc[i & 3] += exp2_approx((__uint_as_float(u[i]) - base) * kLog2e);
+          s = (sc[0] + sc[1]) + (sc[2] + sc[3]);
+          m = mn;
+          if (c + 1 < EPI_COLS / 32) {
+            gemm::tmem_wait_ld();
+            gemm::tmem_regs_ready(v[(c + 1) & 1]);
+          }
+        }
+        if (in) {
+          p.partial[(long long)(t.nb * 2 + half) * q.m + row] = make_float2(m, s);
+          if (target >= col0 && target < min(col0 + EPI_COLS, q.n)) p.target_logit[row] = tl;
+        }
+      } else {
+        float4* acc = nullptr;
+        if (MODE == kProducts && q.acc_mode != kAccNone)
+          acc = q.acc + ((long long)t.index * 2 + rank) * kAccVec * 256 + ew * 32 + lane;
+        uint32_t w[32];  // 64 packed columns
+#pragma unroll
+        for (int c = 0; c < EPI_COLS / 32; ++c) {
+          if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
+          else release();
+          uint32_t(&u)[32] = v[c & 1];
+          if constexpr (MODE == kGradient) {
+            const int cc = col0 + c * 32;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              u[i] = __float_as_uint(exp2_approx((__uint_as_float(u[i]) - lse) * kLog2e));
+            if (target >= cc && target < cc + 32) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (target == cc + i) u[i] = __float_as_uint(__uint_as_float(u[i]) - 1.f);
+            }
+            // Tokens left out get zeros, whatever their logits are.
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float lo = __uint_as_float(u[2 * i]) * weight, hi = __uint_as_float(u[2 * i + 1]) * weight;
+              w[(c & 1) * 16 + i] = weight == 0.f ? 0u : pack2(lo, hi, p.fmt);
+            }
+          } else {
+            if (q.acc_mode == kAccAdd || q.acc_mode == kAccLast) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 o = acc[(long long)(c * 8 + i) * 256];
+                u[4 * i] = __float_as_uint(__uint_as_float(u[4 * i]) + o.x);
+                u[4 * i + 1] = __float_as_uint(__uint_as_float(u[4 * i + 1]) + o.y);
+                u[4 * i + 2] = __float_as_uint(__uint_as_float(u[4 * i + 2]) + o.z);
+                u[4 * i + 3] = __float_as_uint(__uint_as_float(u[4 * i + 3]) + o.w);
+              }
+            }
+            if (q.acc_mode == kAccWrite || q.acc_mode == kAccAdd || q.acc_mode == kAccSlab) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                acc[(long long)(c * 8 + i) * 256] =
+                    make_float4(__uint_as_float(u[4 * i]), __uint_as_float(u[4 * i + 1]), __uint_as_float(u[4 * i + 2]),
+                                __uint_as_float(u[4 * i + 3]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                w[(c & 1) * 16 + i] =
+                    pack2(__uint_as_float(u[2 * i]) * alpha, __uint_as_float(u[2 * i + 1]) * alpha, p.fmt);
+            }
+          }
+          const bool stored = MODE == kGradient || q.acc_mode == kAccNone || q.acc_mode == kAccLast;
+          if ((c & 1) && stored) store_box(p, q, w, stg, lane, row0, col0 + (c - 1) * 32);
+          if (c + 1 < EPI_COLS / 32) {
+            gemm::tmem_wait_ld();
+            gemm::tmem_regs_ready(v[(c + 1) & 1]);
+          }
+        }
+      }
+    }
+    // The staging buffers stay valid until every issued store has completed.
+    if (MODE != kStats && lane == 0) gemm::bulk_wait_all();
+  }
+
+  gemm::tc_fence_before();
+  gemm::cluster_sync_all();  // no CTA leaves while its peer may still touch its smem / barriers
+  gemm::tc_fence_after();
+  if (warp == 1) gemm::tmem_dealloc_pair(tmem_base, NACC * TILE);
+}
+
+// ---------------------------------------------------------------------------
+// The rows' statistics joined: lse, the losses and their reduction.  A CTA
+// takes 32 tokens, its eight warps a strided eighth of the partials each.
+// ---------------------------------------------------------------------------
+enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
+
+struct RowArgs {
+  const float2* partial;
+  const float* target_logit;
+  const long long* target;
+  long long ignore_index, vocab;
+  int tokens, parts, reduction;
+  float* lse;       // [tokens]
+  float* loss;      // [tokens] or [1]
+  float* count;     // [1], tokens that are not left out
+  double* sums;     // [gridDim.x][2]
+  unsigned* ticket;
+};
+
+__global__ void __launch_bounds__(256) loss_rows_kernel(const RowArgs p) {
+  __shared__ float ms[8][32], ss[8][32];
+  __shared__ double total[2][8];
+  __shared__ bool last;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < p.tokens) {
+#pragma unroll 4
+    for (int i = warp; i < p.parts; i += 8) {
+      const float2 o = p.partial[(long long)i * p.tokens + row];
+      const float mn = fmaxf(m, o.x), base = mn == -INFINITY ? 0.f : mn;
+      s = s * exp2f((m - base) * kLog2e) + o.y * exp2f((o.x - base) * kLog2e);
+      m = mn;
+    }
+  }
+  ms[warp][lane] = m;
+  ss[warp][lane] = s;
+  __syncthreads();
+  double nll = 0.0, valid = 0.0;
+  if (warp == 0 && row < p.tokens) {
+    float top = ms[0][lane];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, ms[i][lane]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += ss[i][lane] * exp2f((ms[i][lane] - base) * kLog2e);
+    const float log_sum = logf(sum), lse = base + log_sum;
+    p.lse[row] = lse;
+    const long long t = p.target[row];
+    float v = 0.f;
+    if (t != p.ignore_index) {
+      valid = 1.0;
+      if (t < 0 || t >= p.vocab) {
+        v = NAN;  // no such column
+        report_error(PCB_ERR_INVALID, SITE_LOSS_TARGET);
+      } else {
+        v = (base - p.target_logit[row]) + log_sum;  // the maxima cancel before the small part is added
+      }
+      nll = (double)v;
+    }
+    if (p.reduction == kNone) p.loss[row] = v;
+  }
+  if (p.reduction == kNone) return;
+  if (warp == 0) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      nll += __shfl_xor_sync(0xffffffffu, nll, o);
+      valid += __shfl_xor_sync(0xffffffffu, valid, o);
+    }
+    if (lane == 0) {
+      p.sums[2 * blockIdx.x] = nll;
+      p.sums[2 * blockIdx.x + 1] = valid;
+      __threadfence();
+      last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (!last) return;
+  // The CTA that comes last adds all CTAs' sums, always in the same order.
+  __threadfence();
+  double a = 0.0, b = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) {
+    a += __ldcg(p.sums + 2 * i);
+    b += __ldcg(p.sums + 2 * i + 1);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if (lane == 0) total[0][warp] = a, total[1][warp] = b;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) a += total[0][i], b += total[1][i];
+    p.count[0] = (float)b;
+    p.loss[0] = (float)(p.reduction == kMean ? a / b : a);  // 0 / 0 where every token is left out
+  }
+}
+
+// Losses that are not reduced: their gradients g_i as weights w_i = g_i / A of
+// at most 1 in magnitude and the factor A (a power of two), so that G is
+// rounded at the same place whatever the scale.  One CTA.
+__global__ void __launch_bounds__(1024) loss_weights_kernel(const float* dloss, const long long* target,
+                                                            long long ignore_index, int tokens, float grad_scale,
+                                                            float* weight, float* alpha) {
+  __shared__ uint32_t top[32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  uint32_t m = 0;
+  for (int i = threadIdx.x; i < tokens; i += 1024)
+    if (target[i] != ignore_index) m = max(m, abs_bits(dloss[i]));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m = max(m, top[i]);
+  // Exponent of the largest magnitude; 1 where it is zero, subnormal or not finite.
+  const int e = (int)(m >> 23);
+  const bool usable = e >= 2 && e < 253;
+  const float up = usable ? __uint_as_float((uint32_t)(e + 1) << 23) : 1.f;     // 2^(e + 1) > max
+  const float down = usable ? __uint_as_float((uint32_t)(253 - e) << 23) : 1.f; // 1 / up
+  for (int i = threadIdx.x; i < tokens; i += 1024) weight[i] = dloss[i] * down;
+  if (threadIdx.x == 0) *alpha = up / grad_scale;
+}
+
+// dX from the parts of K: the fp32 accumulators of every part summed in order.
+struct JoinArgs {
+  const float4* acc;
+  int m, n, m_blocks, n_blocks, splits, fmt;
+  uint16_t* out;
+  long long stride;
+};
+__global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs p, const __grid_constant__ Params pp) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float alpha = alpha_of(pp);
+  // blockIdx.x: (tile of the first part, CTA of the pair, float4 of the thread)
+  const int i = blockIdx.x % kAccVec, rank = blockIdx.x / kAccVec % 2, index = blockIdx.x / kAccVec / 2;
+  const int ew = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TileAt t = locate(pp, index);
+  const int row = t.mb * TILE + rank * BM + (ew & 3) * 32 + lane;
+  const int col = t.nb * TILE + (ew >> 2) * EPI_COLS + i * 4;
+  if (row >= p.m || col >= p.n) return;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  const long long part = (long long)p.m_blocks * p.n_blocks * 2 * kAccVec * 256;
+  const float4* a = p.acc + (((long long)index * 2 + rank) * kAccVec + i) * 256 + threadIdx.x;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 o = a[s * part];
+    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+  }
+  const float f[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
+  uint16_t* out = p.out + (long long)row * p.stride + col;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (col + k < p.n) out[k] = (uint16_t)pack2(f[k], 0.f, p.fmt);
+}
+
+}  // namespace loss
+}  // namespace pcb

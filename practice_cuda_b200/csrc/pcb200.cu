@@ -1,7 +1,5 @@
-// libpcb200: the C ABI (include/pcb200.h) over the sm_100a kernels.
-// One translation unit so the device error word is a single symbol.
-#include <cudaTypedefs.h>
-
+// libpcb200: the C ABI (include/pcb200.h) over the sm_100a quantize / BMM
+// kernels.
 #include <atomic>
 #include <cstdio>
 #include <cstdlib>
@@ -10,6 +8,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "host.cuh"
 #include "gemm_sm100.cuh"
 #include "quant_kernels.cuh"
 #include "gemm_fused_sm100.cuh"
@@ -18,81 +17,13 @@
 
 using namespace pcb;
 
+namespace pcb {
+cudaError_t take_loss_device_error(unsigned int (&h)[3]);  // cross_entropy.cu's own word
+}
+
 namespace {
 
-thread_local std::string g_last_error;
 std::atomic<int> g_inject_error{0};
-
-int fail(int status, const char* what) {
-  g_last_error = what;
-  return status;
-}
-
-int check_launch(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    g_last_error = std::string(what) + ": " + cudaGetErrorString(e);
-    return PCB_ERR_LAUNCH;
-  }
-  return PCB_OK;
-}
-
-struct DeviceInfo {
-  int sm_count = 0;
-  int major = 0;
-};
-
-DeviceInfo device_info() {
-  static std::mutex mu;
-  static DeviceInfo cache[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) dev = 0;
-  std::lock_guard<std::mutex> lock(mu);
-  if (cache[dev].sm_count == 0) {
-    cudaDeviceGetAttribute(&cache[dev].sm_count, cudaDevAttrMultiProcessorCount, dev);
-    cudaDeviceGetAttribute(&cache[dev].major, cudaDevAttrComputeCapabilityMajor, dev);
-  }
-  return cache[dev];
-}
-
-bool aligned(const void* p, int64_t a) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)a) == 0; }
-
-template <typename K>
-void ensure_smem_attr(K kernel, int bytes) {
-  // cudaFuncSetAttribute is per function and device; calling it again is cheap
-  // and keeps this stateless across devices and threads.
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
-
-int elem_size(int dt) {
-  switch (dt) {
-    case PCB_DTYPE_F32: return 4;
-    case PCB_DTYPE_F16:
-    case PCB_DTYPE_BF16: return 2;
-    case PCB_DTYPE_E4M3:
-    case PCB_DTYPE_E5M2: return 1;
-    default: return 0;
-  }
-}
-
-bool is_float_in(int dt) { return dt == PCB_DTYPE_F32 || dt == PCB_DTYPE_F16 || dt == PCB_DTYPE_BF16; }
-bool is_fp8(int dt) { return dt == PCB_DTYPE_E4M3 || dt == PCB_DTYPE_E5M2; }
-
-// Dispatch a functor over (input dtype, fp8 output dtype) as compile-time ints.
-template <typename F>
-int dispatch_xy(int xt, int yt, F&& f) {
-  auto with_y = [&](auto xc) -> int {
-    if (yt == PCB_DTYPE_E4M3) return f(xc, std::integral_constant<int, PCB_DTYPE_E4M3>{});
-    if (yt == PCB_DTYPE_E5M2) return f(xc, std::integral_constant<int, PCB_DTYPE_E5M2>{});
-    return fail(PCB_ERR_INVALID, "output dtype must be E4M3 or E5M2");
-  };
-  if (xt == PCB_DTYPE_F32) return with_y(std::integral_constant<int, PCB_DTYPE_F32>{});
-  if (xt == PCB_DTYPE_F16) return with_y(std::integral_constant<int, PCB_DTYPE_F16>{});
-  if (xt == PCB_DTYPE_BF16) return with_y(std::integral_constant<int, PCB_DTYPE_BF16>{});
-  return fail(PCB_ERR_INVALID, "input dtype must be F32, F16 or BF16");
-}
 
 // ---------------------------------------------------------------------------
 // Grouped quantization (per-block and per-channel rows share this driver).
@@ -266,22 +197,8 @@ int launch_groups(const void* x, int xt, int64_t batch, int64_t m, int64_t n, in
 }
 
 // ---------------------------------------------------------------------------
-// TMA descriptors (driver entry point fetched through the runtime, so the
-// library does not link libcuda directly).
+// TMA descriptors.
 // ---------------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaDriverEntryPointQueryResult q;
-    void* p = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
 // 3-D uint8 map (inner, outer, batch) with a 128-byte swizzled box (128, box_outer, 1).
 bool make_map_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t batch,
                  uint64_t outer_stride, uint64_t batch_stride, uint32_t box_outer) {
@@ -534,6 +451,9 @@ int pcb_get_device_error(int* code, int* site, int* info) {
   const unsigned int zero[3] = {0, 0, 0};
   if (cudaMemcpyToSymbol(pcb::g_device_error, zero, sizeof(zero)) != cudaSuccess)
     return check_launch("pcb_get_device_error clear");
+  unsigned int loss[3] = {0, 0, 0};
+  if (take_loss_device_error(loss) != cudaSuccess) return check_launch("pcb_get_device_error read");
+  if (h[0] == 0) std::memcpy(h, loss, sizeof(h));
   if (code) *code = (int)h[0];
   if (site) *site = (int)h[1];
   if (info) *info = (int)h[2];

@@ -1,0 +1,164 @@
+// C entry points of the root-mean-square norm.
+#include <algorithm>
+
+#include "host.cuh"
+#include "rms_norm.cuh"
+
+using namespace pcb;
+
+namespace {
+
+bool fits_units(const void* p, int64_t row_stride, int es) {
+  return aligned(p, 16) && (row_stride * es) % 16 == 0;
+}
+
+template <int XT, int YT, int LANES, int NV>
+int launch_norm_fwd(const norm::FwdArgs& p, cudaStream_t s) {
+  constexpr int threads = LANES > 32 ? LANES : 256, rows = threads / LANES;
+  const int64_t grid = (p.rows + rows - 1) / rows;
+  norm::rms_norm_fwd_kernel<XT, YT, LANES, NV><<<(unsigned)grid, threads, 0, s>>>(p);
+  return check_launch("rms_norm_fwd_kernel");
+}
+
+// Lanes per row: four units of eight elements a lane keep a row in registers
+// at 32 values a thread; rows up to 1024 wide need no barrier.
+template <int XT, int YT>
+int dispatch_norm_fwd(const norm::FwdArgs& p, bool vec, cudaStream_t s) {
+  const int units = p.dim / norm::kUnit;
+  if (vec && units <= 4096) {
+    if (units <= 32) return launch_norm_fwd<XT, YT, 32, 1>(p, s);
+    if (units <= 64) return launch_norm_fwd<XT, YT, 32, 2>(p, s);
+    if (units <= 128) return launch_norm_fwd<XT, YT, 32, 4>(p, s);
+    if (units <= 256) return launch_norm_fwd<XT, YT, 128, 2>(p, s);
+    if (units <= 512) return launch_norm_fwd<XT, YT, 256, 2>(p, s);
+    if (units <= 1024) return launch_norm_fwd<XT, YT, 256, 4>(p, s);
+    if (units <= 2048) return launch_norm_fwd<XT, YT, 512, 4>(p, s);
+    return launch_norm_fwd<XT, YT, 1024, 4>(p, s);
+  }
+  const int64_t grid = std::min<int64_t>(p.rows, (int64_t)device_info().sm_count * 8);
+  norm::rms_norm_fwd_generic_kernel<XT, YT><<<(unsigned)grid, norm::kGenericThreads, 0, s>>>(p);
+  return check_launch("rms_norm_fwd_generic_kernel");
+}
+
+// CTAs of the backward pass: enough to fill the GPU, and no more rows of dw
+// shares than that.
+int norm_bwd_ctas(int64_t rows, int rows_per_cta) {
+  const int64_t ctas = (rows + rows_per_cta - 1) / rows_per_cta;
+  return (int)std::min<int64_t>(ctas, (int64_t)device_info().sm_count * 4);
+}
+
+constexpr int kNormDwSmem = 160 * 1024;  // dw shares of one CTA of the generic backward
+
+template <int XT, int LANES, int NV>
+int launch_norm_bwd(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
+  constexpr int threads = LANES > 256 ? LANES : 256, rows = threads / LANES;
+  parts = norm_bwd_ctas(p.rows, rows);
+  const int smem = rows > 1 ? p.dim * 4 : 0;  // at most 1024 columns of fp32
+  norm::rms_norm_bwd_kernel<XT, LANES, NV><<<parts, threads, smem, s>>>(p);
+  return check_launch("rms_norm_bwd_kernel");
+}
+
+template <int XT>
+int dispatch_norm_bwd(const norm::BwdArgs& p, bool vec, int& parts, cudaStream_t s) {
+  const int units = p.dim / norm::kUnit;
+  if (vec && units <= 2048) {
+    if (units <= 32) return launch_norm_bwd<XT, 32, 1>(p, parts, s);
+    if (units <= 64) return launch_norm_bwd<XT, 32, 2>(p, parts, s);
+    if (units <= 128) return launch_norm_bwd<XT, 64, 2>(p, parts, s);
+    if (units <= 256) return launch_norm_bwd<XT, 128, 2>(p, parts, s);
+    if (units <= 512) return launch_norm_bwd<XT, 256, 2>(p, parts, s);
+    if (units <= 1024) return launch_norm_bwd<XT, 512, 2>(p, parts, s);
+    return launch_norm_bwd<XT, 1024, 2>(p, parts, s);
+  }
+  parts = norm_bwd_ctas(p.rows, 1);
+  const bool in_smem = (int64_t)p.dim * 4 <= kNormDwSmem;
+  const int smem = in_smem ? p.dim * 4 : 0;
+  auto kernel = norm::rms_norm_bwd_generic_kernel<XT>;
+  if (smem > 48 * 1024) ensure_smem_attr(kernel, smem);
+  kernel<<<parts, norm::kGenericThreads, smem, s>>>(p, in_smem ? 1 : 0);
+  return check_launch("rms_norm_bwd_generic_kernel");
+}
+
+int norm_bad_sizes(int64_t rows, int64_t dim) {
+  if (rows < 0 || dim <= 0) return fail(PCB_ERR_INVALID, "rms norm needs rows >= 0 and dim > 0");
+  if (rows > INT32_MAX || dim > (1 << 26)) return fail(PCB_ERR_UNSUPPORTED, "rms norm: dimension too large");
+  return PCB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pcb_rms_norm_fwd(const void* x, int x_dtype, int64_t rows, int64_t dim, int64_t sx, const void* residual,
+                     int64_t sr, const void* weight, int w_dtype, float eps, void* h, int64_t sh, void* y, int64_t sy,
+                     void* q, int q_dtype, int64_t sq, float* scale, int64_t ssr, int64_t ssb, int quant_mode,
+                     int pow2_scales, float quant_eps, float* rstd, void* stream) {
+  if (int st = norm_bad_sizes(rows, dim)) return st;
+  if (!is_float_in(x_dtype) || !is_float_in(w_dtype)) return fail(PCB_ERR_INVALID, "rms norm: bad dtype");
+  if (quant_mode < norm::kQuantNone || quant_mode > norm::kQuantRow)
+    return fail(PCB_ERR_INVALID, "rms norm: quant_mode must be 0 (none), 1 (1x128 blocks) or 2 (rows)");
+  if (quant_mode != norm::kQuantNone && !is_fp8(q_dtype)) return fail(PCB_ERR_INVALID, "rms norm: q must be E4M3 or E5M2");
+  if (pow2_scales && quant_mode != norm::kQuantBlock)
+    return fail(PCB_ERR_UNSUPPORTED, "rms norm: power-of-two scales go with 1x128 blocks");
+  if (quant_mode == norm::kQuantNone && !y) return fail(PCB_ERR_INVALID, "rms norm: neither y nor q is wanted");
+  if (rows == 0) return PCB_OK;
+  if (!x || !weight || !rstd || (residual && !h) || (quant_mode != norm::kQuantNone && (!q || !scale)))
+    return fail(PCB_ERR_INVALID, "null pointer");
+  const norm::FwdArgs p{x, sx, residual, sr, weight, w_dtype, residual ? h : nullptr, sh, y, sy,
+                        quant_mode == norm::kQuantNone ? nullptr : q, sq, scale, ssr, ssb, rstd, rows, (int)dim, eps,
+                        quant_eps, quant_mode, pow2_scales ? 1 : 0};
+  const int es = elem_size(x_dtype);
+  const bool vec = dim % norm::kUnit == 0 && fits_units(x, sx, es) && (!residual || (fits_units(residual, sr, es) && fits_units(h, sh, es))) &&
+                   aligned(weight, 16) && (!y || fits_units(y, sy, es)) &&
+                   (quant_mode == norm::kQuantNone || (aligned(q, 8) && sq % 8 == 0));
+  return dispatch_xy(x_dtype, quant_mode == norm::kQuantNone ? PCB_DTYPE_E4M3 : q_dtype, [&](auto xc, auto yc) -> int {
+    return dispatch_norm_fwd<decltype(xc)::value, decltype(yc)::value>(p, vec, (cudaStream_t)stream);
+  });
+}
+
+int64_t pcb_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t dim) {
+  if (rows <= 0 || dim <= 0) return 0;
+  return (int64_t)norm_bwd_ctas(rows, 1) * dim * 4;
+}
+
+int pcb_rms_norm_bwd(const void* dy, int64_t sdy, const void* h, int64_t sh, int x_dtype, int64_t rows, int64_t dim,
+                     const void* dh, int64_t sdh, const void* weight, int w_dtype, const float* rstd, void* dx,
+                     int64_t sdx, void* dw, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int st = norm_bad_sizes(rows, dim)) return st;
+  if (!is_float_in(x_dtype) || !is_float_in(w_dtype)) return fail(PCB_ERR_INVALID, "rms norm: bad dtype");
+  if (!dw) return fail(PCB_ERR_INVALID, "null pointer");
+  cudaStream_t s = (cudaStream_t)stream;
+  if (rows == 0) {
+    if (cudaMemsetAsync(dw, 0, (size_t)dim * elem_size(w_dtype), s) != cudaSuccess) return check_launch("rms norm dw");
+    return PCB_OK;
+  }
+  if (!dy || !h || !weight || !rstd || !dx) return fail(PCB_ERR_INVALID, "null pointer");
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < pcb_rms_norm_bwd_workspace_bytes(rows, dim))
+    return fail(PCB_ERR_INVALID, "rms norm workspace too small or misaligned");
+  const norm::BwdArgs p{dy, sdy, h, sh, dh, sdh, weight, w_dtype, rstd, dx, sdx, static_cast<float*>(workspace), rows,
+                        (int)dim};
+  const int es = elem_size(x_dtype);
+  const bool vec = dim % norm::kUnit == 0 && fits_units(dy, sdy, es) && fits_units(h, sh, es) &&
+                   (!dh || fits_units(dh, sdh, es)) && fits_units(dx, sdx, es) && aligned(weight, 16);
+  int parts = 0;
+  int st = x_dtype == PCB_DTYPE_F32   ? dispatch_norm_bwd<PCB_DTYPE_F32>(p, vec, parts, s)
+           : x_dtype == PCB_DTYPE_F16 ? dispatch_norm_bwd<PCB_DTYPE_F16>(p, vec, parts, s)
+                                      : dispatch_norm_bwd<PCB_DTYPE_BF16>(p, vec, parts, s);
+  if (st) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((dim + 31) / 32), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const float* partial = p.partial;
+  if (w_dtype == PCB_DTYPE_F32) cudaLaunchKernelEx(&cfg, norm::rms_norm_dw_kernel<PCB_DTYPE_F32>, partial, parts, (int)dim, dw);
+  else if (w_dtype == PCB_DTYPE_F16) cudaLaunchKernelEx(&cfg, norm::rms_norm_dw_kernel<PCB_DTYPE_F16>, partial, parts, (int)dim, dw);
+  else cudaLaunchKernelEx(&cfg, norm::rms_norm_dw_kernel<PCB_DTYPE_BF16>, partial, parts, (int)dim, dw);
+  return check_launch("rms_norm_dw_kernel");
+}
+
+}  // extern "C"

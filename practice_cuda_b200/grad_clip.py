@@ -1,0 +1,229 @@
+"""Global norm of a model's gradients, and clipping by it.
+
+``norm = sqrt(sum g^2)`` over every tensor given (or the largest magnitude),
+then ``g * min(1, max_norm / (norm + eps))``: two launches for up to 1000
+tensors of mixed types, nothing read back by the host.  The reference trains
+without clipping (``fp8_training/fp8_bench/bench/bench_fsdp2.py:120-187``).
+
+* :func:`grad_norm` -- the norm alone.
+* :func:`clip_grad_norm` -- norm and clipping of a list of tensors, in place
+  or into other tensors.
+* :func:`clip_grad_norm_` -- the gradients of a model's parameters, FSDP2
+  shards included.
+"""
+
+from __future__ import annotations
+
+import math
+from array import array
+from typing import Iterable, Optional, Sequence, Union
+
+import torch
+import torch.distributed as dist
+
+from . import _lib
+
+_NORM_TYPES = {2.0: 0, math.inf: 1}
+_DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _norm_code(norm_type: float, what: str) -> int:
+    try:
+        return _NORM_TYPES[float(norm_type)]
+    except (KeyError, ValueError, TypeError):
+        raise ValueError(f"{what}: norm_type must be 2 or inf, got {norm_type!r}") from None
+
+
+def _as_list(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], what: str) -> list[torch.Tensor]:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        raise ValueError(f"{what}: no tensors (their device is where the norm goes)")
+    device = tensors[0].device
+    for t in tensors:
+        if t.dtype not in _DTYPE_CODES:
+            raise ValueError(f"{what}: gradients must be bf16, fp16 or fp32, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{what}: gradients on {device} and {t.device}")
+    _lib.require_cuda(tensors[0], "gradients")
+    return tensors
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill one stretch of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return (a.is_contiguous() and b.is_contiguous()) or a.stride() == b.stride()
+
+
+class _Table:
+    """The host arrays of one call: pointers, sizes and types."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        self.pointers = array("Q", [t.data_ptr() for t in tensors])
+        self.sizes = array("q", [t.numel() for t in tensors])
+        self.types = array("i", [_DTYPE_CODES[t.dtype] for t in tensors])
+        self.count = len(tensors)
+
+    def args(self) -> tuple[int, int, int]:
+        return self.sizes.buffer_info()[0], self.types.buffer_info()[0], self.count
+
+
+def _workspace(count: int, device: torch.device) -> tuple[torch.Tensor, int]:
+    nbytes = _lib.lib().pcb_grad_norm_workspace_bytes(count)
+    return torch.empty(nbytes, device=device, dtype=torch.uint8), nbytes
+
+
+def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], *, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm over all tensors: a 0-dim fp32 tensor on their device."""
+    what = "grad_norm"
+    code = _norm_code(norm_type, what)
+    tensors = _as_list(tensors, what)
+    device = tensors[0].device
+    with torch.cuda.device(device):
+        # A view whose elements do not fill one stretch of memory is copied.
+        tensors = [t if _dense(t) else t.contiguous() for t in tensors]
+        table = _Table(tensors)
+        norm = torch.empty((), device=device, dtype=torch.float32)
+        workspace, nbytes = _workspace(table.count, device)
+        status = _lib.lib().pcb_grad_norm(table.pointers.buffer_info()[0], *table.args(), code, norm.data_ptr(),
+                                          workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
+        if status:
+            _lib.check(status, "pcb_grad_norm")
+    return norm
+
+
+def _targets(tensors: list[torch.Tensor], out: Optional[Sequence[torch.Tensor]], what: str) -> list[torch.Tensor]:
+    if out is None:
+        out = tensors
+    else:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(out) != len(tensors):
+            raise ValueError(f"{what}: {len(out)} outputs for {len(tensors)} gradients")
+        for t, o in zip(tensors, out):
+            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
+                raise ValueError(f"{what}: an output is {tuple(o.shape)} {o.dtype} on {o.device}, "
+                                 f"its gradient {tuple(t.shape)} {t.dtype} on {t.device}")
+    for o in out:
+        if not _dense(o) and any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+            raise ValueError(f"{what}: cannot write to an expanded tensor of shape {tuple(o.shape)}")
+    return out
+
+
+def clip_grad_norm(
+    tensors: Union[torch.Tensor, Iterable[torch.Tensor]],
+    max_norm: float,
+    *,
+    norm_type: float = 2.0,
+    eps: float = 1e-6,
+    out: Optional[Sequence[torch.Tensor]] = None,
+    error_if_nonfinite: bool = False,
+    group: Optional["dist.ProcessGroup"] = None,
+) -> torch.Tensor:
+    """Scale ``tensors`` by ``min(1, max_norm / (norm + eps))`` and return
+    the norm before it (0-dim fp32, on the device).
+
+    In place, or into ``out`` (one tensor each, of the same shape and type).
+    A non-finite norm makes the gradients NaN or 0, as the product says;
+    ``error_if_nonfinite`` raises instead, before anything is written, and
+    waits for the GPU to know.  With ``group``, the tensors are this process's
+    shards: the norm is that of all processes' shards together.
+    """
+    what = "clip_grad_norm"
+    code = _norm_code(norm_type, what)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"{what}: max_norm must not be negative, got {max_norm}")
+    tensors = _as_list(tensors, what)
+    out = _targets(tensors, out, what)
+    device = tensors[0].device
+    lib = _lib.lib()
+    with torch.cuda.device(device):
+        # Views that do not fill one stretch of memory, or whose output lies in
+        # another order, pass through a contiguous copy.
+        direct = [_dense(t) and _dense(o) and _same_order(t, o) for t, o in zip(tensors, out)]
+        src = [t if d else t.contiguous() for t, d in zip(tensors, direct)]
+        dst = [o if d else torch.empty_like(t) for t, o, d in zip(src, out, direct)]
+        table = _Table(src)
+        targets = array("Q", [t.data_ptr() for t in dst])
+        pointers, targets_at = table.pointers.buffer_info()[0], targets.buffer_info()[0]
+        stream = _lib.stream_ptr(device)
+        if group is None and not error_if_nonfinite:
+            norm = torch.empty((), device=device, dtype=torch.float32)
+            workspace, nbytes = _workspace(table.count, device)
+            status = lib.pcb_grad_clip(pointers, targets_at, *table.args(), code, max_norm, eps, norm.data_ptr(),
+                                       workspace.data_ptr(), nbytes, stream)
+            if status:
+                _lib.check(status, "pcb_grad_clip")
+        else:
+            norm = grad_norm(src, norm_type=norm_type)
+            if group is not None:
+                norm = join_norms(norm, norm_type, group)
+            if error_if_nonfinite and not bool(torch.isfinite(norm)):
+                raise RuntimeError(f"{what}: the gradients' norm is {norm.item()}")
+            status = lib.pcb_grad_scale(pointers, targets_at, *table.args(), norm.data_ptr(), max_norm, eps, stream)
+            if status:
+                _lib.check(status, "pcb_grad_scale")
+        for t, o, d in zip(dst, out, direct):
+            if not d:
+                o.copy_(t)
+    return norm
+
+
+def join_norms(norm: torch.Tensor, norm_type: float, group: Optional["dist.ProcessGroup"]) -> torch.Tensor:
+    """The norm over the shards of every process of ``group`` from each one's own."""
+    if float(norm_type) == math.inf:
+        # NaN has to survive the maximum: processes vote on it beside the value.
+        pair = torch.stack([torch.nan_to_num(norm, nan=0.0, posinf=math.inf), torch.isnan(norm).to(norm.dtype)])
+        dist.all_reduce(pair, op=dist.ReduceOp.MAX, group=group)
+        return torch.where(pair[1] > 0, torch.full_like(pair[0], math.nan), pair[0])
+    squares = norm.double().square()
+    dist.all_reduce(squares, op=dist.ReduceOp.SUM, group=group)
+    return squares.sqrt().to(norm.dtype)
+
+
+def clip_grad_norm_(
+    parameters: Union[torch.Tensor, Iterable[torch.Tensor]],
+    max_norm: float,
+    *,
+    norm_type: float = 2.0,
+    eps: float = 1e-6,
+    error_if_nonfinite: bool = False,
+) -> torch.Tensor:
+    """Clip the gradients of ``parameters`` in place by their global norm.
+
+    Parameters without a gradient are left out.  DTensor gradients (FSDP2
+    shards) are clipped shard by shard and their norm is joined over the
+    device mesh they share; mixing sharded and plain gradients, several
+    meshes, or gradients that are not sharded over the whole mesh is refused.
+    """
+    what = "clip_grad_norm_"
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    locals_, group = _local_shards(grads, what)
+    return clip_grad_norm(locals_, max_norm, norm_type=norm_type, eps=eps, error_if_nonfinite=error_if_nonfinite,
+                          group=group)
+
+
+def _local_shards(grads: list[torch.Tensor], what: str):
+    from torch.distributed.tensor import DTensor, Shard
+
+    sharded = [g for g in grads if isinstance(g, DTensor)]
+    if not sharded:
+        return grads, None
+    mesh = sharded[0].device_mesh
+    if len(sharded) != len(grads) or any(g.device_mesh != mesh for g in sharded):
+        raise ValueError(f"{what}: gradients must all be sharded over one device mesh, or all be plain tensors")
+    if mesh.ndim != 1 or any(not isinstance(g.placements[0], Shard) for g in sharded):
+        raise ValueError(f"{what}: sharded gradients need a one-dimensional mesh and a Shard placement")
+    return [g.to_local() for g in sharded], mesh.get_group()

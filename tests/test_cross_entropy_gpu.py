@@ -1,0 +1,336 @@
+"""The output projection's cross entropy against plain 64-bit arithmetic.
+
+Tolerances.  A logit is a fp32 tensor-core sum of `dim` exact products, added
+16 at a time; each addition is off by at most 2^-23 of the running sum, itself
+at most |x| |w|: LOGIT = (dim / 16 + 8) 2^-23 |x| |w|.  A loss is the
+difference of two such values plus a few fp32 roundings (RTOL32 of the
+logits' size).  G is rounded once to the inputs' type (UNIT) after an
+exponential that is off by 2 LOGIT + RTOL32; the products of G with weight and x
+add (terms / 16 + 8) 2^-23 of the magnitudes summed, and the gradient is
+rounded once more."""
+
+import math
+
+import pytest
+import torch
+
+from practice_cuda_b200 import _lib
+from practice_cuda_b200.cross_entropy import linear_cross_entropy
+from tests._util import synthetic
+
+gpu = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+UNIT = {t: torch.finfo(t).eps / 2 for t in (BF16, F16)}
+TINY = {BF16: 2.0 ** -134, F16: 2.0 ** -25}
+RTOL32 = 1e-5
+IGNORE = -100
+
+
+def _inputs(tokens, vocab, dim, dtype, seed=0, ignored=0.0, scale=1.0):
+    x = synthetic((tokens, dim), std=scale, seed=seed, dtype=dtype).cuda()
+    w = synthetic((vocab, dim), std=1.0 / math.sqrt(dim), seed=seed + 1, dtype=dtype).cuda()
+    g = torch.Generator().manual_seed(seed + 2)
+    target = torch.randint(0, vocab, (tokens,), generator=g)
+    target[torch.rand(tokens, generator=g) < ignored] = IGNORE
+    return x, w, target.cuda()
+
+
+def _reference(x, w, target, reduction, dloss):
+    """loss, dx, dw in 64 bits, and how far each may be off."""
+    tokens, dim = x.shape
+    vocab = w.shape[0]
+    unit, tiny = UNIT[x.dtype], TINY[x.dtype]
+    x64, w64 = x.double(), w.double()
+    valid = target != IGNORE
+    logits = x64 @ w64.t()
+    lse = torch.logsumexp(logits, 1)
+    at = torch.where(valid, target, 0)
+    nll = torch.where(valid, lse - logits.gather(1, at[:, None])[:, 0], 0.0)
+    add = 2.0 ** -23
+    logit = (dim / 16 + 8) * add * x64.norm(dim=1) * w64.norm(dim=1).max()
+    nll_off = torch.where(valid, 2 * logit + RTOL32 * (1 + lse.abs() + logits.abs().amax(1)), 0.0)
+    count = valid.sum()
+    share = torch.where(valid, dloss.double() / (count if reduction == "mean" else 1), 0.0)
+    if reduction == "none":
+        loss, loss_off = nll, nll_off
+    else:
+        div = count if reduction == "mean" else 1
+        loss, loss_off = nll.sum() / div, nll_off.sum() / div
+    p = torch.exp(logits - lse[:, None])
+    onehot = torch.zeros_like(p).scatter_(1, at[:, None], 1.0)
+    g = (p - onehot) * share[:, None]
+    g_off = (p * (2 * logit + RTOL32)[:, None] + unit * (p - onehot).abs()) * share.abs()[:, None]
+    dx, dw = g @ w64, g.t() @ x64
+    dx_off = g_off @ w64.abs() + ((vocab / 16 + 8) * add) * (g.abs() @ w64.abs())
+    dw_off = g_off.t() @ x64.abs() + ((tokens / 16 + 8) * add) * (g.abs().t() @ x64.abs())
+    return (loss, loss_off), (dx, unit * dx.abs() + 1.01 * dx_off + tiny), (dw, unit * dw.abs() + 1.01 * dw_off + tiny)
+
+
+def _within(actual, expected, off, what):
+    assert actual.shape == expected.shape, f"{what}: {tuple(actual.shape)} for {tuple(expected.shape)}"
+    d = (actual.double() - expected).abs()
+    assert bool((d <= off).all()), f"{what}: off by {d.max().item():.3e}, worst ratio {(d / off).max().item():.2f}"
+
+
+def _check(x, w, target, reduction="mean", piece=None, dloss=None, what=""):
+    if dloss is None:
+        dloss = torch.rand(target.shape, generator=torch.Generator().manual_seed(1)).cuda() + 0.5
+        dloss = dloss if reduction == "none" else torch.tensor(1.0 if x.dtype == BF16 else 64.0, device="cuda")
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = linear_cross_entropy(x, w, target, reduction=reduction, vocab_piece=piece)
+    assert loss.dtype == torch.float32
+    dx, dw = torch.autograd.grad(loss, (x, w), dloss)
+    expected = _reference(x.detach(), w.detach(), target, reduction, dloss)
+    for got, (value, off), name in zip((loss, dx, dw), expected, ("loss", "dx", "dw")):
+        _within(got.detach(), value, off, f"{what} {name}")
+    assert dx.dtype == x.dtype and dw.dtype == w.dtype
+    assert _lib.device_error()[0] == 0
+    return loss.detach(), dx, dw
+
+
+SHAPES = [
+    (1, 1, 8), (1, 2, 16), (3, 127, 64), (2, 128, 72), (7, 129, 136), (128, 256, 64), (129, 257, 128), (256, 512, 256),
+    (300, 1000, 200), (257, 4099, 520), (1000, 777, 1024), (1, 40000, 256), (33, 20011, 512), (600, 300, 8),
+    (5, 300, 1), (6, 301, 7), (130, 259, 65), (40, 1001, 333),  # widths that are not multiples of 16 bytes
+]
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,dim", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_shapes(tokens, vocab, dim, dtype):
+    x, w, target = _inputs(tokens, vocab, dim, dtype, seed=tokens + vocab + dim)
+    _check(x, w, target, "mean", what="mean")
+    _check(x, w, target, "none", what="none")
+    _check(x, w, target, "sum", what="sum")
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,dim", [(300, 1000, 200), (64, 2500, 128), (520, 4099, 264), (31, 777, 77)])
+@pytest.mark.parametrize("piece", [1, 256, 700, 1024, 10 ** 9])
+def test_pieces_of_the_vocabulary(tokens, vocab, dim, piece):
+    x, w, target = _inputs(tokens, vocab, dim, BF16, seed=piece % 97, ignored=0.2)
+    _check(x, w, target, "mean", piece=piece)
+    _check(x, w, target, "none", piece=piece)
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_ignored_tokens(reduction, dtype):
+    x, w, target = _inputs(400, 900, 192, dtype, seed=5, ignored=0.4)
+    loss, dx, _ = _check(x, w, target, reduction)
+    left_out = target == IGNORE
+    assert int(dx[left_out].count_nonzero()) == 0
+    if reduction == "none":
+        assert int(loss[left_out].count_nonzero()) == 0
+    # What stands in the rows that are left out does not reach the others.
+    other = x.clone()
+    other[left_out] *= 1000.0
+    loss2, dx2, _ = _check(other, w, target, reduction, what="large rows left out")
+    assert torch.equal(loss, loss2) and torch.equal(dx, dx2)
+
+
+@gpu
+def test_every_token_ignored():
+    x, w, target = _inputs(70, 300, 64, BF16, seed=6)
+    target.fill_(IGNORE)
+    x.requires_grad_(), w.requires_grad_()
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(x, w, target, reduction=reduction)
+        reference = torch.nn.functional.cross_entropy((x.float() @ w.float().t()).detach(), target, reduction=reduction)
+        assert torch.equal(loss.detach(), reference) or (math.isnan(loss.item()) and math.isnan(reference.item()))
+        dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+        assert int(dx.count_nonzero()) == 0 and int(dw.count_nonzero()) == 0
+
+
+@gpu
+def test_sure_and_hopeless_tokens():
+    x, w, target = _inputs(256, 512, 128, BF16, seed=7)
+    lean = w[target].float() * torch.linspace(-60, 60, 256, device="cuda")[:, None]
+    loss, _, _ = _check((x.float() + lean).bfloat16(), w, target, "none")
+    assert loss.max().item() > 30 and loss.min().item() < 1e-6 and loss.min().item() >= 0
+
+
+@gpu
+def test_large_and_non_finite_logits():
+    x, w, target = _inputs(200, 600, 64, BF16, seed=8, scale=200.0)  # logits of several hundreds
+    _check(x, w, target, "mean")
+    x, w, target = _inputs(200, 600, 64, BF16, seed=9)
+    clean = linear_cross_entropy(x, w, target, reduction="none")
+    x[3, 5], x[150, 1] = float("nan"), float("inf")
+    loss = linear_cross_entropy(x, w, target, reduction="none")
+    bad = torch.zeros(200, dtype=torch.bool, device="cuda")
+    bad[3] = bad[150] = True
+    assert bool(torch.isnan(loss[bad]).all()) and torch.equal(loss[~bad], clean[~bad])
+    assert math.isnan(linear_cross_entropy(x, w, target).item())
+
+
+@gpu
+@pytest.mark.parametrize("spread", [1e-12, 1.0, 1e6])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_weights_of_the_losses(spread, dtype):
+    x, w, target = _inputs(150, 700, 96, dtype, seed=10, ignored=0.1)
+    dloss = synthetic((150,), seed=11, dtype=torch.float32).cuda() * (spread if dtype == BF16 else min(spread, 1e3))
+    dloss[7] = 0.0
+    _check(x, w, target, "none", dloss=dloss)
+    _check(x, w, target, "none", dloss=torch.zeros_like(dloss))
+
+
+@gpu
+def test_layouts_and_shapes_of_the_arguments():
+    x, w, target = _inputs(24, 300, 128, BF16, seed=12)
+    plain = _check(x, w, target, "none")
+    wide = torch.zeros(24, 200, device="cuda", dtype=BF16)
+    for start in (0, 8, 3):  # rows of a wider tensor, 16-byte aligned or not
+        view = wide[:, start : start + 128]
+        view.copy_(x)
+        for a, b in zip(_check(view, w, target, "none"), plain):
+            assert torch.equal(a, b)
+    wt = w.t().contiguous().t()  # columns contiguous
+    for a, b in zip(_check(x, wt, target, "none"), plain):
+        assert torch.equal(a, b)
+    x3, t2 = x.view(2, 12, 128).requires_grad_(), target.view(2, 12).int()
+    loss = linear_cross_entropy(x3, w, t2, reduction="none")
+    assert loss.shape == (2, 12) and torch.equal(loss.detach().view(24), plain[0])
+    assert torch.autograd.grad(loss.sum(), x3)[0].shape == x3.shape
+    same = x[:1].expand(24, 128)  # one row for every token
+    _check(same, w, target, "mean", what="expanded")
+
+
+@gpu
+def test_only_the_gradients_that_are_needed():
+    x, w, target = _inputs(140, 900, 128, BF16, seed=13)
+    _, dx, dw = _check(x, w, target)
+    x.requires_grad_()
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, w, target), x)[0], dx)
+    x.requires_grad_(False), w.requires_grad_()
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, w, target), w)[0], dw)
+    with torch.no_grad():
+        assert not linear_cross_entropy(x, w, target).requires_grad
+
+
+@gpu
+def test_no_tokens():
+    w = torch.ones(10, 16, device="cuda", dtype=BF16, requires_grad=True)
+    x = torch.empty(0, 16, device="cuda", dtype=BF16, requires_grad=True)
+    target = torch.empty(0, device="cuda", dtype=torch.int64)
+    assert math.isnan(linear_cross_entropy(x, w, target).item())
+    loss = linear_cross_entropy(x, w, target, reduction="sum")
+    assert loss.item() == 0.0
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert dx.shape == (0, 16) and int(dw.count_nonzero()) == 0
+    assert linear_cross_entropy(x, w, target, reduction="none").shape == (0,)
+
+
+@gpu
+def test_target_outside_the_vocabulary_is_reported():
+    x, w, target = _inputs(100, 300, 64, BF16, seed=14)
+    assert _lib.device_error()[0] == 0
+    for bad in (300, -1, 1 << 40, -(1 << 40)):
+        t = target.clone()
+        t[9] = bad
+        loss = linear_cross_entropy(x, w, t, reduction="none")
+        assert math.isnan(loss[9].item()) and int(torch.isnan(loss).sum()) == 1
+        code, site, _ = _lib.device_error()
+        assert code == _lib.PCB_ERR_INVALID and site == 19
+        xg = x.clone().requires_grad_()
+        dx = torch.autograd.grad(linear_cross_entropy(xg, w, t), xg)[0]
+        assert bool(torch.isnan(dx[9]).all()) and int(torch.isnan(dx).any(1).sum()) == 1
+        assert _lib.device_error()[0] == _lib.PCB_ERR_INVALID and _lib.device_error()[0] == 0
+
+
+@gpu
+def test_gradient_against_differences():
+    """Central differences along directions of +-1/16 steps.
+
+    x holds multiples of 1/8 below 4 and w multiples of 1/64 below 1/2, so
+    both steps are exact in fp16.  A step moves a logit by about
+    sqrt(dim) / 16 * |w| = 0.1: the cubic term is below 2e-3 of the slope's
+    terms, G and the gradients are rounded to 2^-11, and the two losses'
+    roundings (1e-5 of their size) are divided by the step's 1/8."""
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randint(-16, 16, (6, 64), generator=g) / 8).to(F16).cuda().requires_grad_()
+    w = (torch.randint(-16, 16, (50, 64), generator=g) / 64).to(F16).cuda().requires_grad_()
+    target = torch.randint(0, 50, (6,), generator=g).cuda()
+    dx, dw = torch.autograd.grad(linear_cross_entropy(x, w, target, reduction="sum"), (x, w))
+    for k, (t, grad, step) in enumerate(((x, dx, 1 / 16), (w, dw, 1 / 256))):
+        for _ in range(4):
+            v = (torch.randint(0, 2, tuple(t.shape), generator=g).cuda() * 2 - 1).to(F16)
+            ends = []
+            for sign in (1, -1):
+                moved = t.detach() + sign * step * v
+                assert torch.equal((moved - t.detach()).double(), sign * step * v.double())
+                args = (moved, w) if k == 0 else (x, moved)
+                ends.append(linear_cross_entropy(*(a.detach() for a in args), target, reduction="none").double().sum())
+            slope = (ends[0] - ends[1]) / (2 * step)
+            inner = (grad.double() * v.double()).sum()
+            terms = grad.double().norm() * math.sqrt(grad.numel())
+            assert abs(inner - slope).item() <= 4e-3 * terms.item() + 1e-5 * ends[0].abs().item() / (2 * step)
+
+
+@gpu
+def test_repeatability_stream_and_graph():
+    x, w, target = _inputs(500, 3000, 256, BF16, seed=15)
+    first = _check(x, w, target, "mean")
+    for _ in range(3):
+        for a, b in zip(_check(x, w, target, "mean"), first):
+            assert torch.equal(a, b)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    with torch.cuda.stream(stream):
+        loss = linear_cross_entropy(xg, wg, target)
+        grads = torch.autograd.grad(loss, (xg, wg))
+    stream.synchronize()
+    for a, b in zip((loss, *grads), first):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = linear_cross_entropy(x, w, target)
+    x.copy_(x.flip(0))
+    target.copy_(target.flip(0))
+    graph.replay()
+    assert abs(captured.item() - first[0].item()) <= 1e-6 * first[0].item()
+
+
+@gpu
+def test_refusals():
+    x, w, target = _inputs(8, 32, 16, BF16, seed=16)
+    for bad in (
+        lambda: linear_cross_entropy(x.float(), w.float(), target),
+        lambda: linear_cross_entropy(x, w.half(), target),
+        lambda: linear_cross_entropy(x, w[:, :8], target),
+        lambda: linear_cross_entropy(x, w[:0], target),
+        lambda: linear_cross_entropy(x, w, target[:4]),
+        lambda: linear_cross_entropy(x, w, target.float()),
+        lambda: linear_cross_entropy(x, w, target.cpu()),
+        lambda: linear_cross_entropy(x, w, target, reduction="batch"),
+        lambda: linear_cross_entropy(x, w, target, vocab_piece=0),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_refuses_cpu_tensors():
+    with pytest.raises(ValueError, match="CUDA"):
+        linear_cross_entropy(torch.ones(2, 8).bfloat16(), torch.ones(4, 8).bfloat16(), torch.zeros(2, dtype=torch.int64))
+
+
+def test_entry_points_reject_bad_arguments_without_gpu():
+    lib = _lib.lib()
+
+    def forward(dtype=2, tokens=4, vocab=8, dim=16, sx=16, reduction=2, x=256, ws=256, nbytes=1 << 30):
+        return lib.pcb_linear_ce_fwd(x, sx, 256, 16, dtype, tokens, vocab, dim, 256, IGNORE, reduction, 256, 256, 256,
+                                     ws, nbytes, None)
+
+    for kwargs in ({"dtype": 0}, {"dtype": 3}, {"tokens": -1}, {"vocab": 0}, {"dim": 0}, {"reduction": 3}, {"x": None},
+                   {"ws": None}, {"ws": 16}, {"nbytes": 8}):
+        assert forward(**kwargs) == _lib.PCB_ERR_INVALID, kwargs
+    assert forward(tokens=0) == _lib.PCB_OK
+    assert forward(sx=17) == _lib.PCB_ERR_LAYOUT and forward(x=264) == _lib.PCB_ERR_LAYOUT
+    assert forward(vocab=1 << 40) == _lib.PCB_ERR_UNSUPPORTED
+    need = lib.pcb_linear_ce_bwd_workspace_bytes(4096, 32000, 4096, 0, 1)
+    # one piece of G (at most 128 MiB) and dX's accumulators, not the logits of the whole vocabulary
+    assert need < (128 << 20) + 4096 * 4096 * 4 + (1 << 20)
