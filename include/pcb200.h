@@ -388,12 +388,13 @@ int64_t pcb_linear_ce_fwd_workspace_bytes(int64_t tokens, int64_t vocab);
  * token's loss and gradients NaN and is reported through
  * pcb_get_device_error().  Logits, statistics and sums are fp32.
  * Writes loss ([tokens], or one value: the sum, or the mean over the tokens
- * that are not left out, NaN if there are none), lse [tokens] and count [1]
+ * that are not left out, NaN if there are none), stats [2, tokens] (each
+ * token's largest logit, and log2 of sum_j exp(l_ij - that)) and count [1]
  * (those tokens), which the backward pass reads.  tokens == 0 writes nothing.
  */
 int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
-                      float* loss, float* lse, float* count, void* workspace, int64_t workspace_bytes, void* stream);
+                      float* loss, float* stats, float* count, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_bwd; piece and
  * want_dx as there. */
@@ -409,7 +410,7 @@ int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t
  */
 int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
-                      const float* lse, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
+                      const float* stats, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
                       int64_t sdw, int64_t piece, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -67,15 +67,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
         lib = _lib.lib()
         with torch.cuda.device(device):
             loss = torch.empty(tokens if reduction == 0 else (), device=device, dtype=torch.float32)
-            stats = torch.empty(tokens + 1, device=device, dtype=torch.float32)  # lse, count
+            stats = torch.empty(2 * tokens + 1, device=device, dtype=torch.float32)  # [2, tokens], count
             if tokens == 0:
                 loss.fill_(float("nan") if reduction == 2 else 0.0)
             nbytes = lib.pcb_linear_ce_fwd_workspace_bytes(tokens, vocab)
             workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
-            lse = stats.data_ptr()
+            at = stats.data_ptr()
             status = lib.pcb_linear_ce_fwd(
                 x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x.dtype], tokens, vocab, dim,
-                target.data_ptr(), ignore_index, reduction, loss.data_ptr(), lse, lse + 4 * tokens,
+                target.data_ptr(), ignore_index, reduction, loss.data_ptr(), at, at + 8 * tokens,
                 workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
             if status:
                 _lib.check(status, "pcb_linear_ce_fwd")
@@ -98,10 +98,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
             dw = torch.empty((vocab, dim), device=device, dtype=x2.dtype) if want_dw else None
             nbytes = lib.pcb_linear_ce_bwd_workspace_bytes(tokens, vocab, dim, piece, int(want_dx))
             workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
-            lse = stats.data_ptr()
+            at = stats.data_ptr()
             status = lib.pcb_linear_ce_bwd(
                 x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x2.dtype], tokens, vocab, dim,
-                target.data_ptr(), ignore_index, reduction, lse, lse + 4 * tokens, dloss.data_ptr(),
+                target.data_ptr(), ignore_index, reduction, at, at + 8 * tokens, dloss.data_ptr(),
                 dx.data_ptr() if want_dx else None, dim, dw.data_ptr() if want_dw else None, dim, piece,
                 workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
             if status:

@@ -165,7 +165,9 @@ loss::Params base_params(int dtype, int64_t vocab, const int64_t* target, int64_
   p.target = reinterpret_cast<const long long*>(target);
   p.ignore_index = ignore_index;
   p.vocab = vocab;
-  p.grad_scale = dtype == PCB_DTYPE_BF16 ? 1.f : 16384.f;
+  // Keeps the small entries of G (1 / vocab and less) off the 16-bit types'
+  // subnormals; at most 2^14 itself, within fp16.
+  p.grad_scale = 16384.f;
   return p;
 }
 
@@ -189,11 +191,11 @@ int64_t pcb_linear_ce_fwd_workspace_bytes(int64_t tokens, int64_t vocab) {
 
 int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
-                      float* loss_out, float* lse, float* count, void* workspace, int64_t workspace_bytes,
+                      float* loss_out, float* stats, float* count, void* workspace, int64_t workspace_bytes,
                       void* stream) {
   if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
   if (tokens == 0) return PCB_OK;
-  if (!target || !loss_out || !lse || !count) return fail(PCB_ERR_INVALID, "null pointer");
+  if (!target || !loss_out || !stats || !count) return fail(PCB_ERR_INVALID, "null pointer");
   const FwdPlan plan(tokens, vocab);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
     return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
@@ -211,7 +213,7 @@ int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw,
   p.ticket = reinterpret_cast<unsigned*>(ws + plan.ticket);
   if (int st = launch_product<loss::kStats>(p, s)) return st;
   loss::RowArgs r{p.partial, p.target_logit, p.target, ignore_index, vocab, (int)tokens, 2 * q.n_blocks, reduction,
-                  lse, loss_out, count, reinterpret_cast<double*>(ws + plan.sums), p.ticket};
+                  stats, loss_out, count, reinterpret_cast<double*>(ws + plan.sums), p.ticket};
   return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), 256, s, r);
 }
 
@@ -222,7 +224,7 @@ int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t
 
 int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
-                      const float* lse, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
+                      const float* stats, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
                       int64_t sdw, int64_t piece, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
   cudaStream_t s = (cudaStream_t)stream;
@@ -232,7 +234,7 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     return PCB_OK;
   }
   if (!dx && !dw) return PCB_OK;
-  if (!target || !lse || !count || !dloss) return fail(PCB_ERR_INVALID, "null pointer");
+  if (!target || !stats || !count || !dloss) return fail(PCB_ERR_INVALID, "null pointer");
   const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
     return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
@@ -241,7 +243,7 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
   void* g = ws + plan.g;
   float4* acc = reinterpret_cast<float4*>(ws + plan.acc);
   loss::Params base = base_params(dtype, vocab, target, ignore_index);
-  base.lse = lse;
+  base.stats = stats;
   if (reduction == loss::kNone) {
     float* row_weight = reinterpret_cast<float*>(ws + plan.weight);
     float* alpha = reinterpret_cast<float*>(ws + plan.alpha);

@@ -1,8 +1,8 @@
 // Softmax cross entropy of an output projection without its logits.
 //
-//   l = X W^T (X [tokens, dim], W [vocab, dim]),  lse_i = log sum_j exp(l_ij),
-//   nll_i = lse_i - l_i,target
-//   G_ij = (exp(l_ij - lse_i) - [j = target_i]) w_i,  dX = a G W,  dW = a G^T X
+//   l = X W^T (X [tokens, dim], W [vocab, dim]),
+//   m_i = max_j l_ij, s_i = sum_j exp(l_ij - m_i), nll_i = (m_i - l_i,target) + log s_i
+//   G_ij = (exp(l_ij - m_i) / s_i - [j = target_i]) w_i,  dX = a G W,  dW = a G^T X
 //
 // One tcgen05 product kernel in three forms:
 //   kStats     a tile of logits leaves the tensor memory as the maximum and the
@@ -14,7 +14,9 @@
 //              order of 1 and the loss's scale stays in fp32).
 //   kProducts  dX += G W and dW = G^T X of that piece in one launch: the tiles
 //              of both share the grid, so neither leaves SMs idle at its end.
-// Logits, softmax statistics and every sum are fp32; tiles are 256 x 256 on a
+// Logits, softmax statistics and every sum are fp32 (m and log2 s are kept apart:
+// their sum would lose the small part of a sure token's probability beside a large
+// logit); tiles are 256 x 256 on a
 // CTA pair (cta_group::2), 64-deep stages of 128-byte swizzled operands by TMA,
 // two accumulators of 256 fp32 columns in tensor memory, so that a tile's
 // epilogue runs under the next tile's products.  Bound by the tensor cores.
@@ -76,7 +78,7 @@ struct Params {
   const long long* target;
   long long ignore_index;
   long long vocab;
-  const float* lse;
+  const float* stats;       // [2][m]: m_i and log2 s_i
   const float* row_weight;  // null: 1
   float grad_scale;         // power of two that G carries
   int col0;                 // first vocabulary column of the piece
@@ -109,9 +111,18 @@ __device__ __forceinline__ void umma_f16_pair_elect(uint32_t d_tmem, uint32_t a_
       : "memory");
 }
 
+// Terms below 2^-126 count as zero: beside a sum of at least 1.
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// With results below 2^-126 kept: a column that no token is likely to take has
+// nothing but such entries in G, and its gradient is theirs.
+__device__ __forceinline__ float exp2_subnormal(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -339,12 +350,13 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
       const bool in = row < q.m;
       // Row values are read before the wait, so their latency is hidden.
       long long target = -1;
-      float lse = 0.f, weight = 0.f;
+      float top = 0.f, log2_sum = 0.f, weight = 0.f;
       if (MODE != kProducts && in) {
         target = p.target[row];
         const bool valid = target != p.ignore_index;
         if (MODE == kGradient && valid) {
-          lse = p.lse[row];
+          top = p.stats[row];
+          log2_sum = p.stats[q.m + row];
           weight = p.grad_scale * (p.row_weight ? p.row_weight[row] : 1.f);
           if (target < 0 || target >= p.vocab) weight = NAN;  // no such column
         }
@@ -415,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
             const int cc = col0 + c * 32;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              u[i] = __float_as_uint(exp2_approx((__uint_as_float(u[i]) - lse) * kLog2e));
+              u[i] = __float_as_uint(exp2_subnormal(fmaf(__uint_as_float(u[i]) - top, kLog2e, -log2_sum)));
             if (target >= cc && target < cc + 32) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
@@ -471,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
 }
 
 // ---------------------------------------------------------------------------
-// The rows' statistics joined: lse, the losses and their reduction.  A CTA
+// The rows' statistics joined, the losses and their reduction.  A CTA
 // takes 32 tokens, its eight warps a strided eighth of the partials each.
 // ---------------------------------------------------------------------------
 enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
@@ -482,7 +494,7 @@ struct RowArgs {
   const long long* target;
   long long ignore_index, vocab;
   int tokens, parts, reduction;
-  float* lse;       // [tokens]
+  float* stats;     // [2][tokens]
   float* loss;      // [tokens] or [1]
   float* count;     // [1], tokens that are not left out
   double* sums;     // [gridDim.x][2]
@@ -518,8 +530,9 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const RowArgs p) {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += ss[i][lane] * exp2f((ms[i][lane] - base) * kLog2e);
-    const float log_sum = logf(sum), lse = base + log_sum;
-    p.lse[row] = lse;
+    const float log_sum = logf(sum);
+    p.stats[row] = base;
+    p.stats[p.tokens + row] = log2f(sum);
     const long long t = p.target[row];
     float v = 0.f;
     if (t != p.ignore_index) {
