@@ -26,33 +26,86 @@ bool make_map(CUtensorMap* map, const void* base, int dt, int64_t inner, int64_t
 bool load_map(CUtensorMap* map, const void* base, int dt, int64_t inner, int64_t outer, int64_t stride, int box_outer) {
   return make_map(map, base, dt, inner, outer, stride, box_outer, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
+// An MN-major operand as (64 elements, K rows, slabs of 64 elements): one load
+// brings both slabs of a 128-wide tile side by side.  Whole slabs only: the
+// last one must lie within the row's stride.
+bool slab_map(CUtensorMap* map, const void* base, int dt, int64_t slabs, int64_t rows, int64_t stride) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)slabs};
+  const cuuint64_t strides[2] = {(cuuint64_t)stride * 2, 128};
+  const cuuint32_t box[3] = {64, loss::BK, 2};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, dt == PCB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// B of a product of G: [rows, dim], dim contiguous.
+bool load_b(loss::Problem& q, const void* base, int dt, int64_t dim, int64_t rows, int64_t stride) {
+  q.b_slabs = dim % 64 == 0 ? 1 : 0;
+  return q.b_slabs ? slab_map(&q.b, base, dt, dim / 64, rows, stride) : load_map(&q.b, base, dt, dim, rows, stride, loss::BK);
+}
 bool store_map(CUtensorMap* map, void* base, int dt, int64_t inner, int64_t outer, int64_t stride) {
   return make_map(map, base, dt, inner, outer, stride, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE);
 }
 
 constexpr int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <int MODE>
-int launch_product(const loss::Params& p, cudaStream_t s) {
-  auto kernel = loss::vocab_product_kernel<MODE>;
-  ensure_smem_attr(kernel, loss::SMEM_ALLOC);
+template <int MODE, bool PAIR>
+int launch_product_as(const loss::Params& p, cudaStream_t s) {
+  auto kernel = loss::vocab_product_kernel<MODE, PAIR>;
+  if constexpr (MODE != loss::kProducts) {
+    // These kernels re-split their registers with setmaxnreg, which is only
+    // valid when the launch holds exactly kLaunchRegs per thread (otherwise
+    // setmaxnreg.inc could never be satisfied).
+    static const int num_regs = [&] {
+      cudaFuncAttributes fa{};
+      return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : -1;
+    }();
+    if (num_regs != loss::kLaunchRegs)
+      return fail(PCB_ERR_UNSUPPORTED, "cross entropy kernel register count differs from its setmaxnreg split");
+  }
+  constexpr int smem = loss::Smem<PAIR>::ALLOC;
+  ensure_smem_attr(kernel, smem);
+  const int sms = device_info().sm_count;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * std::min(p.num_tiles, device_info().sm_count / 2)), 1, 1);
+  cfg.gridDim = dim3((unsigned)(PAIR ? 2 * std::min(p.num_tiles, sms / 2) : std::min(p.num_tiles, sms)), 1, 1);
   cfg.blockDim = dim3(loss::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = loss::SMEM_ALLOC;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
   // griddepcontrol.wait precedes every global access of the kernel.
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = PAIR ? 2 : 1;
   cudaLaunchKernelEx(&cfg, kernel, p);
   return check_launch("vocab_product_kernel");
+}
+
+// Up to 128 tokens a CTA has a tile to itself.
+bool on_pairs(int64_t tokens) { return tokens > loss::BM; }
+
+template <int MODE>
+int launch_product(const loss::Params& p, bool pair, cudaStream_t s) {
+  if constexpr (MODE != loss::kProducts)
+    if (!pair) return launch_product_as<MODE, false>(p, s);
+  return launch_product_as<MODE, true>(p, s);
+}
+
+// Columns of a logit tile.  On single CTAs: the vocabulary in as few rounds
+// over the SMs as 256-column tiles need, and evenly so (a multiple of 16, the
+// step of the instruction's N).
+int logit_tile(int64_t tokens, int64_t vocab) {
+  if (on_pairs(tokens)) return loss::TILE;
+  const int64_t sms = std::max(1, device_info().sm_count);
+  const int64_t rounds = up(vocab, sms * loss::TILE);
+  return (int)std::max<int64_t>(32, up(up(vocab, sms * rounds), 16) * 16);
 }
 
 template <typename K, typename... A>
@@ -71,11 +124,11 @@ int launch_after(K kernel, const char* what, int64_t grid, int threads, cudaStre
 }
 
 // tile counts and K split of a problem
-void shape(loss::Problem& q, int64_t m, int64_t n, int64_t k, int splits) {
+void shape(loss::Problem& q, int64_t m, int64_t n, int64_t k, int splits, bool pair = true, int tile_n = loss::TILE) {
   q.m = (int)m;
   q.n = (int)n;
-  q.m_blocks = (int)up(m, loss::TILE);
-  q.n_blocks = (int)up(n, loss::TILE);
+  q.m_blocks = (int)up(m, pair ? loss::TILE : loss::BM);
+  q.n_blocks = (int)up(n, tile_n);
   q.k_stages = (int)up(k, loss::BK);
   q.split_stages = (int)up(q.k_stages, splits);
   q.splits = (int)up(q.k_stages, q.split_stages);  // none of them empty
@@ -118,7 +171,7 @@ struct FwdPlan {
   int64_t partial, target_logit, sums, ticket, bytes;
   FwdPlan(int64_t tokens, int64_t vocab) {
     Cut c;
-    partial = c.take(up(vocab, loss::TILE) * 2 * tokens * 8);
+    partial = c.take(up(vocab, logit_tile(tokens, vocab)) * 2 * tokens * 8);
     target_logit = c.take(tokens * 4);
     sums = c.take(up(tokens, 32) * 16);
     ticket = c.take(4);
@@ -165,9 +218,6 @@ loss::Params base_params(int dtype, int64_t vocab, const int64_t* target, int64_
   p.target = reinterpret_cast<const long long*>(target);
   p.ignore_index = ignore_index;
   p.vocab = vocab;
-  // Keeps the small entries of G (1 / vocab and less) off the 16-bit types'
-  // subnormals; at most 2^14 itself, within fp16.
-  p.grad_scale = 16384.f;
   return p;
 }
 
@@ -204,17 +254,20 @@ int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw,
   char* ws = static_cast<char*>(workspace);
   loss::Params p = base_params(dtype, vocab, target, ignore_index);
   loss::Problem& q = p.prob[0];
-  if (!load_map(&q.a, x, dtype, dim, tokens, sx, loss::BM) || !load_map(&q.b, weight, dtype, dim, vocab, sw, loss::TILE / 2))
+  const bool pair = on_pairs(tokens);
+  p.tile_n = logit_tile(tokens, vocab);
+  if (!load_map(&q.a, x, dtype, dim, tokens, sx, loss::BM) ||
+      !load_map(&q.b, weight, dtype, dim, vocab, sw, pair ? loss::TILE / 2 : p.tile_n))
     return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-  shape(q, tokens, vocab, dim, 1);
+  shape(q, tokens, vocab, dim, 1, pair, p.tile_n);
   p.num_tiles = q.tiles;
   p.partial = reinterpret_cast<float2*>(ws + plan.partial);
   p.target_logit = reinterpret_cast<float*>(ws + plan.target_logit);
   p.ticket = reinterpret_cast<unsigned*>(ws + plan.ticket);
-  if (int st = launch_product<loss::kStats>(p, s)) return st;
+  if (int st = launch_product<loss::kStats>(p, pair, s)) return st;
   loss::RowArgs r{p.partial, p.target_logit, p.target, ignore_index, vocab, (int)tokens, 2 * q.n_blocks, reduction,
                   stats, loss_out, count, reinterpret_cast<double*>(ws + plan.sums), p.ticket};
-  return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), 256, s, r);
+  return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), loss::kRowWarps * 32, s, r);
 }
 
 int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx) {
@@ -248,7 +301,7 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     float* row_weight = reinterpret_cast<float*>(ws + plan.weight);
     float* alpha = reinterpret_cast<float*>(ws + plan.alpha);
     if (int st = launch_after(loss::loss_weights_kernel, "loss_weights_kernel", 1, 1024, s, dloss, base.target,
-                              (long long)ignore_index, (int)tokens, base.grad_scale, row_weight, alpha))
+                              (long long)ignore_index, (int)tokens, row_weight, alpha))
       return st;
     base.row_weight = row_weight;
     base.alpha = alpha;
@@ -262,24 +315,27 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     bool ok = true;
     loss::Params p = base;
     p.col0 = (int)col0;
+    const bool pair = on_pairs(tokens);
+    p.tile_n = logit_tile(tokens, cols);
     loss::Problem& q = p.prob[0];
     ok &= load_map(&q.a, x, dtype, dim, tokens, sx, loss::BM);
-    ok &= load_map(&q.b, w, dtype, dim, cols, sw, loss::TILE / 2);
+    ok &= load_map(&q.b, w, dtype, dim, cols, sw, pair ? loss::TILE / 2 : p.tile_n);
     ok &= store_map(&q.c_box, g, dtype, cols, tokens, plan.pitch);
-    shape(q, tokens, cols, dim, 1);
-    q.c_tma = 1;
+    shape(q, tokens, cols, dim, 1, pair, p.tile_n);
+    q.c_tma = pair;  // a single CTA's column halves need not be whole 64-column boxes
     q.c = g;
     q.scm = plan.pitch;
     p.num_tiles = q.tiles;
     if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-    if (int st = launch_product<loss::kGradient>(p, s)) return st;
+    if (int st = launch_product<loss::kGradient>(p, pair, s)) return st;
 
     p = base;
+    p.tile_n = loss::TILE;
     int n = 0;
     if (dx) {
       loss::Problem& d = p.prob[n++];
       ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, loss::BM);
-      ok &= load_map(&d.b, w, dtype, dim, cols, sw, loss::BK);
+      ok &= load_b(d, w, dtype, dim, cols, sw);
       shape(d, tokens, dim, cols, plan.splits);
       d.acc = acc;
       if (plan.splits > 1) d.acc_mode = loss::kAccSlab;
@@ -291,8 +347,8 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     }
     if (dw) {
       loss::Problem& d = p.prob[n++];
-      ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, loss::BK);
-      ok &= load_map(&d.b, x, dtype, dim, tokens, sx, loss::BK);
+      ok &= slab_map(&d.a, g, dtype, plan.pitch / 64, tokens, plan.pitch);  // rows of dW beyond cols are not stored
+      ok &= load_b(d, x, dtype, dim, tokens, sx);
       shape(d, cols, dim, tokens, 1);
       d.a_mn = 1;
       char* out = static_cast<char*>(dw) + col0 * sdw * 2;
@@ -302,8 +358,14 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
       if (d.c_tma) ok &= store_map(&d.c_box, out, dtype, dim, cols, sdw);
     }
     if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-    p.num_tiles = p.prob[0].tiles + (n > 1 ? p.prob[1].tiles : 0);
-    if (int st = launch_product<loss::kProducts>(p, s)) return st;
+    p.num_tiles = p.prob[0].tiles;
+    if (n > 1) {
+      const int pairs = device_info().sm_count / 2, left = p.prob[0].tiles % pairs;
+      p.num_tiles += p.prob[1].tiles;
+      if (left > 0 && p.num_tiles >= pairs)
+        p.extra = std::min(p.prob[0].split_stages / p.prob[1].k_stages, p.prob[1].tiles / (pairs - left));
+    }
+    if (int st = launch_product<loss::kProducts>(p, true, s)) return st;
     if (dx && plan.splits > 1) {
       const loss::Problem& d = p.prob[0];
       const loss::JoinArgs j{acc, d.m, d.n, d.m_blocks, d.n_blocks, d.splits, p.fmt, static_cast<uint16_t*>(dx), sdx};

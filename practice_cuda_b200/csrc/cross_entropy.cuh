@@ -14,12 +14,18 @@
 //              order of 1 and the loss's scale stays in fp32).
 //   kProducts  dX += G W and dW = G^T X of that piece in one launch: the tiles
 //              of both share the grid, so neither leaves SMs idle at its end.
-// Logits, softmax statistics and every sum are fp32 (m and log2 s are kept apart:
+// Logits, softmax statistics and every sum are fp32.  m and log2 s are kept apart:
 // their sum would lose the small part of a sure token's probability beside a large
-// logit); tiles are 256 x 256 on a
-// CTA pair (cta_group::2), 64-deep stages of 128-byte swizzled operands by TMA,
-// two accumulators of 256 fp32 columns in tensor memory, so that a tile's
-// epilogue runs under the next tile's products.  Bound by the tensor cores.
+// logit.  The tensor cores truncate as they accumulate, which moves a logit of 4096
+// products by about 3e-6 of its size towards zero, and a mean loss with it; so
+// the logits' accumulators are added up in registers every 512 products
+// (measured on the loss: 2.9e-6 before, see kChunkStages).
+//
+// Tiles are 256 x 256 on a CTA pair (cta_group::2), fed by 64-deep stages of
+// 128-byte swizzled operands by TMA, with two accumulators of 256 fp32 columns in
+// tensor memory, so that an epilogue runs under the next products.  Up to 128
+// tokens, where reading W is what takes the time, a tile is one CTA's: 128 rows
+// and as many columns as spread the vocabulary evenly over the SMs.
 #pragma once
 
 #include "gemm_sm100.cuh"
@@ -34,24 +40,39 @@ constexpr int BM = 128;            // rows of the tile per CTA
 constexpr int TILE = 256;          // tile rows of the pair, and tile columns
 constexpr int BK = 64;             // K elements of a stage: one 128-byte swizzle atom of 16-bit values
 constexpr int UMMA_K = 16;
-constexpr int STAGES = 6;
+constexpr int kChunkStages = 8;    // stages between two promotions of a logit's accumulator
 constexpr int A_BYTES = BM * BK * 2;
-constexpr int B_BYTES = TILE / 2 * BK * 2;  // each CTA stages half of the columns
 constexpr int SLAB = 64 * BK * 2;           // 64 MN elements x 64 K rows of an MN-major operand
 constexpr int NACC = 2;
 constexpr int kThreads = 384;
 constexpr int kEpiWarp0 = 4;
-constexpr int EPI_COLS = TILE / 2;  // columns of an epilogue thread
+constexpr int EPI_COLS = TILE / 2;  // columns of an epilogue thread, at most
+// Register split of the logit kernels (setmaxnreg), whose epilogue threads
+// hold 128 fp32 accumulators: what the launch holds is checked on the host.
+constexpr int kLaunchRegs = 168;
+constexpr int kLowRegs = 56, kHighRegs = 224;
+static_assert(128 * kLowRegs + 256 * kHighRegs == kThreads * kLaunchRegs, "register split must match the launch");
 constexpr int kGroupM = 16;         // tile rows that share the columns of W in L2
 constexpr int kAccVec = EPI_COLS / 4;  // float4s of an epilogue thread's share of a tile
 constexpr float kLog2e = 1.4426950408889634f;
+// G carries 2^kGradShift (taken out of `alpha`): its small entries (1 / vocab,
+// and a column that no token is likely to take has nothing larger) stay off
+// the subnormals of the 16-bit types and of the exponential, and the largest,
+// 2^14, is within fp16.  The shift is a term of the exponent, so it costs nothing.
+constexpr int kGradShift = 14;
+constexpr float kGradScale = 16384.f;
 
-constexpr int OFF_B = STAGES * A_BYTES;
-constexpr int OFF_CSTG = OFF_B + STAGES * B_BYTES;  // 4 KB per epilogue warp
-constexpr int OFF_BAR = OFF_CSTG + 8 * 4096;
-constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 2 * NACC) * 8;
-constexpr int SMEM_ALLOC = OFF_MISC + 16 + 1024;  // slack for the 1 KB alignment
-static_assert(SMEM_ALLOC <= 232448, "shared memory per CTA");
+template <bool PAIR>
+struct Smem {
+  static constexpr int STAGES = PAIR ? 6 : 4;
+  static constexpr int B_BYTES = (PAIR ? TILE / 2 : TILE) * BK * 2;  // a pair's CTA stages half of the columns
+  static constexpr int OFF_B = STAGES * A_BYTES;
+  static constexpr int OFF_CSTG = OFF_B + STAGES * B_BYTES;  // 4 KB per epilogue warp
+  static constexpr int OFF_BAR = OFF_CSTG + 8 * 4096;
+  static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 2 * NACC) * 8;
+  static constexpr int ALLOC = OFF_MISC + 16 + 1024;  // slack for the 1 KB alignment
+  static_assert(ALLOC <= 232448, "shared memory per CTA");
+};
 
 enum Site : int { SITE_LOSS_PRODUCER = 16, SITE_LOSS_MMA = 17, SITE_LOSS_EPILOGUE = 18, SITE_LOSS_TARGET = 19 };
 
@@ -62,7 +83,8 @@ struct Problem {
   int m_blocks, n_blocks, splits;  // splits: parts of K, each a tile of its own
   int tiles;                       // m_blocks * n_blocks * splits
   int k_stages, split_stages;
-  int a_mn;   // A is M-major (kProducts)
+  int a_mn;   // A is M-major (kProducts; B is N-major there)
+  int b_slabs;  // B's map takes both of a CTA's 64-column slabs in one load
   int c_tma;  // C leaves through TMA stores
   void* c;
   long long scm;
@@ -73,6 +95,8 @@ struct Problem {
 struct Params {
   Problem prob[2];
   int num_tiles;
+  int extra;   // tiles of prob[1] that the workers with one tile less of prob[0] take first
+  int tile_n;  // tile columns (TILE on a CTA pair)
   int fmt;  // 0 fp16, 1 bf16
   // rows
   const long long* target;
@@ -80,7 +104,6 @@ struct Params {
   long long vocab;
   const float* stats;       // [2][m]: m_i and log2 s_i
   const float* row_weight;  // null: 1
-  float grad_scale;         // power of two that G carries
   int col0;                 // first vocabulary column of the piece
   float2* partial;          // [n_blocks * 2][m]: maximum and sum of exponentials
   float* target_logit;      // [m]
@@ -95,34 +118,39 @@ __device__ __forceinline__ float alpha_of(const Params& p) {
   if (p.alpha) return *p.alpha;
   float a = *p.dloss;
   if (p.count) a = *p.count > 0.f ? __fdiv_rn(a, *p.count) : 0.f;
-  return a / p.grad_scale;
+  return a * (1.f / kGradScale);
 }
 
-__device__ __forceinline__ void umma_f16_pair_elect(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
-                                                    uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred e, p;\n\t.reg .b64 ad, bd;\n\t"
-      "mov.b64 ad, {%1, %2};\n\t"
-      "mov.b64 bd, {%3, %4};\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void umma_f16_elect(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                               uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 ad, bd;\n\t"
+        "mov.b64 ad, {%1, %2};\n\t"
+        "mov.b64 bd, {%3, %4};\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %5, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 ad, bd;\n\t"
+        "mov.b64 ad, {%1, %2};\n\t"
+        "mov.b64 bd, {%3, %4};\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %5, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
 }
 
-// Terms below 2^-126 count as zero: beside a sum of at least 1.
+// Results below 2^-126 are zero.
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// With results below 2^-126 kept: a column that no token is likely to take has
-// nothing but such entries in G, and its gradient is theirs.
-__device__ __forceinline__ float exp2_subnormal(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -133,6 +161,28 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, int fmt) {
   }
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The tile that worker `w` of `workers` (CTAs or pairs) takes in turn `i`, or -1.
+// Workers take turns.  Where prob[0]'s long tiles do not come out even, the
+// workers with one less of them take `extra` of prob[1]'s short ones in its
+// place, and the turns go on from there.
+__device__ __forceinline__ int tile_of(const Params& p, int w, int workers, int i) {
+  const int t0 = p.prob[0].tiles;
+  const int own = (t0 - w + workers - 1) / workers;
+  if (i < own) return i * workers + w;
+  i -= own;
+  int at = t0;
+  const int r = t0 % workers;
+  if (p.extra) {  // only where r > 0
+    if (w >= r) {
+      if (i < p.extra) return t0 + i * (workers - r) + (w - r);
+      i -= p.extra;
+    }
+    at += p.extra * (workers - r);
+  }
+  const int tile = at + i * workers + w;
+  return tile < p.num_tiles ? tile : -1;
 }
 
 struct TileAt {
@@ -159,9 +209,10 @@ __device__ __forceinline__ TileAt locate(const Params& p, int tile) {
 
 // 64 columns of a warp's 32 rows: every lane packs its row's 128 bytes into the
 // warp's staging buffer (128-byte swizzle), from where one TMA store takes
-// the box, or, where C's rows do not suit TMA, the warp writes row by row.
-__device__ __forceinline__ void store_box(const Params& p, const Problem& q, const uint32_t (&w)[32], uint32_t stg,
-                                          int lane, int row0, int col) {
+// the box, or, where C's rows do not suit TMA, the warp writes row by row
+// (columns below `limit`).
+__device__ __forceinline__ void store_box(const Problem& q, const uint32_t (&w)[32], uint32_t stg, int lane, int row0,
+                                          int col, int limit) {
   if (lane == 0) gemm::bulk_wait_read<0>();
   __syncwarp();
   const uint32_t swz = (uint32_t)(lane & 7);
@@ -188,31 +239,37 @@ __device__ __forceinline__ void store_box(const Params& p, const Problem& q, con
       uint16_t v;
       const uint32_t src = stg + (uint32_t)r * 128u + ((((uint32_t)e >> 3) ^ ((uint32_t)r & 7u)) << 4) + ((uint32_t)e & 7u) * 2u;
       asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
-      if (col + e < q.n) c[(long long)(row0 + r) * q.scm + col + e] = v;
+      if (col + e < limit) c[(long long)(row0 + r) * q.scm + col + e] = v;
     }
   }
   __syncwarp();
 }
 
-template <int MODE>
+template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid_constant__ Params p) {
-  constexpr uint32_t STAGE_TX = 2 * (A_BYTES + B_BYTES);  // of both CTAs, on the leader's barrier
+  static_assert(PAIR || MODE != kProducts, "the products of G run on CTA pairs");
+  using S = Smem<PAIR>;
+  constexpr int STAGES = S::STAGES;
+  constexpr int TILE_M = PAIR ? TILE : BM;
+  constexpr bool CHUNKED = MODE != kProducts;
+  // Bytes of a stage on the (leader's) full barrier.
+  const uint32_t stage_tx = PAIR ? 2 * (A_BYTES + S::B_BYTES) : A_BYTES + (uint32_t)p.tile_n * BK * 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t s_base = smem_u32(smem);
-  const uint32_t bar_full = s_base + OFF_BAR;         // [STAGES]
+  const uint32_t bar_full = s_base + S::OFF_BAR;      // [STAGES]
   const uint32_t bar_empty = bar_full + 8 * STAGES;   // [STAGES]
   const uint32_t bar_tfull = bar_empty + 8 * STAGES;  // [NACC]
   const uint32_t bar_tempty = bar_tfull + 8 * NACC;   // [NACC]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::OFF_MISC + 4);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = gemm::cluster_ctarank();
+  const uint32_t rank = PAIR ? gemm::cluster_ctarank() : 0u;
   const bool leader = rank == 0;
-  const int first_tile = (int)(blockIdx.x >> 1);
-  const int tile_step = (int)(gridDim.x >> 1);
+  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+  const int workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -221,16 +278,22 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
     }
     for (int i = 0; i < NACC; ++i) {
       mbar_init(bar_tfull + 8 * i, 1);
-      mbar_init(bar_tempty + 8 * i, 16);  // one arrive per epilogue warp of both CTAs
+      mbar_init(bar_tempty + 8 * i, PAIR ? 16 : 8);  // one arrive per epilogue warp (of both CTAs)
     }
     *abort_flag = 0;
     fence_barrier_init();
     gemm::prefetch_tmap(&p.prob[0].a);
     gemm::prefetch_tmap(&p.prob[0].b);
   }
-  if (warp == 1) gemm::tmem_alloc_pair(smem_u32(tmem_slot), NACC * TILE);
-  gemm::tc_fence_before();
-  gemm::cluster_sync_all();  // both CTAs' barriers exist before any remote arrive / TMA
+  if constexpr (PAIR) {
+    if (warp == 1) gemm::tmem_alloc_pair(smem_u32(tmem_slot), NACC * TILE);
+    gemm::tc_fence_before();
+    gemm::cluster_sync_all();  // both CTAs' barriers exist before any remote arrive / TMA
+  } else {
+    if (warp == 1) gemm::tmem_alloc(smem_u32(tmem_slot), NACC * TILE);
+    gemm::tc_fence_before();
+    __syncthreads();
+  }
   gemm::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // The set-up above overlaps the previous kernel's tail; nothing global is
@@ -238,233 +301,284 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
 
-  if (warp == 0) {
-    // ------------------------------ TMA producer ------------------------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int tile = first_tile; tile < p.num_tiles && ok; tile += tile_step) {
-        const TileAt t = locate(p, tile);
-        const Problem& q = p.prob[t.prob];
-        const int a_row = t.mb * TILE + (int)rank * BM;
-        const int b_col = t.nb * TILE + (int)rank * (TILE / 2);
-        const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
-        for (int ks = t.split * q.split_stages; ks < ks1; ++ks) {
-          if (!mbar_spin_bounded(bar_empty + 8 * stage, phase ^ 1, abort_flag, SITE_LOSS_PRODUCER)) {
-            ok = false;
-            break;
-          }
-          const uint32_t fb = bar_full + 8 * stage;
-          const uint32_t a_dst = s_base + stage * A_BYTES;
-          const uint32_t b_dst = s_base + OFF_B + stage * B_BYTES;
-          if (leader) mbar_arrive_expect_tx(fb, STAGE_TX);
-          const uint32_t fbl = gemm::mapa_shared(fb, 0);
-          if (MODE == kProducts && q.a_mn) {
-            gemm::tma_load_3d_pair(a_dst, &q.a, fbl, a_row, ks * BK, 0);
-            gemm::tma_load_3d_pair(a_dst + SLAB, &q.a, fbl, a_row + 64, ks * BK, 0);
-          } else {
-            gemm::tma_load_3d_pair(a_dst, &q.a, fbl, ks * BK, a_row, 0);
-          }
-          if (MODE == kProducts) {
-            gemm::tma_load_3d_pair(b_dst, &q.b, fbl, b_col, ks * BK, 0);
-            gemm::tma_load_3d_pair(b_dst + SLAB, &q.b, fbl, b_col + 64, ks * BK, 0);
-          } else {
-            gemm::tma_load_3d_pair(b_dst, &q.b, fbl, ks * BK, b_col, 0);
-          }
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
+  if (warp < kEpiWarp0) {
+    if constexpr (CHUNKED) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
+    if (warp == 0) {
+      // ------------------------------ TMA producer ------------------------------
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
+          const TileAt t = locate(p, tile);
+          const Problem& q = p.prob[t.prob];
+          const int a_row = t.mb * TILE_M + (int)rank * BM;
+          const int b_col = PAIR ? t.nb * TILE + (int)rank * (TILE / 2) : t.nb * p.tile_n;
+          const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
+          for (int ks = t.split * q.split_stages; ks < ks1; ++ks) {
+            if (!mbar_spin_bounded(bar_empty + 8 * stage, phase ^ 1, abort_flag, SITE_LOSS_PRODUCER)) {
+              ok = false;
+              break;
+            }
+            const uint32_t fb = bar_full + 8 * stage;
+            const uint32_t a_dst = s_base + stage * A_BYTES;
+            const uint32_t b_dst = s_base + S::OFF_B + stage * S::B_BYTES;
+            if (leader) mbar_arrive_expect_tx(fb, stage_tx);
+            if constexpr (PAIR) {
+              const uint32_t fbl = gemm::mapa_shared(fb, 0);
+              if (MODE == kProducts && q.a_mn) {
+                gemm::tma_load_3d_pair(a_dst, &q.a, fbl, 0, ks * BK, a_row / 64);
+              } else {
+                gemm::tma_load_3d_pair(a_dst, &q.a, fbl, ks * BK, a_row, 0);
+              }
+              if (MODE == kProducts && q.b_slabs) {
+                gemm::tma_load_3d_pair(b_dst, &q.b, fbl, 0, ks * BK, b_col / 64);
+              } else if (MODE == kProducts) {
+                gemm::tma_load_3d_pair(b_dst, &q.b, fbl, b_col, ks * BK, 0);
+                gemm::tma_load_3d_pair(b_dst + SLAB, &q.b, fbl, b_col + 64, ks * BK, 0);
+              } else {
+                gemm::tma_load_3d_pair(b_dst, &q.b, fbl, ks * BK, b_col, 0);
+              }
+            } else {
+              gemm::tma_load_3d(a_dst, &q.a, fb, ks * BK, a_row, 0);
+              gemm::tma_load_3d(b_dst, &q.b, fb, ks * BK, b_col, 0);
+            }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
         }
-      }
-      if (!ok) {
-        // Let the copies already issued land before the CTA can exit.
-        for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(bar_full + 8 * s, 0, abort_flag, SITE_LOSS_PRODUCER);
-      }
-    }
-  } else if (warp == 1) {
-    // ------------------------------- MMA issuer -------------------------------
-    if (leader) {
-      int stage = 0;
-      uint32_t phase = 0, acc_cnt = 0;
-      bool ok = true;
-      auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-        return mbar_spin_bounded_warp(bar, parity, abort_flag, SITE_LOSS_MMA);
-      };
-      const uint64_t k_desc = gemm::make_sw128_desc(s_base, 16u), mn_desc = gemm::make_sw128_desc(s_base, SLAB);
-      constexpr uint32_t K_STEP = UMMA_K * 2 >> 4;      // 32 bytes along a K-major row
-      constexpr uint32_t MN_STEP = UMMA_K * 128 >> 4;   // 16 K rows of an MN-major slab
-      constexpr uint32_t B_STEP = MODE == kProducts ? MN_STEP : K_STEP;
-      const uint64_t b_desc = MODE == kProducts ? mn_desc : k_desc;
-      for (int tile = first_tile; tile < p.num_tiles && ok; tile += tile_step, ++acc_cnt) {
-        const TileAt t = locate(p, tile);
-        const Problem& q = p.prob[t.prob];
-        const bool a_mn = MODE == kProducts && q.a_mn;
-        const uint64_t a_desc = a_mn ? mn_desc : k_desc;
-        const uint32_t a_step = a_mn ? MN_STEP : K_STEP;
-        const uint32_t idesc = gemm::make_idesc(TILE, p.fmt, p.fmt, a_mn ? 1 : 0, MODE == kProducts ? 1 : 0, 2 * BM);
-        const uint32_t abuf = acc_cnt % NACC, d_tmem = tmem_base + abuf * TILE;
-        if (!wait(bar_tempty + 8 * abuf, ((acc_cnt / NACC) & 1) ^ 1)) {
-          ok = false;
-          break;
+        if (!ok) {
+          // Let the copies already issued land before the CTA can exit.
+          for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(bar_full + 8 * s, 0, abort_flag, SITE_LOSS_PRODUCER);
         }
-        const int ks0 = t.split * q.split_stages, ks1 = min(q.k_stages, ks0 + q.split_stages);
-        for (int ks = ks0; ks < ks1; ++ks) {
-          if (!wait(bar_full + 8 * stage, phase)) {
-            ok = false;
-            break;
-          }
-          gemm::tc_fence_after();
-          const uint32_t a_lo = (uint32_t)a_desc + (uint32_t)(stage * A_BYTES >> 4);
-          const uint32_t b_lo = (uint32_t)b_desc + (uint32_t)((OFF_B + stage * B_BYTES) >> 4);
+      }
+    } else if (warp == 1) {
+      // ------------------------------- MMA issuer -------------------------------
+      if (leader) {
+        int stage = 0;
+        uint32_t phase = 0, acc_cnt = 0;
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+          return mbar_spin_bounded_warp(bar, parity, abort_flag, SITE_LOSS_MMA);
+        };
+        const uint64_t k_desc = gemm::make_sw128_desc(s_base, 16u), mn_desc = gemm::make_sw128_desc(s_base, SLAB);
+        constexpr uint32_t K_STEP = UMMA_K * 2 >> 4;     // 32 bytes along a K-major row
+        constexpr uint32_t MN_STEP = UMMA_K * 128 >> 4;  // 16 K rows of an MN-major slab
+        constexpr uint32_t B_STEP = MODE == kProducts ? MN_STEP : K_STEP;
+        const uint64_t b_desc = MODE == kProducts ? mn_desc : k_desc;
+        for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
+          const TileAt t = locate(p, tile);
+          const Problem& q = p.prob[t.prob];
+          const bool a_mn = MODE == kProducts && q.a_mn;
+          const uint64_t a_desc = a_mn ? mn_desc : k_desc;
+          const uint32_t a_step = a_mn ? MN_STEP : K_STEP;
+          const uint32_t idesc =
+              gemm::make_idesc(p.tile_n, p.fmt, p.fmt, a_mn ? 1 : 0, MODE == kProducts ? 1 : 0, TILE_M);
+          const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
+          int ks = t.split * q.split_stages;
+          while (ks < ks1 && ok) {
+            const uint32_t abuf = acc_cnt % NACC, d_tmem = tmem_base + abuf * TILE;
+            if (!wait(bar_tempty + 8 * abuf, ((acc_cnt / NACC) & 1) ^ 1)) {
+              ok = false;
+              break;
+            }
+            const int stop = CHUNKED ? min(ks1, ks + kChunkStages) : ks1;
+            for (bool fresh = true; ks < stop; ++ks, fresh = false) {
+              if (!wait(bar_full + 8 * stage, phase)) {
+                ok = false;
+                break;
+              }
+              gemm::tc_fence_after();
+              const uint32_t a_lo = (uint32_t)a_desc + (uint32_t)(stage * A_BYTES >> 4);
+              const uint32_t b_lo = (uint32_t)b_desc + (uint32_t)((S::OFF_B + stage * S::B_BYTES) >> 4);
 #pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk)
-            umma_f16_pair_elect(d_tmem, a_lo + kk * a_step, (uint32_t)(a_desc >> 32), b_lo + kk * B_STEP,
-                                (uint32_t)(b_desc >> 32), idesc, (kk > 0 || ks > ks0) ? 1u : 0u);
-          gemm::umma_commit_elect<true>(bar_empty + 8 * stage);  // stage (of both CTAs) free once these retire
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
+              for (int kk = 0; kk < BK / UMMA_K; ++kk)
+                umma_f16_elect<PAIR>(d_tmem, a_lo + kk * a_step, (uint32_t)(a_desc >> 32), b_lo + kk * B_STEP,
+                                     (uint32_t)(b_desc >> 32), idesc, (kk > 0 || !fresh) ? 1u : 0u);
+              gemm::umma_commit_elect<PAIR>(bar_empty + 8 * stage);  // stage (of both CTAs) free once these retire
+              if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            }
+            if (!ok) break;
+            gemm::umma_commit_elect<PAIR>(bar_tfull + 8 * abuf);  // accumulator ready (both CTAs)
+            ++acc_cnt;
           }
         }
-        if (!ok) break;
-        gemm::umma_commit_elect<true>(bar_tfull + 8 * abuf);  // accumulator ready (both CTAs)
       }
     }
-  } else if (warp >= kEpiWarp0) {
+  } else {
     // -------------------------------- epilogue --------------------------------
+    if constexpr (CHUNKED) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHighRegs));
     const int ew = warp - kEpiWarp0;  // 0..7
     const int quarter = warp & 3;     // tensor-memory lanes 32 * quarter .. + 31
     const int half = ew >> 2;         // column half
-    const uint32_t stg = s_base + OFF_CSTG + (uint32_t)ew * 4096u;
-    const uint32_t bar_tempty_l = gemm::mapa_shared(bar_tempty, 0);
-    uint32_t acc_cnt = 0;
+    const int half_cols = PAIR ? EPI_COLS : p.tile_n / 2;
+    const uint32_t stg = s_base + S::OFF_CSTG + (uint32_t)ew * 4096u;
+    const uint32_t bar_tempty_l = PAIR ? gemm::mapa_shared(bar_tempty, 0) : bar_tempty;
     const float alpha = MODE == kProducts ? alpha_of(p) : 1.f;
-    for (int tile = first_tile; tile < p.num_tiles; tile += tile_step, ++acc_cnt) {
+    uint32_t acc_cnt = 0;
+    bool ok = true;
+    for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
       const TileAt t = locate(p, tile);
       const Problem& q = p.prob[t.prob];
-      const int row0 = t.mb * TILE + (int)rank * BM + quarter * 32;  // of the warp
+      const int row0 = t.mb * TILE_M + (int)rank * BM + quarter * 32;  // of the warp
       const int row = row0 + lane;
-      const int col0 = t.nb * TILE + half * EPI_COLS;
+      const int col0 = t.nb * (PAIR ? TILE : p.tile_n) + half * half_cols;
+      const int limit = min(q.n, col0 + half_cols);  // columns of this half
       const bool in = row < q.m;
-      // Row values are read before the wait, so their latency is hidden.
-      long long target = -1;
-      float top = 0.f, log2_sum = 0.f, weight = 0.f;
-      if (MODE != kProducts && in) {
-        target = p.target[row];
-        const bool valid = target != p.ignore_index;
-        if (MODE == kGradient && valid) {
-          top = p.stats[row];
-          log2_sum = p.stats[q.m + row];
-          weight = p.grad_scale * (p.row_weight ? p.row_weight[row] : 1.f);
-          if (target < 0 || target >= p.vocab) weight = NAN;  // no such column
-        }
-        target = valid ? target - p.col0 : -1;
-      }
-      const uint32_t abuf = acc_cnt % NACC;
-      if (!mbar_spin_bounded_warp(bar_tfull + 8 * abuf, (acc_cnt / NACC) & 1, abort_flag, SITE_LOSS_EPILOGUE)) break;
-      gemm::tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * TILE + half * EPI_COLS;
-      auto release = [&] {  // this warp has read its part of the accumulator
+      auto wait_full = [&](uint32_t abuf) -> bool {
+        if (!mbar_spin_bounded_warp(bar_tfull + 8 * abuf, (acc_cnt / NACC) & 1, abort_flag, SITE_LOSS_EPILOGUE))
+          return false;
+        gemm::tc_fence_after();
+        return true;
+      };
+      auto release = [&](uint32_t abuf) {  // this warp has read its part of the accumulator
         gemm::tc_fence_before();
         __syncwarp();
-        if (lane == 0) gemm::mbar_arrive_cluster(bar_tempty_l + 8 * abuf);
+        if (lane == 0) {
+          if constexpr (PAIR) gemm::mbar_arrive_cluster(bar_tempty_l + 8 * abuf);
+          else mbar_arrive(bar_tempty + 8 * abuf);
+        }
       };
-      uint32_t v[2][32];
-      gemm::tmem_ld32_nowait(taddr, v[0]);
-      gemm::tmem_wait_ld();
-      gemm::tmem_regs_ready(v[0]);
+      auto address = [&](uint32_t abuf) {
+        return tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * TILE + half * half_cols;
+      };
 
-      if constexpr (MODE == kStats) {
-        float m = -INFINITY, s = 0.f, tl = 0.f;
-#pragma unroll
-        for (int c = 0; c < EPI_COLS / 32; ++c) {
-          if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
-          else release();
-          uint32_t(&u)[32] = v[c & 1];
-          const int cc = col0 + c * 32;
-          if (cc + 32 > q.n) {  // columns beyond the vocabulary
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (cc + i >= q.n) u[i] = 0xff800000u;
-          }
-          if (target >= cc && target < cc + 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (target == cc + i) tl = __uint_as_float(u[i]);
-          }
-          float mc[4] = {m, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mc[i & 3] = fmaxf(mc[i & 3], __uint_as_float(u[i]));
-          const float mn = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
-          const float base = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: exp(-inf - 0) = 0
-          float sc[4] = {s * exp2_approx((m - base) * kLog2e), 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) sc[i & 3] += exp2_approx((__uint_as_float(u[i]) - base) * kLog2e);
-          s = (sc[0] + sc[1]) + (sc[2] + sc[3]);
-          m = mn;
-          if (c + 1 < EPI_COLS / 32) {
-            gemm::tmem_wait_ld();
-            gemm::tmem_regs_ready(v[(c + 1) & 1]);
-          }
-        }
+      if constexpr (CHUNKED) {
+        // Row values are read before the wait, so their latency is hidden.
+        int target = -1;  // within the piece
+        float top = 0.f, shift = 0.f, weight = 0.f;
         if (in) {
-          p.partial[(long long)(t.nb * 2 + half) * q.m + row] = make_float2(m, s);
-          if (target >= col0 && target < min(col0 + EPI_COLS, q.n)) p.target_logit[row] = tl;
+          const long long tv = p.target[row];
+          const bool valid = tv != p.ignore_index;
+          if (MODE == kGradient && valid) {
+            top = p.stats[row];
+            shift = (float)kGradShift - p.stats[q.m + row];
+            weight = p.row_weight ? p.row_weight[row] : 1.f;
+            if (tv < 0 || tv >= p.vocab) weight = NAN;  // no such column
+          }
+          if (valid && tv >= p.col0 + col0 && tv < p.col0 + limit) target = (int)(tv - p.col0);
         }
-      } else {
-        float4* acc = nullptr;
-        if (MODE == kProducts && q.acc_mode != kAccNone)
-          acc = q.acc + ((long long)t.index * 2 + rank) * kAccVec * 256 + ew * 32 + lane;
-        uint32_t w[32];  // 64 packed columns
+        // The logits: the accumulators of every 512 products, summed.
+        float acc[EPI_COLS];
+        const int chunks = (q.k_stages + kChunkStages - 1) / kChunkStages;
+        for (int ch = 0; ch < chunks; ++ch, ++acc_cnt) {
+          const uint32_t abuf = acc_cnt % NACC;
+          if (!wait_full(abuf)) {
+            ok = false;
+            break;
+          }
+          const uint32_t taddr = address(abuf);
+          uint32_t v[2][32];
+          gemm::tmem_ld32_nowait(taddr, v[0]);
+          gemm::tmem_wait_ld();
+          gemm::tmem_regs_ready(v[0]);
 #pragma unroll
-        for (int c = 0; c < EPI_COLS / 32; ++c) {
-          if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
-          else release();
-          uint32_t(&u)[32] = v[c & 1];
-          if constexpr (MODE == kGradient) {
-            const int cc = col0 + c * 32;
+          for (int c = 0; c < EPI_COLS / 32; ++c) {
+            if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
+            else release(abuf);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              u[i] = __float_as_uint(exp2_subnormal(fmaf(__uint_as_float(u[i]) - top, kLog2e, -log2_sum)));
-            if (target >= cc && target < cc + 32) {
+            for (int j = 0; j < 32; ++j) {
+              const float x = __uint_as_float(v[c & 1][j]);
+              acc[c * 32 + j] = ch == 0 ? x : acc[c * 32 + j] + x;
+            }
+            if (c + 1 < EPI_COLS / 32) {
+              gemm::tmem_wait_ld();
+              gemm::tmem_regs_ready(v[(c + 1) & 1]);
+            }
+          }
+        }
+        if (!ok) break;
+
+        if constexpr (MODE == kStats) {
+          float tl = 0.f;
+          if (target >= 0) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (target == cc + i) u[i] = __float_as_uint(__uint_as_float(u[i]) - 1.f);
+            for (int j = 0; j < EPI_COLS; ++j)
+              if (target == col0 + j) tl = acc[j];
+          }
+          if (col0 + EPI_COLS > limit) {  // columns beyond this half, or the vocabulary
+#pragma unroll
+            for (int j = 0; j < EPI_COLS; ++j)
+              if (col0 + j >= limit) acc[j] = -INFINITY;
+          }
+          float mc[4] = {acc[0], acc[1], acc[2], acc[3]};
+#pragma unroll
+          for (int j = 4; j < EPI_COLS; ++j) mc[j & 3] = fmaxf(mc[j & 3], acc[j]);
+          const float m = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
+          const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf: exp(-inf - 0) = 0
+          float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < EPI_COLS; ++j) sc[j & 3] += exp2_approx((acc[j] - base) * kLog2e);
+          if (in) {
+            p.partial[(long long)(t.nb * 2 + half) * q.m + row] = make_float2(m, (sc[0] + sc[1]) + (sc[2] + sc[3]));
+            if (target >= 0) p.target_logit[row] = tl;
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < EPI_COLS / 64; ++b) {  // boxes of 64 columns
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              acc[b * 64 + j] = exp2_approx(fmaf(acc[b * 64 + j] - top, kLog2e, shift));
+            if (target >= col0 + b * 64 && target < col0 + b * 64 + 64) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j)
+                if (target == col0 + b * 64 + j) acc[b * 64 + j] -= kGradScale;
             }
             // Tokens left out get zeros, whatever their logits are.
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float lo = __uint_as_float(u[2 * i]) * weight, hi = __uint_as_float(u[2 * i + 1]) * weight;
-              w[(c & 1) * 16 + i] = weight == 0.f ? 0u : pack2(lo, hi, p.fmt);
-            }
-          } else {
-            if (q.acc_mode == kAccAdd || q.acc_mode == kAccLast) {
+            for (int j = 0; j < 32; ++j)
+              w[j] = weight == 0.f
+                         ? 0u
+                         : pack2(acc[b * 64 + 2 * j] * weight, acc[b * 64 + 2 * j + 1] * weight, p.fmt);
+            if (b * 64 < half_cols) store_box(q, w, stg, lane, row0, col0 + b * 64, limit);
+          }
+        }
+      } else {
+        const uint32_t abuf = acc_cnt % NACC;
+        if (!wait_full(abuf)) break;
+        ++acc_cnt;
+        const uint32_t taddr = address(abuf);
+        float4* acc = nullptr;
+        if (q.acc_mode != kAccNone) acc = q.acc + ((long long)t.index * 2 + rank) * kAccVec * 256 + ew * 32 + lane;
+        const bool add = q.acc_mode == kAccAdd || q.acc_mode == kAccLast;
+        const bool stored = q.acc_mode == kAccNone || q.acc_mode == kAccLast;
+        uint32_t v[2][32], w[32];  // w: 64 packed columns
+        gemm::tmem_ld32_nowait(taddr, v[0]);
+        gemm::tmem_wait_ld();
+        gemm::tmem_regs_ready(v[0]);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 o = acc[(long long)(c * 8 + i) * 256];
-                u[4 * i] = __float_as_uint(__uint_as_float(u[4 * i]) + o.x);
-                u[4 * i + 1] = __float_as_uint(__uint_as_float(u[4 * i + 1]) + o.y);
-                u[4 * i + 2] = __float_as_uint(__uint_as_float(u[4 * i + 2]) + o.z);
-                u[4 * i + 3] = __float_as_uint(__uint_as_float(u[4 * i + 3]) + o.w);
-              }
-            }
-            if (q.acc_mode == kAccWrite || q.acc_mode == kAccAdd || q.acc_mode == kAccSlab) {
+        for (int c = 0; c < EPI_COLS / 32; ++c) {
+          if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
+          else release(abuf);
+          uint32_t(&u)[32] = v[c & 1];
+          if (add) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                acc[(long long)(c * 8 + i) * 256] =
-                    make_float4(__uint_as_float(u[4 * i]), __uint_as_float(u[4 * i + 1]), __uint_as_float(u[4 * i + 2]),
-                                __uint_as_float(u[4 * i + 3]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                w[(c & 1) * 16 + i] =
-                    pack2(__uint_as_float(u[2 * i]) * alpha, __uint_as_float(u[2 * i + 1]) * alpha, p.fmt);
+            for (int j = 0; j < 8; ++j) {
+              const float4 o = acc[(long long)(c * 8 + j) * 256];
+              u[4 * j] = __float_as_uint(__uint_as_float(u[4 * j]) + o.x);
+              u[4 * j + 1] = __float_as_uint(__uint_as_float(u[4 * j + 1]) + o.y);
+              u[4 * j + 2] = __float_as_uint(__uint_as_float(u[4 * j + 2]) + o.z);
+              u[4 * j + 3] = __float_as_uint(__uint_as_float(u[4 * j + 3]) + o.w);
             }
           }
-          const bool stored = MODE == kGradient || q.acc_mode == kAccNone || q.acc_mode == kAccLast;
-          if ((c & 1) && stored) store_box(p, q, w, stg, lane, row0, col0 + (c - 1) * 32);
+          if (stored) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[(c & 1) * 16 + j] = pack2(__uint_as_float(u[2 * j]) * alpha, __uint_as_float(u[2 * j + 1]) * alpha, p.fmt);
+            if (c & 1) store_box(q, w, stg, lane, row0, col0 + (c - 1) * 32, limit);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              acc[(long long)(c * 8 + j) * 256] =
+                  make_float4(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), __uint_as_float(u[4 * j + 2]),
+                              __uint_as_float(u[4 * j + 3]));
+          }
           if (c + 1 < EPI_COLS / 32) {
             gemm::tmem_wait_ld();
             gemm::tmem_regs_ready(v[(c + 1) & 1]);
@@ -476,15 +590,23 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
     if (MODE != kStats && lane == 0) gemm::bulk_wait_all();
   }
 
+  __syncwarp();
   gemm::tc_fence_before();
-  gemm::cluster_sync_all();  // no CTA leaves while its peer may still touch its smem / barriers
-  gemm::tc_fence_after();
-  if (warp == 1) gemm::tmem_dealloc_pair(tmem_base, NACC * TILE);
+  if constexpr (PAIR) {
+    gemm::cluster_sync_all();  // no CTA leaves while its peer may still touch its smem / barriers
+    gemm::tc_fence_after();
+    if (warp == 1) gemm::tmem_dealloc_pair(tmem_base, NACC * TILE);
+  } else {
+    __syncthreads();
+    gemm::tc_fence_after();
+    if (warp == 1) gemm::tmem_dealloc(tmem_base, NACC * TILE);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // The rows' statistics joined, the losses and their reduction.  A CTA
-// takes 32 tokens, its eight warps a strided eighth of the partials each.
+// takes 32 tokens, each of its 32 warps a strided part of the partials, read
+// eight at a time.
 // ---------------------------------------------------------------------------
 enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
 
@@ -501,20 +623,30 @@ struct RowArgs {
   unsigned* ticket;
 };
 
-__global__ void __launch_bounds__(256) loss_rows_kernel(const RowArgs p) {
-  __shared__ float ms[8][32], ss[8][32];
-  __shared__ double total[2][8];
+constexpr int kRowWarps = 32, kRowLoads = 8;
+__global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs p) {
+  __shared__ float ms[kRowWarps][32], ss[kRowWarps][32];
+  __shared__ double total[2][kRowWarps];
   __shared__ bool last;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
   if (row < p.tokens) {
-#pragma unroll 4
-    for (int i = warp; i < p.parts; i += 8) {
-      const float2 o = p.partial[(long long)i * p.tokens + row];
-      const float mn = fmaxf(m, o.x), base = mn == -INFINITY ? 0.f : mn;
-      s = s * exp2f((m - base) * kLog2e) + o.y * exp2f((o.x - base) * kLog2e);
+    for (int i = warp; i < p.parts; i += kRowWarps * kRowLoads) {
+      float2 o[kRowLoads];
+#pragma unroll
+      for (int j = 0; j < kRowLoads; ++j) {
+        const int part = i + j * kRowWarps;
+        o[j] = part < p.parts ? p.partial[(long long)part * p.tokens + row] : make_float2(-INFINITY, 0.f);
+      }
+      float mn = m;
+#pragma unroll
+      for (int j = 0; j < kRowLoads; ++j) mn = fmaxf(mn, o[j].x);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      s *= exp2f((m - base) * kLog2e);
+#pragma unroll
+      for (int j = 0; j < kRowLoads; ++j) s += o[j].y * exp2f((o[j].x - base) * kLog2e);
       m = mn;
     }
   }
@@ -525,11 +657,11 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const RowArgs p) {
   if (warp == 0 && row < p.tokens) {
     float top = ms[0][lane];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, ms[i][lane]);
+    for (int i = 1; i < kRowWarps; ++i) top = fmaxf(top, ms[i][lane]);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += ss[i][lane] * exp2f((ms[i][lane] - base) * kLog2e);
+    for (int i = 0; i < kRowWarps; ++i) sum += ss[i][lane] * exp2f((ms[i][lane] - base) * kLog2e);
     const float log_sum = logf(sum);
     p.stats[row] = base;
     p.stats[p.tokens + row] = log2f(sum);
@@ -566,7 +698,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const RowArgs p) {
   // The CTA that comes last adds all CTAs' sums, always in the same order.
   __threadfence();
   double a = 0.0, b = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) {
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kRowWarps * 32) {
     a += __ldcg(p.sums + 2 * i);
     b += __ldcg(p.sums + 2 * i + 1);
   }
@@ -578,7 +710,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const RowArgs p) {
   if (lane == 0) total[0][warp] = a, total[1][warp] = b;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) a += total[0][i], b += total[1][i];
+    for (int i = 1; i < kRowWarps; ++i) a += total[0][i], b += total[1][i];
     p.count[0] = (float)b;
     p.loss[0] = (float)(p.reduction == kMean ? a / b : a);  // 0 / 0 where every token is left out
   }
@@ -588,8 +720,8 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const RowArgs p) {
 // at most 1 in magnitude and the factor A (a power of two), so that G is
 // rounded at the same place whatever the scale.  One CTA.
 __global__ void __launch_bounds__(1024) loss_weights_kernel(const float* dloss, const long long* target,
-                                                            long long ignore_index, int tokens, float grad_scale,
-                                                            float* weight, float* alpha) {
+                                                            long long ignore_index, int tokens, float* weight,
+                                                            float* alpha) {
   __shared__ uint32_t top[32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   uint32_t m = 0;
@@ -606,7 +738,7 @@ __global__ void __launch_bounds__(1024) loss_weights_kernel(const float* dloss, 
   const float up = usable ? __uint_as_float((uint32_t)(e + 1) << 23) : 1.f;     // 2^(e + 1) > max
   const float down = usable ? __uint_as_float((uint32_t)(253 - e) << 23) : 1.f; // 1 / up
   for (int i = threadIdx.x; i < tokens; i += 1024) weight[i] = dloss[i] * down;
-  if (threadIdx.x == 0) *alpha = up / grad_scale;
+  if (threadIdx.x == 0) *alpha = up * (1.f / kGradScale);
 }
 
 // dX from the parts of K: the fp32 accumulators of every part summed in order.
