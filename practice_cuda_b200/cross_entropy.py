@@ -57,28 +57,34 @@ def _check(x, weight, target, reduction, piece):
         raise ValueError(f"{what}: vocab_piece must be positive, got {piece}")
 
 
+def _forward(x, weight, target, ignore_index, reduction):
+    """loss, and what the backward pass reads."""
+    x2, w2 = _aligned_rows(x), _aligned_rows(weight)
+    tokens, dim = x.shape
+    vocab = weight.shape[0]
+    device = x.device
+    lib = _lib.lib()
+    with _lib.on_device(device):
+        loss = x.new_empty((tokens,) if reduction == 0 else (), dtype=torch.float32)
+        stats = x.new_empty((2 * tokens + 1,), dtype=torch.float32)  # [2, tokens], count
+        if tokens == 0:
+            loss.fill_(float("nan") if reduction == 2 else 0.0)
+        nbytes = lib.pcb_linear_ce_fwd_workspace_bytes(tokens, vocab)
+        workspace = x.new_empty((nbytes,), dtype=torch.uint8)
+        at = stats.data_ptr()
+        status = lib.pcb_linear_ce_fwd(
+            x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x.dtype], tokens, vocab, dim,
+            target.data_ptr(), ignore_index, reduction, loss.data_ptr(), at, at + 8 * tokens,
+            workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
+        if status:
+            _lib.check(status, "pcb_linear_ce_fwd")
+    return loss, x2, w2, stats
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction, piece):
-        x2, w2 = _aligned_rows(x), _aligned_rows(weight)
-        tokens, dim = x.shape
-        vocab = weight.shape[0]
-        device = x.device
-        lib = _lib.lib()
-        with torch.cuda.device(device):
-            loss = torch.empty(tokens if reduction == 0 else (), device=device, dtype=torch.float32)
-            stats = torch.empty(2 * tokens + 1, device=device, dtype=torch.float32)  # [2, tokens], count
-            if tokens == 0:
-                loss.fill_(float("nan") if reduction == 2 else 0.0)
-            nbytes = lib.pcb_linear_ce_fwd_workspace_bytes(tokens, vocab)
-            workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
-            at = stats.data_ptr()
-            status = lib.pcb_linear_ce_fwd(
-                x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x.dtype], tokens, vocab, dim,
-                target.data_ptr(), ignore_index, reduction, loss.data_ptr(), at, at + 8 * tokens,
-                workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
-            if status:
-                _lib.check(status, "pcb_linear_ce_fwd")
+        loss, x2, w2, stats = _forward(x, weight, target, ignore_index, reduction)
         ctx.save_for_backward(x2, w2, target, stats)
         ctx.args = (ignore_index, reduction, piece)
         return loss
@@ -92,12 +98,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
         device = x2.device
         want_dx, want_dw = ctx.needs_input_grad[:2]
         lib = _lib.lib()
-        with torch.cuda.device(device):
+        with _lib.on_device(device):
             dloss = dloss.to(torch.float32).contiguous()
-            dx = torch.empty((tokens, dim), device=device, dtype=x2.dtype) if want_dx else None
-            dw = torch.empty((vocab, dim), device=device, dtype=x2.dtype) if want_dw else None
+            dx = x2.new_empty((tokens, dim)) if want_dx else None
+            dw = x2.new_empty((vocab, dim)) if want_dw else None
             nbytes = lib.pcb_linear_ce_bwd_workspace_bytes(tokens, vocab, dim, piece, int(want_dx))
-            workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+            workspace = x2.new_empty((nbytes,), dtype=torch.uint8)
             at = stats.data_ptr()
             status = lib.pcb_linear_ce_bwd(
                 x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x2.dtype], tokens, vocab, dim,
@@ -134,6 +140,11 @@ def linear_cross_entropy(
     _check(x, weight, target, reduction, vocab_piece)
     shape = target.shape
     x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
-    t = target.reshape(-1).to(torch.int64).contiguous()
-    loss = _LinearCrossEntropy.apply(x2, weight, t, int(ignore_index), _REDUCTIONS[reduction], int(vocab_piece or 0))
-    return loss.view(shape) if reduction == "none" else loss
+    t = target if target.ndim == 1 else target.reshape(-1)
+    t = t.to(torch.int64).contiguous()
+    code = _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropy.apply(x2, weight, t, int(ignore_index), code, int(vocab_piece or 0))
+    else:
+        loss = _forward(x2, weight, t, int(ignore_index), code)[0]
+    return loss.view(shape) if code == 0 and len(shape) != 1 else loss

@@ -40,11 +40,12 @@ int dispatch_norm_fwd(const norm::FwdArgs& p, bool vec, cudaStream_t s) {
   return check_launch("rms_norm_fwd_generic_kernel");
 }
 
-// CTAs of the backward pass: enough to fill the GPU, and no more rows of dw
-// shares than that.
-int norm_bwd_ctas(int64_t rows, int rows_per_cta) {
+// CTAs of the backward pass: those that are resident at once, each of which
+// leaves one row of dw shares.
+constexpr int kNormBwdMost = 4;  // per SM, in any variant
+int norm_bwd_ctas(int64_t rows, int rows_per_cta, int per_sm) {
   const int64_t ctas = (rows + rows_per_cta - 1) / rows_per_cta;
-  return (int)std::min<int64_t>(ctas, (int64_t)device_info().sm_count * 4);
+  return (int)std::min<int64_t>(ctas, (int64_t)device_info().sm_count * per_sm);
 }
 
 constexpr int kNormDwSmem = 160 * 1024;  // dw shares of one CTA of the generic backward
@@ -52,7 +53,7 @@ constexpr int kNormDwSmem = 160 * 1024;  // dw shares of one CTA of the generic 
 template <int XT, int LANES, int NV>
 int launch_norm_bwd(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
   constexpr int threads = LANES > 256 ? LANES : 256, rows = threads / LANES;
-  parts = norm_bwd_ctas(p.rows, rows);
+  parts = norm_bwd_ctas(p.rows, rows, LANES > 256 ? 1 : 2);
   const int smem = rows > 1 ? p.dim * 4 : 0;  // at most 1024 columns of fp32
   norm::rms_norm_bwd_kernel<XT, LANES, NV><<<parts, threads, smem, s>>>(p);
   return check_launch("rms_norm_bwd_kernel");
@@ -62,15 +63,17 @@ template <int XT>
 int dispatch_norm_bwd(const norm::BwdArgs& p, bool vec, int& parts, cudaStream_t s) {
   const int units = p.dim / norm::kUnit;
   if (vec && units <= 2048) {
+    // Two units a lane, or one of fp32, whose rows take twice the registers.
+    constexpr int NV = XT == PCB_DTYPE_F32 ? 1 : 2;
     if (units <= 32) return launch_norm_bwd<XT, 32, 1>(p, parts, s);
-    if (units <= 64) return launch_norm_bwd<XT, 32, 2>(p, parts, s);
-    if (units <= 128) return launch_norm_bwd<XT, 64, 2>(p, parts, s);
-    if (units <= 256) return launch_norm_bwd<XT, 128, 2>(p, parts, s);
-    if (units <= 512) return launch_norm_bwd<XT, 256, 2>(p, parts, s);
-    if (units <= 1024) return launch_norm_bwd<XT, 512, 2>(p, parts, s);
+    if (units <= 64) return launch_norm_bwd<XT, 64 / NV, NV>(p, parts, s);
+    if (units <= 128) return launch_norm_bwd<XT, 128 / NV, NV>(p, parts, s);
+    if (units <= 256) return launch_norm_bwd<XT, 256 / NV, NV>(p, parts, s);
+    if (units <= 512) return launch_norm_bwd<XT, 512 / NV, NV>(p, parts, s);
+    if (units <= 1024) return launch_norm_bwd<XT, 1024 / NV, NV>(p, parts, s);
     return launch_norm_bwd<XT, 1024, 2>(p, parts, s);
   }
-  parts = norm_bwd_ctas(p.rows, 1);
+  parts = norm_bwd_ctas(p.rows, 1, kNormBwdMost);
   const bool in_smem = (int64_t)p.dim * 4 <= kNormDwSmem;
   const int smem = in_smem ? p.dim * 4 : 0;
   auto kernel = norm::rms_norm_bwd_generic_kernel<XT>;
@@ -118,7 +121,7 @@ int pcb_rms_norm_fwd(const void* x, int x_dtype, int64_t rows, int64_t dim, int6
 
 int64_t pcb_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t dim) {
   if (rows <= 0 || dim <= 0) return 0;
-  return (int64_t)norm_bwd_ctas(rows, 1) * dim * 4;
+  return (int64_t)norm_bwd_ctas(rows, 1, kNormBwdMost) * dim * 4;
 }
 
 int pcb_rms_norm_bwd(const void* dy, int64_t sdy, const void* h, int64_t sh, int x_dtype, int64_t rows, int64_t dim,

@@ -383,25 +383,27 @@ __global__ void __launch_bounds__(kGenericThreads) rms_norm_fwd_generic_kernel(c
 // the grid.  A lane keeps its columns' weights and its share of dw in
 // registers over all rows; the CTA's shares are joined in shared memory and
 // written to partial[blockIdx.x], which rms_norm_dw_kernel sums in a fixed
-// order.  Bound by HBM traffic (dy, h, dh read once, dx written once).
+// order.  Bound by HBM traffic (dy, h, dh read once, dx written once); the next
+// row's values are loaded before this row's are used, so that a row's sum, which
+// all of its threads wait for, does not leave the memory idle.
 template <int XT, int LANES, int NV>
-__global__ void __launch_bounds__(LANES > 256 ? LANES : 256) rms_norm_bwd_kernel(const BwdArgs p) {
+__global__ void __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : 2) rms_norm_bwd_kernel(const BwdArgs p) {
   using T = typename InType<XT>::T;
   constexpr int THREADS = LANES > 256 ? LANES : 256;
   constexpr int ROWS = THREADS / LANES;  // rows in flight per CTA
   constexpr int WARPS = LANES / 32;      // warps per row
-  constexpr bool W_REG = LANES < 1024;   // 1024 threads have 64 registers each: they read the weight again
+  constexpr bool ROOMY = LANES < 1024;   // 1024 threads have 64 registers each: the weight is read again, no row ahead
   extern __shared__ float dw_shared[];   // [dim] when ROWS > 1
   __shared__ float red[2][THREADS / 32];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int units = p.dim / kUnit;
-  float w_reg[W_REG ? NV : 1][8], dw[NV][8];
+  float w_reg[ROOMY ? NV : 1][8], dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int u = lane + i * LANES;
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[i][k] = 0.f;
-    if constexpr (W_REG) {
+    if constexpr (ROOMY) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) w_reg[i][k] = 0.f;
       if (u < units) load_weight(p.w, p.w_dtype, u, w_reg[i]);
@@ -409,29 +411,38 @@ __global__ void __launch_bounds__(LANES > 256 ? LANES : 256) rms_norm_bwd_kernel
   }
   auto weight = [&](int i, float (&w)[8]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = W_REG ? w_reg[W_REG ? i : 0][k] : 0.f;
-    if (!W_REG && lane + i * LANES < units) load_weight(p.w, p.w_dtype, lane + i * LANES, w);
+    for (int k = 0; k < 8; ++k) w[k] = ROOMY ? w_reg[ROOMY ? i : 0][k] : 0.f;
+    if (!ROOMY && lane + i * LANES < units) load_weight(p.w, p.w_dtype, lane + i * LANES, w);
   };
   const float inv_dim = 1.f / (float)p.dim;
   int turn = 0;
-  // Every group of the CTA takes the same number of turns, since the sums of
-  // rows wider than a warp meet at a CTA barrier.
-  for (long long row0 = (long long)blockIdx.x * ROWS; row0 < p.rows; row0 += (long long)gridDim.x * ROWS, turn ^= 1) {
-    const long long row = row0 + group;
+  Raw8<T> dyv[NV], hv[NV], dhv[NV];
+  float rstd = 0.f;
+  auto load_row = [&](long long row, Raw8<T>(&a)[NV], Raw8<T>(&b)[NV], Raw8<T>(&c)[NV], float& s) {
     const bool live = row < p.rows;
-    Raw8<T> dyv[NV], hv[NV], dhv[NV];
-    float rstd = 0.f;
-    if (live) rstd = __ldg(p.rstd + row);
+    s = live ? __ldg(p.rstd + row) : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = lane + i * LANES;
-      dyv[i].zero(), hv[i].zero(), dhv[i].zero();
+      a[i].zero(), b[i].zero(), c[i].zero();
       if (live && u < units) {
-        dyv[i].load(static_cast<const T*>(p.dy) + row * p.sdy + u * kUnit);
-        hv[i].load(static_cast<const T*>(p.h) + row * p.sh + u * kUnit);
-        if (p.dh) dhv[i].load(static_cast<const T*>(p.dh) + row * p.sdh + u * kUnit);
+        a[i].load(static_cast<const T*>(p.dy) + row * p.sdy + u * kUnit);
+        b[i].load(static_cast<const T*>(p.h) + row * p.sh + u * kUnit);
+        if (p.dh) c[i].load(static_cast<const T*>(p.dh) + row * p.sdh + u * kUnit);
       }
     }
+  };
+  const long long step = (long long)gridDim.x * ROWS;
+  if (ROOMY) load_row((long long)blockIdx.x * ROWS + group, dyv, hv, dhv, rstd);
+  // Every group of the CTA takes the same number of turns, since the sums of
+  // rows wider than a warp meet at a CTA barrier.
+  for (long long row0 = (long long)blockIdx.x * ROWS; row0 < p.rows; row0 += step, turn ^= 1) {
+    const long long row = row0 + group;
+    const bool live = row < p.rows;
+    Raw8<T> dy_next[NV], h_next[NV], dh_next[NV];
+    float rstd_next = 0.f;
+    if (ROOMY) load_row(row + step, dy_next, h_next, dh_next, rstd_next);
+    else load_row(row, dyv, hv, dhv, rstd);
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -458,11 +469,10 @@ __global__ void __launch_bounds__(LANES > 256 ? LANES : 256) rms_norm_bwd_kernel
       for (int i = 0; i < WARPS; ++i) dot += r[group * WARPS + i];
     }
     const float mean = dot * inv_dim;
-    if (!live) continue;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = lane + i * LANES;
-      if (u >= units) continue;
+      if (!live || u >= units) continue;
       float a[8], b[8], d[8], w[8];
       dyv[i].unpack(a);
       hv[i].unpack(b);
@@ -476,6 +486,11 @@ __global__ void __launch_bounds__(LANES > 256 ? LANES : 256) rms_norm_bwd_kernel
       Raw8<T> o;
       o.pack(d);
       o.store(static_cast<T*>(p.dx) + row * p.sdx + u * kUnit);
+    }
+    if (ROOMY) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) dyv[i] = dy_next[i], hv[i] = h_next[i], dhv[i] = dh_next[i];
+      rstd = rstd_next;
     }
   }
   float* out = p.partial + (long long)blockIdx.x * p.dim;

@@ -38,13 +38,13 @@ def _as_list(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], what: str) ->
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         raise ValueError(f"{what}: no tensors (their device is where the norm goes)")
-    device = tensors[0].device
-    for t in tensors:
-        if t.dtype not in _DTYPE_CODES:
-            raise ValueError(f"{what}: gradients must be bf16, fp16 or fp32, got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{what}: gradients on {device} and {t.device}")
-    _lib.require_cuda(tensors[0], "gradients")
+    first = tensors[0]
+    for dtype in {t.dtype for t in tensors}:
+        if dtype not in _DTYPE_CODES:
+            raise ValueError(f"{what}: gradients must be bf16, fp16 or fp32, got {dtype}")
+    if len({t.get_device() for t in tensors}) != 1:
+        raise ValueError(f"{what}: gradients on {sorted({str(t.device) for t in tensors})}")
+    _lib.require_cuda(first, "gradients")
     return tensors
 
 
@@ -88,7 +88,7 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], *, norm_type
     code = _norm_code(norm_type, what)
     tensors = _as_list(tensors, what)
     device = tensors[0].device
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         # A view whose elements do not fill one stretch of memory is copied.
         tensors = [t if _dense(t) else t.contiguous() for t in tensors]
         table = _Table(tensors)
@@ -109,11 +109,11 @@ def _targets(tensors: list[torch.Tensor], out: Optional[Sequence[torch.Tensor]],
         if len(out) != len(tensors):
             raise ValueError(f"{what}: {len(out)} outputs for {len(tensors)} gradients")
         for t, o in zip(tensors, out):
-            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
+            if o.shape != t.shape or o.dtype != t.dtype or o.get_device() != t.get_device():
                 raise ValueError(f"{what}: an output is {tuple(o.shape)} {o.dtype} on {o.device}, "
                                  f"its gradient {tuple(t.shape)} {t.dtype} on {t.device}")
     for o in out:
-        if not _dense(o) and any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+        if not o.is_contiguous() and not _dense(o) and any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
             raise ValueError(f"{what}: cannot write to an expanded tensor of shape {tuple(o.shape)}")
     return out
 
@@ -146,12 +146,14 @@ def clip_grad_norm(
     out = _targets(tensors, out, what)
     device = tensors[0].device
     lib = _lib.lib()
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         # Views that do not fill one stretch of memory, or whose output lies in
         # another order, pass through a contiguous copy.
-        direct = [_dense(t) and _dense(o) and _same_order(t, o) for t, o in zip(tensors, out)]
-        src = [t if d else t.contiguous() for t, d in zip(tensors, direct)]
-        dst = [o if d else torch.empty_like(t) for t, o, d in zip(src, out, direct)]
+        src, dst, direct = tensors, out, None
+        if not (all(t.is_contiguous() for t in tensors) and all(o.is_contiguous() for o in out)):
+            direct = [_dense(t) and _dense(o) and _same_order(t, o) for t, o in zip(tensors, out)]
+            src = [t if d else t.contiguous() for t, d in zip(tensors, direct)]
+            dst = [o if d else torch.empty_like(t) for t, o, d in zip(src, out, direct)]
         table = _Table(src)
         targets = array("Q", [t.data_ptr() for t in dst])
         pointers, targets_at = table.pointers.buffer_info()[0], targets.buffer_info()[0]
@@ -172,9 +174,10 @@ def clip_grad_norm(
             status = lib.pcb_grad_scale(pointers, targets_at, *table.args(), norm.data_ptr(), max_norm, eps, stream)
             if status:
                 _lib.check(status, "pcb_grad_scale")
-        for t, o, d in zip(dst, out, direct):
-            if not d:
-                o.copy_(t)
+        if direct is not None:
+            for t, o, d in zip(dst, out, direct):
+                if not d:
+                    o.copy_(t)
     return norm
 
 

@@ -102,35 +102,45 @@ def rms_norm_quant(
     dim = x.shape[-1]
     x2 = _rows(x, dim)
     rows, device = x2.shape[0], x.device
-    with torch.cuda.device(device):
-        h = r2 = None
+    with _lib.on_device(device):
+        h = y = q = scale = None
+        xp, rp, hp, yp, qp, scp = x2.data_ptr(), None, None, None, None, None
+        rs = q_code = ss = sb = 0
         if residual is not None:
             _check_like(residual, x, "residual", what)
             r2 = _rows(residual, dim)
-            h = torch.empty((rows, dim), device=device, dtype=x.dtype)
-        y = torch.empty((rows, dim), device=device, dtype=x.dtype) if return_y or quant is None else None
-        rstd = torch.empty(rows, device=device, dtype=torch.float32)
-        q = scale = None
-        sb = 0
+            h = _like(x2)
+            rp, rs, hp = r2.data_ptr(), r2.stride(0), h.data_ptr()
+        if return_y or quant is None:
+            y = _like(x2)
+            yp = y.data_ptr()
         if quant is not None:
-            q = torch.empty((rows, dim), device=device, dtype=fp8_dtype)
-            blocks = -(-dim // _BLOCK)
-            scale = torch.empty((rows, blocks) if quant == "block" else (rows,), device=device, dtype=torch.float32)
-            sb = 1 if quant == "block" else 0
+            q = _like(x2, fp8_dtype)
+            if quant == "block":
+                ss, sb = -(-dim // _BLOCK), 1
+                scale = x2.new_empty((rows, ss), dtype=torch.float32)
+            else:
+                ss = 1
+                scale = x2.new_empty((rows,), dtype=torch.float32)
+            qp, q_code, scp = q.data_ptr(), _lib.PCB_DTYPE[fp8_dtype], scale.data_ptr()
+        rstd = x2.new_empty((rows,), dtype=torch.float32)
         status = _lib.lib().pcb_rms_norm_fwd(
-            x2.data_ptr(), _lib.PCB_DTYPE[x.dtype], rows, dim, x2.stride(0),
-            r2.data_ptr() if r2 is not None else None, r2.stride(0) if r2 is not None else 0,
-            weight.data_ptr(), _lib.PCB_DTYPE[weight.dtype], eps,
-            h.data_ptr() if h is not None else None, dim,
-            y.data_ptr() if y is not None else None, dim,
-            q.data_ptr() if q is not None else None, _lib.PCB_DTYPE[fp8_dtype] if q is not None else 0, dim,
-            scale.data_ptr() if scale is not None else None, scale.stride(0) if scale is not None else 0, sb,
+            xp, _lib.PCB_DTYPE[x.dtype], rows, dim, x2.stride(0), rp, rs,
+            weight.data_ptr(), _lib.PCB_DTYPE[weight.dtype], eps, hp, dim, yp, dim, qp, q_code, dim, scp, ss, sb,
             _QUANT_MODES[quant], int(pow2_scales), quant_eps, rstd.data_ptr(), _lib.stream_ptr(device))
         if status:
             _lib.check(status, "pcb_rms_norm_fwd")
-    result = _quant_result(q, scale, quant) if q is not None else None
-    return RMSNormResult(y.view(x.shape) if y is not None else None, result,
-                         h.view(x.shape) if h is not None else x, rstd)
+    if x2 is not x:
+        y = y.view(x.shape) if y is not None else None
+        h = h.view(x.shape) if h is not None else None
+    return RMSNormResult(y, _quant_result(q, scale, quant) if q is not None else None, h if h is not None else x, rstd)
+
+
+def _like(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A contiguous tensor of t's [rows, dim]."""
+    if t.is_contiguous():
+        return torch.empty_like(t) if dtype is None else torch.empty_like(t, dtype=dtype)
+    return t.new_empty(t.shape) if dtype is None else t.new_empty(t.shape, dtype=dtype)
 
 
 def _quant_result(q: torch.Tensor, scale: torch.Tensor, quant: str) -> QuantResult:
@@ -168,24 +178,24 @@ def rms_norm_backward(
         raise ValueError(f"{what}: rstd must be fp32 of shape ({rows},) on {device}, "
                          f"got {rstd.dtype} {tuple(rstd.shape)} on {rstd.device}")
     rstd = rstd.contiguous()
-    with torch.cuda.device(device):
-        dh2 = None
+    with _lib.on_device(device):
+        dhp, dhs = None, 0
         if dresidual is not None:
             _check_like(dresidual, h, "dresidual", what)
             dh2 = _rows(dresidual, dim)
-        dx = torch.empty((rows, dim), device=device, dtype=h.dtype)
-        dw = torch.empty(dim, device=device, dtype=weight.dtype)
+            dhp, dhs = dh2.data_ptr(), dh2.stride(0)
+        dx = _like(h2)
+        dw = torch.empty_like(weight)
         lib = _lib.lib()
         nbytes = lib.pcb_rms_norm_bwd_workspace_bytes(rows, dim)
-        workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+        workspace = h2.new_empty((nbytes,), dtype=torch.uint8)
         status = lib.pcb_rms_norm_bwd(
-            dy2.data_ptr(), dy2.stride(0), h2.data_ptr(), h2.stride(0), _lib.PCB_DTYPE[h.dtype], rows, dim,
-            dh2.data_ptr() if dh2 is not None else None, dh2.stride(0) if dh2 is not None else 0,
+            dy2.data_ptr(), dy2.stride(0), h2.data_ptr(), h2.stride(0), _lib.PCB_DTYPE[h.dtype], rows, dim, dhp, dhs,
             weight.data_ptr(), _lib.PCB_DTYPE[weight.dtype], rstd.data_ptr(), dx.data_ptr(), dim, dw.data_ptr(),
             workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
         if status:
             _lib.check(status, "pcb_rms_norm_bwd")
-    return dx.view(h.shape), dw
+    return dx if h2 is h else dx.view(h.shape), dw
 
 
 class _RMSNorm(torch.autograd.Function):
