@@ -24,11 +24,14 @@ so no transposed copies are made.
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 import torch.nn as nn
 
 from .impls.b200_per_block import b200_per_block_quant
 from .impls._common import bmm_scaled
+from .registry import QuantResult
 
 E4M3 = torch.float8_e4m3fn
 
@@ -113,15 +116,19 @@ def _gemm(a, a_scale, a_strides, qbm, b, b_scale, b_strides, qbn, out_dtype, blo
 
 class _FP8BlockLinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x2d: torch.Tensor, weight: torch.Tensor, w_data, w_scale, pow2: bool = False):
+    def forward(ctx, x2d: torch.Tensor, weight: torch.Tensor, w_data, w_scale, pow2: bool = False, x_data=None,
+                x_scale=None):
         # x2d [T, in] bf16; weight is the high-precision parameter (for its
-        # grad) and (w_data, w_scale) its 128x128 quantization.
+        # grad) and (w_data, w_scale) its 128x128 quantization; (x_data,
+        # x_scale) x2d's 1x128 one, where the caller has it.
         ctx.pow2 = pow2
-        qx = b200_per_block_quant(x2d, block_m=1, block_n=128, pow2_scales=pow2)  # [T, in], scales [T, in/128]
+        if x_data is None:
+            qx = b200_per_block_quant(x2d, block_m=1, block_n=128, pow2_scales=pow2)  # [T, in], scales [T, in/128]
+            x_data, x_scale = qx.tensor, qx.dequant_scale
         # y[T, out] = qx @ w.T: B = w.T is K-major (w stored [out, in]).
         wt = w_data.t()
         ws = w_scale
-        y = _gemm(qx.tensor, qx.dequant_scale, tuple(qx.dequant_scale.stride()), 1,
+        y = _gemm(x_data, x_scale, tuple(x_scale.stride()), 1,
                   wt, ws, (ws.stride(1), ws.stride(0)), 128, x2d.dtype, pow2)
         ctx.save_for_backward(x2d, w_data, w_scale)
         ctx.w_dtype = weight.dtype
@@ -144,7 +151,7 @@ class _FP8BlockLinearFn(torch.autograd.Function):
         b = qx_t.tensor                                            # [T, in], N-major
         sb = qx_t.dequant_scale                                    # [T/128, in] -> (kg, n)
         dw = _gemm(a, sa, (sa.stride(1), sa.stride(0)), 1, b, sb, tuple(sb.stride()), 1, ctx.w_dtype, pow2)
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None, None
 
 
 class FP8BlockLinear(nn.Linear):
@@ -160,7 +167,11 @@ class FP8BlockLinear(nn.Linear):
 
     scaling: str = "fp32"
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, quantized: Optional[QuantResult] = None) -> torch.Tensor:
+        """``quantized``: x's 1x128 quantization with this layer's kind of
+        scales, where the caller has it already (the norm before several
+        linears, ``rms_norm.rms_norm``); x itself is still what the weight
+        gradient quantizes along the tokens."""
         w = self.weight
         if isinstance(w, BlockFP8Weight):  # unsharded by the FSDP2 FP8 all-gather
             w_data, w_scale = w._data, w._scale
@@ -172,7 +183,14 @@ class FP8BlockLinear(nn.Linear):
         x2d = x.reshape(-1, shape[-1])
         if x2d.stride(-1) != 1:
             x2d = x2d.contiguous()
-        y = _FP8BlockLinearFn.apply(x2d, w_hp, w_data, w_scale, self.scaling == "e8m0")
+        x_data = x_scale = None
+        if quantized is not None:
+            x_data, x_scale = quantized.tensor, quantized.dequant_scale
+            blocks = (x2d.shape[0], -(-x2d.shape[1] // 128))
+            if x_data.shape != x2d.shape or x_data.dtype != E4M3 or tuple(x_scale.shape) != blocks:
+                raise ValueError(f"quantized input must be e4m3 {tuple(x2d.shape)} with 1x128 scales {blocks}, got "
+                                 f"{x_data.dtype} {tuple(x_data.shape)} with {tuple(x_scale.shape)}")
+        y = _FP8BlockLinearFn.apply(x2d, w_hp, w_data, w_scale, self.scaling == "e8m0", x_data, x_scale)
         y = y.reshape(*shape[:-1], y.shape[-1])
         if self.bias is not None:
             y = y + self.bias

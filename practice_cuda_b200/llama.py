@@ -8,6 +8,12 @@ head stay bf16: the head's 32000 output rows do not split into whole
 all-gather requires.  Attention itself runs in bf16 through
 ``scaled_dot_product_attention`` (it is not a linear layer).  Weights are
 random-init; inputs are synthetic token ids.
+
+``LlamaConfig.fused`` runs what lies between the linears on this package's
+kernels too: each norm adds the residual and quantizes its output once for the
+projections that share it (``rms_norm``), and the loss is taken without the
+logits (``linear_cross_entropy``).  It wants bf16 parameters (or FSDP2's bf16
+mixed precision).  ``train.py`` runs it with ``clip_grad_norm_``.
 """
 
 from __future__ import annotations
@@ -18,7 +24,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .cross_entropy import linear_cross_entropy
 from .fp8_linear import FP8BlockLinear
+from .rms_norm import rms_norm
 
 
 @dataclass
@@ -32,6 +40,7 @@ class LlamaConfig:
     norm_eps: float = 1e-5
     rope_theta: float = 10000.0
     linear_scaling: str = "fp32"  # FP8BlockLinear.scaling: "fp32" or "e8m0"
+    fused: bool = False  # norms with the residual and the FP8 output, loss without logits
 
     def linear_params(self) -> int:
         """Parameters in linear layers incl. the LM head (the FLOP basis)."""
@@ -71,6 +80,7 @@ class Block(nn.Module):
         super().__init__()
         d, f = cfg.dim, cfg.ffn_dim
         self.n_heads = cfg.n_heads
+        self.pow2 = cfg.linear_scaling == "e8m0"
         self.attn_norm = RMSNorm(d, cfg.norm_eps)
         self.wq = FP8BlockLinear(d, d, bias=False)
         self.wk = FP8BlockLinear(d, d, bias=False)
@@ -83,18 +93,36 @@ class Block(nn.Module):
         for lin in (self.wq, self.wk, self.wv, self.wo, self.w1, self.w3, self.w2):
             lin.scaling = cfg.linear_scaling
 
-    def forward(self, x, cos, sin):
-        b, t, d = x.shape
-        h = self.attn_norm(x)
+    def attention(self, h, cos, sin, hq=None):
+        b, t, d = h.shape
         hd = d // self.n_heads
-        q = self.wq(h).view(b, t, self.n_heads, hd).transpose(1, 2)
-        k = self.wk(h).view(b, t, self.n_heads, hd).transpose(1, 2)
-        v = self.wv(h).view(b, t, self.n_heads, hd).transpose(1, 2)
+        hq = () if hq is None else (hq,)
+        q = self.wq(h, *hq).view(b, t, self.n_heads, hd).transpose(1, 2)
+        k = self.wk(h, *hq).view(b, t, self.n_heads, hd).transpose(1, 2)
+        v = self.wv(h, *hq).view(b, t, self.n_heads, hd).transpose(1, 2)
         q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-        x = x + self.wo(a.transpose(1, 2).reshape(b, t, d))
+        return self.wo(a.transpose(1, 2).reshape(b, t, d))
+
+    def forward(self, x, cos, sin):
+        x = x + self.attention(self.attn_norm(x), cos, sin)
         h = self.mlp_norm(x)
         return x + self.w2(F.silu(self.w1(h)) * self.w3(h))
+
+
+class FusedBlock(Block):
+    """:class:`Block` with its norms on ``rms_norm``: (x, delta) goes from
+    block to block, delta being what the next norm adds to x."""
+
+    def norm(self, norm, x, delta):
+        if delta is None:
+            return rms_norm(x, norm.weight, eps=norm.eps, quant="block", pow2_scales=self.pow2)
+        return rms_norm(delta, norm.weight, x, eps=norm.eps, quant="block", pow2_scales=self.pow2)
+
+    def forward(self, x, delta, cos, sin):
+        h, x, hq = self.norm(self.attn_norm, x, delta)
+        h, x, hq = self.norm(self.mlp_norm, x, self.attention(h, cos, sin, hq))
+        return x, self.w2(F.silu(self.w1(h, hq)) * self.w3(h, hq))
 
 
 class Llama(nn.Module):
@@ -102,7 +130,7 @@ class Llama(nn.Module):
         super().__init__()
         self.cfg = cfg
         self.embed = nn.Embedding(cfg.vocab, cfg.dim)
-        self.layers = nn.ModuleList(Block(cfg) for _ in range(cfg.n_layers))
+        self.layers = nn.ModuleList((FusedBlock if cfg.fused else Block)(cfg) for _ in range(cfg.n_layers))
         self.norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.head = nn.Linear(cfg.dim, cfg.vocab, bias=False)
 
@@ -114,9 +142,24 @@ class Llama(nn.Module):
                     t = getattr(p, "_tensor", p)
                     t.normal_(0.0, 0.02, generator=g)
 
-    def forward(self, tokens):
+    def forward(self, tokens, targets=None):
+        """Logits, or with ``targets`` (token ids; -100 is left out) their mean cross entropy."""
         x = self.embed(tokens)
         cos, sin = rope_tables(self.cfg, tokens.device)
+        if self.cfg.fused:
+            delta = None
+            for layer in self.layers:
+                x, delta = layer(x, delta, cos, sin)
+            if delta is None:
+                h = rms_norm(x, self.norm.weight, eps=self.norm.eps)[0]
+            else:
+                h = rms_norm(delta, self.norm.weight, x, eps=self.norm.eps)[0]
+            if targets is not None:
+                return linear_cross_entropy(h, self.head.weight, targets)
+            return self.head(h)
         for layer in self.layers:
             x = layer(x, cos, sin)
-        return self.head(self.norm(x))
+        logits = self.head(self.norm(x))
+        if targets is None:
+            return logits
+        return F.cross_entropy(logits.float().view(-1, self.cfg.vocab), targets.reshape(-1))
