@@ -130,6 +130,9 @@ void shape(loss::Problem& q, int64_t m, int64_t n, int64_t k, int splits, bool p
   q.m_blocks = (int)up(m, pair ? loss::TILE : loss::BM);
   q.n_blocks = (int)up(n, tile_n);
   q.k_stages = (int)up(k, loss::BK);
+  const int chunks = std::max(1, (q.k_stages + loss::kChunkStages / 2) / loss::kChunkStages);
+  q.chunk_stages = (int)up(q.k_stages, chunks);  // even chunks: a last one of a stage or two would stall the others
+  q.a_rows = (int)std::min<int64_t>(loss::BM, up(m, 8) * 8);
   q.split_stages = (int)up(q.k_stages, splits);
   q.splits = (int)up(q.k_stages, q.split_stages);  // none of them empty
   q.tiles = q.m_blocks * q.n_blocks * q.splits;
@@ -256,10 +259,10 @@ int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw,
   loss::Problem& q = p.prob[0];
   const bool pair = on_pairs(tokens);
   p.tile_n = logit_tile(tokens, vocab);
-  if (!load_map(&q.a, x, dtype, dim, tokens, sx, loss::BM) ||
+  shape(q, tokens, vocab, dim, 1, pair, p.tile_n);
+  if (!load_map(&q.a, x, dtype, dim, tokens, sx, q.a_rows) ||
       !load_map(&q.b, weight, dtype, dim, vocab, sw, pair ? loss::TILE / 2 : p.tile_n))
     return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-  shape(q, tokens, vocab, dim, 1, pair, p.tile_n);
   p.num_tiles = q.tiles;
   p.partial = reinterpret_cast<float2*>(ws + plan.partial);
   p.target_logit = reinterpret_cast<float*>(ws + plan.target_logit);
@@ -318,10 +321,10 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     const bool pair = on_pairs(tokens);
     p.tile_n = logit_tile(tokens, cols);
     loss::Problem& q = p.prob[0];
-    ok &= load_map(&q.a, x, dtype, dim, tokens, sx, loss::BM);
+    shape(q, tokens, cols, dim, 1, pair, p.tile_n);
+    ok &= load_map(&q.a, x, dtype, dim, tokens, sx, q.a_rows);
     ok &= load_map(&q.b, w, dtype, dim, cols, sw, pair ? loss::TILE / 2 : p.tile_n);
     ok &= store_map(&q.c_box, g, dtype, cols, tokens, plan.pitch);
-    shape(q, tokens, cols, dim, 1, pair, p.tile_n);
     q.c_tma = pair;  // a single CTA's column halves need not be whole 64-column boxes
     q.c = g;
     q.scm = plan.pitch;
@@ -334,9 +337,9 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     int n = 0;
     if (dx) {
       loss::Problem& d = p.prob[n++];
-      ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, loss::BM);
-      ok &= load_b(d, w, dtype, dim, cols, sw);
       shape(d, tokens, dim, cols, plan.splits);
+      ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, d.a_rows);
+      ok &= load_b(d, w, dtype, dim, cols, sw);
       d.acc = acc;
       if (plan.splits > 1) d.acc_mode = loss::kAccSlab;
       else if (plan.pieces > 1) d.acc_mode = i == 0 ? loss::kAccWrite : i + 1 < plan.pieces ? loss::kAccAdd : loss::kAccLast;

@@ -40,7 +40,7 @@ constexpr int BM = 128;            // rows of the tile per CTA
 constexpr int TILE = 256;          // tile rows of the pair, and tile columns
 constexpr int BK = 64;             // K elements of a stage: one 128-byte swizzle atom of 16-bit values
 constexpr int UMMA_K = 16;
-constexpr int kChunkStages = 8;    // stages between two promotions of a logit's accumulator
+constexpr int kChunkStages = 8;    // stages between two promotions of a logit's accumulator, about
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int SLAB = 64 * BK * 2;           // 64 MN elements x 64 K rows of an MN-major operand
 constexpr int NACC = 2;
@@ -83,6 +83,8 @@ struct Problem {
   int m_blocks, n_blocks, splits;  // splits: parts of K, each a tile of its own
   int tiles;                       // m_blocks * n_blocks * splits
   int k_stages, split_stages;
+  int chunk_stages;  // of the logits: stages between two promotions
+  int a_rows;        // rows of A that a load brings (K-major A)
   int a_mn;   // A is M-major (kProducts; B is N-major there)
   int b_slabs;  // B's map takes both of a CTA's 64-column slabs in one load
   int c_tma;  // C leaves through TMA stores
@@ -253,7 +255,9 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
   constexpr int TILE_M = PAIR ? TILE : BM;
   constexpr bool CHUNKED = MODE != kProducts;
   // Bytes of a stage on the (leader's) full barrier.
-  const uint32_t stage_tx = PAIR ? 2 * (A_BYTES + S::B_BYTES) : A_BYTES + (uint32_t)p.tile_n * BK * 2;
+  // The rows of A below a_rows are loaded; those of the tile beyond it hold
+  // whatever was there and reach no row that is stored.
+  const uint32_t b_bytes = PAIR ? 2 * S::B_BYTES : (uint32_t)p.tile_n * BK * 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t s_base = smem_u32(smem);
@@ -323,7 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
             const uint32_t fb = bar_full + 8 * stage;
             const uint32_t a_dst = s_base + stage * A_BYTES;
             const uint32_t b_dst = s_base + S::OFF_B + stage * S::B_BYTES;
-            if (leader) mbar_arrive_expect_tx(fb, stage_tx);
+            const uint32_t a_bytes = (uint32_t)(PAIR ? 2 : 1) * (MODE == kProducts && q.a_mn ? A_BYTES : q.a_rows * BK * 2);
+            if (leader) mbar_arrive_expect_tx(fb, a_bytes + b_bytes);
             if constexpr (PAIR) {
               const uint32_t fbl = gemm::mapa_shared(fb, 0);
               if (MODE == kProducts && q.a_mn) {
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
               ok = false;
               break;
             }
-            const int stop = CHUNKED ? min(ks1, ks + kChunkStages) : ks1;
+            const int stop = CHUNKED ? min(ks1, ks + q.chunk_stages) : ks1;
             for (bool fresh = true; ks < stop; ++ks, fresh = false) {
               if (!wait(bar_full + 8 * stage, phase)) {
                 ok = false;
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
         }
         // The logits: the accumulators of every 512 products, summed.
         float acc[EPI_COLS];
-        const int chunks = (q.k_stages + kChunkStages - 1) / kChunkStages;
+        const int chunks = (q.k_stages + q.chunk_stages - 1) / q.chunk_stages;
         for (int ch = 0; ch < chunks; ++ch, ++acc_cnt) {
           const uint32_t abuf = acc_cnt % NACC;
           if (!wait_full(abuf)) {
