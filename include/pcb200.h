@@ -413,6 +413,15 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
                       const float* stats, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
                       int64_t sdw, int64_t piece, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * Copy of [rows, cols] 16-bit elements between row strides (in elements;
+ * columns contiguous on both sides): what gives pcb_linear_ce_* rows that
+ * start on 16-byte boundaries, or on 128-byte lines.  dst: 4-byte aligned, an
+ * even row stride.  Elements of dst beyond cols are not written.
+ */
+int pcb_repack_u16(const void* src, int64_t rows, int64_t cols, int64_t src_stride, void* dst, int64_t dst_stride,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -139,6 +139,7 @@ _SIGNATURES = {
     "pcb_grad_norm": (_i, [_vp, _vp, _vp, _i64, _i, _vp, _vp, _i64, _vp]),
     "pcb_grad_clip": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _f, _f, _vp, _vp, _i64, _vp]),
     "pcb_grad_scale": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _f, _f, _vp]),
+    "pcb_repack_u16": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "pcb_linear_ce_fwd_workspace_bytes": (_i64, [_i64, _i64]),
     "pcb_linear_ce_fwd": (
         _i,

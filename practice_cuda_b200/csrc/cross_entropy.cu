@@ -237,6 +237,20 @@ cudaError_t take_loss_device_error(unsigned int (&h)[3]) {
 
 extern "C" {
 
+int pcb_repack_u16(const void* src, int64_t rows, int64_t cols, int64_t src_stride, void* dst, int64_t dst_stride,
+                   void* stream) {
+  if (rows < 0 || cols < 0 || dst_stride < cols) return fail(PCB_ERR_INVALID, "bad repack sizes");
+  if (cols > (1 << 26)) return fail(PCB_ERR_UNSUPPORTED, "repack: dimension too large");
+  if (rows == 0 || cols == 0) return PCB_OK;
+  if (!src || !dst) return fail(PCB_ERR_INVALID, "null pointer");
+  if (!aligned(src, 2) || !aligned(dst, 4) || dst_stride % 2 != 0)
+    return fail(PCB_ERR_LAYOUT, "repack: dst needs 4-byte aligned rows");
+  const int64_t grid = std::min<int64_t>(rows, (int64_t)device_info().sm_count * 8);
+  loss::repack_rows_kernel<<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(
+      static_cast<const uint16_t*>(src), rows, (int)cols, src_stride, static_cast<uint32_t*>(dst), dst_stride / 2);
+  return check_launch("repack_rows_kernel");
+}
+
 int64_t pcb_linear_ce_fwd_workspace_bytes(int64_t tokens, int64_t vocab) {
   if (tokens <= 0 || vocab <= 0) return 0;
   return FwdPlan(tokens, vocab).bytes;

@@ -746,6 +746,41 @@ __global__ void __launch_bounds__(1024) loss_weights_kernel(const float* dloss, 
   if (threadIdx.x == 0) *alpha = up * (1.f / kGradScale);
 }
 
+// Rows copied to another stride, two elements (a word of dst) a thread at a
+// time: a row that starts on an odd element is read as the aligned words around it
+// and shifted, so loads and stores stay whole and contiguous across the warp.
+constexpr int kRepackLoads = 8;
+__global__ void __launch_bounds__(256) repack_rows_kernel(const uint16_t* src, long long rows, int cols,
+                                                          long long src_stride, uint32_t* dst, long long dst_words) {
+  const int words = (cols + 1) / 2;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src + row * src_stride);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+    const bool odd = at & 2;
+    uint32_t* out = dst + row * dst_words;
+    for (int j0 = threadIdx.x; j0 < words; j0 += 256 * kRepackLoads) {
+      uint32_t a[kRepackLoads], b[kRepackLoads];
+#pragma unroll
+      for (int k = 0; k < kRepackLoads; ++k) {
+        const int j = j0 + k * 256;
+        a[k] = b[k] = 0;
+        if (j < words) {
+          a[k] = __ldg(w + j);
+          if (odd && 2 * j + 1 < cols) b[k] = __ldg(w + j + 1);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRepackLoads; ++k) {
+        const int j = j0 + k * 256;
+        if (j >= words) break;
+        const uint32_t v = odd ? __funnelshift_r(a[k], b[k], 16) : a[k];
+        if (2 * j + 1 < cols) out[j] = v;
+        else *reinterpret_cast<uint16_t*>(out + j) = (uint16_t)v;
+      }
+    }
+  }
+}
+
 // dX from the parts of K: the fp32 accumulators of every part summed in order.
 struct JoinArgs {
   const float4* acc;

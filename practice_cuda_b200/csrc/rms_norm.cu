@@ -12,29 +12,55 @@ bool fits_units(const void* p, int64_t row_stride, int es) {
   return aligned(p, 16) && (row_stride * es) % 16 == 0;
 }
 
-template <int XT, int YT, int LANES, int NV>
-int launch_norm_fwd(const norm::FwdArgs& p, cudaStream_t s) {
-  constexpr int threads = LANES > 32 ? LANES : 256, rows = threads / LANES;
-  const int64_t grid = (p.rows + rows - 1) / rows;
-  norm::rms_norm_fwd_kernel<XT, YT, LANES, NV><<<(unsigned)grid, threads, 0, s>>>(p);
+template <int XT, int YT, int LANES, int NV, int MAX_THREADS>
+int launch_norm_fwd(const norm::FwdArgs& p, int threads, cudaStream_t s) {
+  const int64_t rows = LANES ? MAX_THREADS / (LANES ? LANES : 1) : 1;  // per CTA
+  norm::rms_norm_fwd_kernel<XT, YT, LANES, NV, MAX_THREADS>
+      <<<(unsigned)((p.rows + rows - 1) / rows), LANES ? MAX_THREADS : threads, 0, s>>>(p);
   return check_launch("rms_norm_fwd_kernel");
 }
 
-// Lanes per row: four units of eight elements a lane keep a row in registers
-// at 32 values a thread; rows up to 1024 wide need no barrier.
+int threads_of(int items, int per_thread, int step) {
+  const int t = (items + per_thread - 1) / per_thread;
+  return (t + step - 1) / step * step;
+}
+
+// False: the rows are too wide for these kernels.
+template <int XT, int YT, int WT>
+bool launch_norm_fwd_elems(const norm::FwdArgs& p, cudaStream_t s) {
+  const int threads = threads_of(p.dim, norm::kElems, 128);
+  if (p.dim <= 32 * norm::kElems)
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, true, 256><<<(unsigned)((p.rows + 7) / 8), 256, 0, s>>>(p);
+  else if (threads <= 512)
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, 512><<<(unsigned)p.rows, threads, 0, s>>>(p);
+  else if (threads <= 1024)
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, 1024><<<(unsigned)p.rows, threads, 0, s>>>(p);
+  else
+    return false;
+  return true;
+}
+
+// Four units of eight elements a lane keep a row in registers at 32 values a
+// thread.  Rows up to 1024 wide are a warp's (up to 128 wide, half a warp's)
+// and need no barrier; wider ones get a CTA of as many warps as they need
+// (128 threads at 4096: 97 us for 16384 rows of bf16 on a B200, 101 us with two
+// units a lane).
 template <int XT, int YT>
 int dispatch_norm_fwd(const norm::FwdArgs& p, bool vec, cudaStream_t s) {
   const int units = p.dim / norm::kUnit;
   if (vec && units <= 4096) {
-    if (units <= 32) return launch_norm_fwd<XT, YT, 32, 1>(p, s);
-    if (units <= 64) return launch_norm_fwd<XT, YT, 32, 2>(p, s);
-    if (units <= 128) return launch_norm_fwd<XT, YT, 32, 4>(p, s);
-    if (units <= 256) return launch_norm_fwd<XT, YT, 128, 2>(p, s);
-    if (units <= 512) return launch_norm_fwd<XT, YT, 256, 2>(p, s);
-    if (units <= 1024) return launch_norm_fwd<XT, YT, 256, 4>(p, s);
-    if (units <= 2048) return launch_norm_fwd<XT, YT, 512, 4>(p, s);
-    return launch_norm_fwd<XT, YT, 1024, 4>(p, s);
+    if (units <= 16) return launch_norm_fwd<XT, YT, 16, 1, 256>(p, 0, s);
+    if (units <= 32) return launch_norm_fwd<XT, YT, 32, 1, 256>(p, 0, s);
+    if (units <= 64) return launch_norm_fwd<XT, YT, 32, 2, 256>(p, 0, s);
+    if (units <= 128) return launch_norm_fwd<XT, YT, 32, 4, 256>(p, 0, s);
+    if (units <= 2048) return launch_norm_fwd<XT, YT, 0, 4, 512>(p, threads_of(units, 4, 32), s);
+    return launch_norm_fwd<XT, YT, 0, 4, 1024>(p, threads_of(units, 4, 32), s);
   }
+  const bool same = p.w_dtype == XT, f32 = p.w_dtype == PCB_DTYPE_F32;
+  if ((same && launch_norm_fwd_elems<XT, YT, XT>(p, s)) ||
+      (!same && f32 && launch_norm_fwd_elems<XT, YT, PCB_DTYPE_F32>(p, s)))
+    return check_launch("rms_norm_fwd_elems_kernel");
+  // Rows too wide, or a weight of the other 16-bit type.
   const int64_t grid = std::min<int64_t>(p.rows, (int64_t)device_info().sm_count * 8);
   norm::rms_norm_fwd_generic_kernel<XT, YT><<<(unsigned)grid, norm::kGenericThreads, 0, s>>>(p);
   return check_launch("rms_norm_fwd_generic_kernel");
@@ -59,6 +85,26 @@ int launch_norm_bwd(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
   return check_launch("rms_norm_bwd_kernel");
 }
 
+// False: the rows are too wide for these kernels.  Eight columns a thread keep
+// clear of register spills, sixteen take the widths beyond.
+template <int XT, int WT>
+bool launch_norm_bwd_elems(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
+  if (p.dim <= 32 * norm::kElems) {
+    parts = norm_bwd_ctas(p.rows, 8, 2);
+    norm::rms_norm_bwd_elems_kernel<XT, WT, true, norm::kElems, 256><<<parts, 256, 0, s>>>(p);
+  } else if (p.dim <= 512 * 8) {
+    const int threads = threads_of(p.dim, 8, 32);
+    parts = norm_bwd_ctas(p.rows, 1, std::min(kNormBwdMost, 1024 / threads));
+    norm::rms_norm_bwd_elems_kernel<XT, WT, false, 8, 512><<<parts, threads, 0, s>>>(p);
+  } else if (p.dim <= 512 * 16) {
+    parts = norm_bwd_ctas(p.rows, 1, 1);
+    norm::rms_norm_bwd_elems_kernel<XT, WT, false, 16, 512><<<parts, threads_of(p.dim, 16, 32), 0, s>>>(p);
+  } else {
+    return false;
+  }
+  return true;
+}
+
 template <int XT>
 int dispatch_norm_bwd(const norm::BwdArgs& p, bool vec, int& parts, cudaStream_t s) {
   const int units = p.dim / norm::kUnit;
@@ -73,6 +119,10 @@ int dispatch_norm_bwd(const norm::BwdArgs& p, bool vec, int& parts, cudaStream_t
     if (units <= 1024) return launch_norm_bwd<XT, 1024 / NV, NV>(p, parts, s);
     return launch_norm_bwd<XT, 1024, 2>(p, parts, s);
   }
+  const bool same = p.w_dtype == XT, f32 = p.w_dtype == PCB_DTYPE_F32;
+  if ((same && launch_norm_bwd_elems<XT, XT>(p, parts, s)) ||
+      (!same && f32 && launch_norm_bwd_elems<XT, PCB_DTYPE_F32>(p, parts, s)))
+    return check_launch("rms_norm_bwd_elems_kernel");
   parts = norm_bwd_ctas(p.rows, 1, kNormBwdMost);
   const bool in_smem = (int64_t)p.dim * 4 <= kNormDwSmem;
   const int smem = in_smem ? p.dim * 4 : 0;

@@ -148,36 +148,81 @@ __device__ __forceinline__ void load_weight(const void* w, int dt, int u, float 
   }
 }
 
-// Sum / unsigned max over the LANES threads that share a row (a warp, or the
-// whole CTA through `red`, one word per warp).  Every thread gets the result,
-// formed in the same order.
+// Sum and unsigned maximum over a warp's groups of LANES lanes; every lane
+// gets the result, formed in the same order.
 template <int LANES>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (LANES > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < LANES / 32; ++i) v += red[i];
-    __syncthreads();
-  }
+  for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 template <int LANES>
-__device__ __forceinline__ uint32_t row_max(uint32_t v, float* red) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if constexpr (LANES > 32) {
-    uint32_t* r = reinterpret_cast<uint32_t*>(red);
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if constexpr (LANES == 32) {
+    return __reduce_max_sync(0xffffffffu, v);
+  } else {
 #pragma unroll
-    for (int i = 0; i < LANES / 32; ++i) v = max(v, r[i]);
-    __syncthreads();
+    for (int o = LANES / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
   }
+}
+// The same over the CTA, in one barrier; `red` is not used again.
+struct CtaRed {
+  float sum[32];
+  uint32_t top[32];
+};
+__device__ __forceinline__ void cta_sum_max(float& v, uint32_t& top, CtaRed& red) {
+  v = lanes_sum<32>(v);
+  top = lanes_max<32>(top);
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) red.sum[warp] = v, red.top[warp] = top;
+  __syncthreads();
+  v = 0.f, top = 0;
+  for (int i = 0; i < warps; ++i) v += red.sum[i], top = max(top, red.top[i]);
+}
+// For loops over rows: two barriers, `red` can be used again.
+template <int THREADS>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = lanes_sum<32>(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) v += red[i];
+  __syncthreads();
   return v;
+}
+template <int THREADS>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, float* red) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(red);
+  v = lanes_max<32>(v);
+  if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) v = max(v, r[i]);
+  __syncthreads();
+  return v;
+}
+
+// max(|m|, |a|, |b|), NaN if any of them is.
+__device__ __forceinline__ float max3_abs(float m, float a, float b) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
+  return r;
+}
+// f s w of eight elements.
+__device__ __forceinline__ void scale8(float (&f)[8], float s, const float (&w)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) {
+    const float2 t = __fmul2_rn(__fmul2_rn(make_float2(f[k], f[k + 1]), make_float2(s, s)), make_float2(w[k], w[k + 1]));
+    f[k] = t.x, f[k + 1] = t.y;
+  }
+}
+__device__ __forceinline__ float max8_abs(float m, const float (&f)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) m = max3_abs(m, f[k], f[k + 1]);
+  return m;
 }
 
 // 1 / sqrt(mean + eps), correctly rounded: an error here would move a whole
@@ -196,87 +241,98 @@ __device__ __forceinline__ float quant_factor(uint32_t amax_bits, const FwdArgs&
   return f;
 }
 
-// Forward, one row per LANES threads, the whole row in registers (NV units of
-// eight elements a lane): one reading of x and r, one writing of each output.
-// Units 16 lanes wide are one 128-column block, so its amax is a 16-lane
-// shuffle.  Bound by HBM traffic.
-template <int XT, int YT, int LANES, int NV>
-__global__ void __launch_bounds__(LANES > 32 ? LANES : 256) rms_norm_fwd_kernel(const FwdArgs p) {
+// Forward, the whole row in registers (NV units of eight elements a lane): one
+// reading of x and r, one writing of each output.  A row is LANES (16 or 32)
+// lanes of a warp, or with LANES == 0 a CTA of as many threads as the width needs.
+// Sixteen lanes hold one 128-column block, so its amax is a shuffle.  A row's
+// scale needs max |h s w|, taken as s max |h w| so that the one barrier of the sum
+// serves it too.  A CTA ends with its row: many rows at once hide a row's way
+// through its loads, sum and stores better than resident CTAs that load the next
+// row ahead (16384 x 4096 bf16 on a B200, every output: 98 us against 116; weights
+// loaded with the row instead of where they are used, which costs registers: 122).
+// Bound by HBM traffic where all outputs are wanted (606 MB in 98 us, 6.2 TB/s), by
+// instruction issue where one FP8 byte is written for two bytes read.
+template <int XT, int YT, int LANES, int NV, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS) rms_norm_fwd_kernel(const FwdArgs p) {
   using T = typename InType<XT>::T;
-  constexpr int ROWS = LANES > 32 ? 1 : 256 / LANES;  // rows per CTA
-  __shared__ float red[32];
-  const int lane = threadIdx.x % LANES;
-  const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / LANES;
-  if (row >= p.rows) return;  // a whole warp at a time
-  const int units = p.dim / kUnit;
-  const T* x = static_cast<const T*>(p.x) + row * p.sx;
-  const T* r = p.res ? static_cast<const T*>(p.res) + row * p.sr : nullptr;
+  constexpr int ROWS = LANES ? MAX_THREADS / (LANES ? LANES : 1) : 1;  // per CTA
+  const int lanes = LANES ? LANES : (int)blockDim.x;
+  const int lane = LANES ? (int)threadIdx.x % (LANES ? LANES : 1) : (int)threadIdx.x;
+  const long long row = (long long)blockIdx.x * ROWS + (LANES ? threadIdx.x / (LANES ? LANES : 1) : 0);
+  const bool live = row < p.rows;  // the lanes of a warp stay together for its shuffles
+  const int units = live ? p.dim / kUnit : 0;
   Raw8<T> hv[NV], rv[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int u = lane + i * LANES;
+    const int u = lane + i * lanes;
+    hv[i].zero(), rv[i].zero();
     if (u < units) {
-      hv[i].load(x + u * kUnit);
-      if (r) rv[i].load(r + u * kUnit);
-    } else {
-      hv[i].zero();
-      rv[i].zero();
+      hv[i].load(static_cast<const T*>(p.x) + row * p.sx + u * kUnit);
+      if (p.res) rv[i].load(static_cast<const T*>(p.res) + row * p.sr + u * kUnit);
     }
   }
-  float ss = 0.f;
+  float2 ss2 = make_float2(0.f, 0.f);
+  float top_hw = 0.f;  // max |h w|, for a row's scale
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    const int u = lane + i * lanes;
     float f[8];
     hv[i].unpack(f);
-    if (r) {
+    if (p.res) {
       float g[8];
       rv[i].unpack(g);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] += g[k];
+      for (int k = 0; k < 8; k += 2) {
+        const float2 t = __fadd2_rn(make_float2(f[k], f[k + 1]), make_float2(g[k], g[k + 1]));
+        f[k] = t.x, f[k + 1] = t.y;
+      }
       hv[i].pack(f);  // rounded to T: the residual that later layers read
       hv[i].unpack(f);
-      const int u = lane + i * LANES;
       if (u < units) hv[i].store(static_cast<T*>(p.h) + row * p.sh + u * kUnit);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fmaf(f[k], f[k], ss);
+    for (int k = 0; k < 8; k += 2) {
+      const float2 t = make_float2(f[k], f[k + 1]);
+      ss2 = __ffma2_rn(t, t, ss2);
+    }
+    if (p.quant_mode == kQuantRow && u < units) {
+      float w[8];
+      load_weight(p.w, p.w_dtype, u, w);
+      #pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= w[k];
+      top_hw = max8_abs(top_hw, f);
+    }
   }
-  const float rstd = rstd_of(row_sum<LANES>(ss, red), p.dim, p.eps);
-  if (lane == 0) p.rstd[row] = rstd;
+  float ss = ss2.x + ss2.y;
+  uint32_t top = abs_bits(top_hw);
+  if constexpr (LANES == 0) {
+    __shared__ CtaRed red;
+    cta_sum_max(ss, top, red);
+  } else {
+    ss = lanes_sum<LANES ? LANES : 32>(ss);
+    if (p.quant_mode == kQuantRow) top = lanes_max<LANES ? LANES : 32>(top);
+  }
+  const float rstd = rstd_of(ss, p.dim, p.eps);
+  if (live && lane == 0) p.rstd[row] = rstd;
 
   float factor = 0.f;
   if (p.quant_mode == kQuantRow) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int u = lane + i * LANES;
-      if (u < units) {
-        float f[8], w[8];
-        hv[i].unpack(f);
-        load_weight(p.w, p.w_dtype, u, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) amax = max(amax, abs_bits(f[k] * rstd * w[k]));
-      }
-    }
     float scale;
-    factor = quant_factor<YT>(row_max<LANES>(amax, red), p, scale);
-    if (lane == 0) p.scale[row * p.ssr] = scale;
+    factor = quant_factor<YT>(abs_bits(__uint_as_float(top) * rstd), p, scale);
+    if (live && lane == 0) p.scale[row * p.ssr] = scale;
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int u = lane + i * LANES;
+    const int u = lane + i * lanes;
     const bool in = u < units;
     float f[8];
-    uint32_t amax = 0;
+    float m = 0.f;
     if (in) {
       float w[8];
       hv[i].unpack(f);
       load_weight(p.w, p.w_dtype, u, w);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        f[k] = f[k] * rstd * w[k];
-        amax = max(amax, abs_bits(f[k]));
-      }
+      scale8(f, rstd, w);
+      m = max8_abs(0.f, f);
       if (p.y) {
         Raw8<T> o;
         o.pack(f);
@@ -285,24 +341,136 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256) rms_norm_fwd_kernel(
     }
     if (p.quant_mode == kQuantNone) continue;
     if (p.quant_mode == kQuantBlock) {
-#pragma unroll
-      for (int o = 8; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       float scale;
-      factor = quant_factor<YT>(amax, p, scale);
+      factor = quant_factor<YT>(lanes_max<16>(abs_bits(m)), p, scale);
       if (in && (lane & 15) == 0) p.scale[row * p.ssr + (long long)(u >> 4) * p.ssb] = scale;
     }
     if (in) {
-      uint2 o;
-      o.x = cvt2_fp8<YT>(__fmul_rn(f[0], factor), __fmul_rn(f[1], factor)) |
-            (uint32_t)cvt2_fp8<YT>(__fmul_rn(f[2], factor), __fmul_rn(f[3], factor)) << 16;
-      o.y = cvt2_fp8<YT>(__fmul_rn(f[4], factor), __fmul_rn(f[5], factor)) |
-            (uint32_t)cvt2_fp8<YT>(__fmul_rn(f[6], factor), __fmul_rn(f[7], factor)) << 16;
+      uint32_t q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 t = __fmul2_rn(make_float2(f[2 * k], f[2 * k + 1]), make_float2(factor, factor));
+        q[k] = cvt2_fp8<YT>(t.x, t.y);
+      }
+      const uint2 o = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
       *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.q) + row * p.sq + u * kUnit) = o;
     }
   }
 }
 
-// Forward for any width, stride and alignment: one CTA per row, element by
+// The same element by element, for rows that do not suit 16-byte loads (odd
+// widths, strides or alignments): a thread holds the columns t, t + threads, ...
+// (NE of them), so every access of a warp is contiguous and all of a row's loads
+// are in flight together.  A row is a warp's (widths up to 32 NE) or a CTA's,
+// whose threads are a multiple of 128: four warps hold a 128-column block.
+constexpr int kElems = 16;
+// WT is the weight's type: x's or fp32.
+template <int XT, int YT, int WT, bool WARP, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS) rms_norm_fwd_elems_kernel(const FwdArgs p) {
+  using T = typename InType<XT>::T;
+  using W = typename InType<WT>::T;
+  constexpr int NE = kElems;
+  const int threads = WARP ? 32 : (int)blockDim.x;
+  const int t = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
+  const long long row = WARP ? (long long)blockIdx.x * (MAX_THREADS / 32) + (threadIdx.x >> 5) : (long long)blockIdx.x;
+  if (row >= p.rows) return;  // a whole warp, or nobody
+  const T* x = static_cast<const T*>(p.x) + row * p.sx;
+  T raw[NE], res[NE];
+  W w[NE];
+#pragma unroll
+  for (int k = 0; k < NE; ++k) {
+    const int c = t + k * threads;
+    raw[k] = res[k] = from_f32<T>(0.f);
+    w[k] = from_f32<W>(0.f);
+    if (c < p.dim) {
+      raw[k] = x[c];
+      w[k] = static_cast<const W*>(p.w)[c];
+      if (p.res) res[k] = static_cast<const T*>(p.res)[row * p.sr + c];
+    }
+  }
+  float f[NE];
+  float ss = 0.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < NE; ++k) {
+    const int c = t + k * threads;
+    f[k] = InType<XT>::to_f32(raw[k]);
+    if (p.res) {
+      const T h = from_f32<T>(f[k] + InType<XT>::to_f32(res[k]));
+      f[k] = InType<XT>::to_f32(h);
+      if (c < p.dim) static_cast<T*>(p.h)[row * p.sh + c] = h;
+    }
+    ss = fmaf(f[k], f[k], ss);
+    if (p.quant_mode == kQuantRow) top = max(top, abs_bits(f[k] * InType<WT>::to_f32(w[k])));
+  }
+  if constexpr (WARP) {
+    ss = lanes_sum<32>(ss);
+    top = lanes_max<32>(top);
+  } else {
+    __shared__ CtaRed red;
+    cta_sum_max(ss, top, red);
+  }
+  const float rstd = rstd_of(ss, p.dim, p.eps);
+  if (t == 0) p.rstd[row] = rstd;
+#pragma unroll
+  for (int k = 0; k < NE; ++k) {
+    const int c = t + k * threads;
+    f[k] = f[k] * rstd * InType<WT>::to_f32(w[k]);
+    if (p.y && c < p.dim) static_cast<T*>(p.y)[row * p.sy + c] = from_f32<T>(f[k]);
+  }
+  if (p.quant_mode == kQuantNone) return;
+  uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.sq;
+  if (p.quant_mode == kQuantRow) {
+    float scale;
+    const float factor = quant_factor<YT>(abs_bits(__uint_as_float(top) * rstd), p, scale);
+    if (t == 0) p.scale[row * p.ssr] = scale;
+#pragma unroll
+    for (int k = 0; k < NE; ++k)
+      if (t + k * threads < p.dim) q[t + k * threads] = cvt1_fp8<YT>(__fmul_rn(f[k], factor));
+    return;
+  }
+  if constexpr (WARP) {
+#pragma unroll
+    for (int b = 0; b < NE / 4; ++b) {  // a warp's four columns a lane
+      uint32_t amax = 0;
+#pragma unroll
+      for (int k = 4 * b; k < 4 * b + 4; ++k)
+        if (t + k * 32 < p.dim) amax = max(amax, abs_bits(f[k]));
+      if (b * kQuantCols >= p.dim) break;
+      float scale;
+      const float factor = quant_factor<YT>(lanes_max<32>(amax), p, scale);
+      if (t == 0) p.scale[row * p.ssr + (long long)b * p.ssb] = scale;
+#pragma unroll
+      for (int k = 4 * b; k < 4 * b + 4; ++k)
+        if (t + k * 32 < p.dim) q[t + k * 32] = cvt1_fp8<YT>(__fmul_rn(f[k], factor));
+    }
+  } else {
+    // Block b of the row: the four warps 4 (b % groups) .. + 3 in pass b / groups.
+    __shared__ uint32_t tops[NE][MAX_THREADS / 32];
+    __shared__ float factors[NE * MAX_THREADS / 128];
+    const int warp = t >> 5, groups = threads / 128;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const uint32_t m = lanes_max<32>(t + k * threads < p.dim ? abs_bits(f[k]) : 0u);
+      if ((t & 31) == 0) tops[k][warp] = m;
+    }
+    __syncthreads();
+    for (int b = t; b * kQuantCols < p.dim; b += threads) {
+      const uint32_t* m = tops[b / groups] + 4 * (b % groups);
+      float scale;
+      factors[b] = quant_factor<YT>(max(max(m[0], m[1]), max(m[2], m[3])), p, scale);
+      p.scale[row * p.ssr + (long long)b * p.ssb] = scale;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const int c = t + k * threads;
+      if (c < p.dim) q[c] = cvt1_fp8<YT>(__fmul_rn(f[k], factors[k * groups + (warp >> 2)]));
+    }
+  }
+}
+
+// Forward for rows too wide for registers: one CTA per row, element by
 // element, h read again (from L1 / L2) for each pass over the row.
 template <int XT, int YT>
 __global__ void __launch_bounds__(kGenericThreads) rms_norm_fwd_generic_kernel(const FwdArgs p) {
@@ -524,7 +692,91 @@ __global__ void __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : 2
   }
 }
 
-// Backward for any width, stride and alignment: a CTA per row, element by
+// Backward element by element, for rows that do not suit 16-byte loads: as in
+// the forward, a thread holds the columns t, t + threads, ... with their share of
+// dw, over all rows of its warp (widths up to 32 NE) or CTA.
+template <int XT, int WT, bool WARP, int NE, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS) rms_norm_bwd_elems_kernel(const BwdArgs p) {
+  using T = typename InType<XT>::T;
+  using W = typename InType<WT>::T;
+  constexpr int ROWS = WARP ? MAX_THREADS / 32 : 1;
+  __shared__ float red[2][MAX_THREADS / 32];
+  __shared__ float dw_shared[WARP ? 32 * NE : 1];
+  const int threads = WARP ? 32 : (int)blockDim.x;
+  const int t = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
+  const int group = WARP ? (int)threadIdx.x >> 5 : 0;
+  const float inv_dim = 1.f / (float)p.dim;
+  float dw[NE];
+  W w[NE];
+#pragma unroll
+  for (int k = 0; k < NE; ++k) {
+    dw[k] = 0.f;
+    w[k] = t + k * threads < p.dim ? static_cast<const W*>(p.w)[t + k * threads] : from_f32<W>(0.f);
+  }
+  int turn = 0;
+  for (long long row = (long long)blockIdx.x * ROWS + group; row < p.rows; row += (long long)gridDim.x * ROWS, turn ^= 1) {
+    T a[NE], h[NE], d[NE];
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const int c = t + k * threads;
+      a[k] = h[k] = d[k] = from_f32<T>(0.f);
+      if (c < p.dim) {
+        a[k] = static_cast<const T*>(p.dy)[row * p.sdy + c];
+        h[k] = static_cast<const T*>(p.h)[row * p.sh + c];
+        if (p.dh) d[k] = static_cast<const T*>(p.dh)[row * p.sdh + c];
+      }
+    }
+    const float rstd = __ldg(p.rstd + row);
+    float dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const float n = InType<XT>::to_f32(h[k]) * rstd, g = InType<XT>::to_f32(a[k]);  // zeros beyond the width
+      dot = fmaf(n, g * InType<WT>::to_f32(w[k]), dot);
+      dw[k] = fmaf(g, n, dw[k]);
+    }
+    dot = lanes_sum<32>(dot);
+    if constexpr (!WARP) {
+      // Two buffers in turn: one barrier a row is enough.
+      float* r = red[turn];
+      if ((t & 31) == 0) r[t >> 5] = dot;
+      __syncthreads();
+      dot = 0.f;
+      for (int i = 0; i < threads / 32; ++i) dot += r[i];
+    }
+    const float mean = dot * inv_dim;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const int c = t + k * threads;
+      if (c < p.dim) {
+        const float v = rstd * (InType<XT>::to_f32(a[k]) * InType<WT>::to_f32(w[k]) -
+                                InType<XT>::to_f32(h[k]) * rstd * mean);
+        static_cast<T*>(p.dx)[row * p.sdx + c] = from_f32<T>(p.dh ? v + InType<XT>::to_f32(d[k]) : v);
+      }
+    }
+  }
+  float* out = p.partial + (long long)blockIdx.x * p.dim;
+  if constexpr (WARP) {
+    // The warps add their shares one after the other: a fixed order.
+    for (int g = 0; g < ROWS; ++g) {
+      __syncthreads();
+      if (group == g) {
+#pragma unroll
+        for (int k = 0; k < NE; ++k) {
+          const int c = t + k * 32;
+          if (c < p.dim) dw_shared[c] = g == 0 ? dw[k] : dw_shared[c] + dw[k];
+        }
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.dim; c += MAX_THREADS) out[c] = dw_shared[c];
+  } else {
+#pragma unroll
+    for (int k = 0; k < NE; ++k)
+      if (t + k * threads < p.dim) out[t + k * threads] = dw[k];
+  }
+}
+
+// Backward for rows too wide for registers: a CTA per row, element by
 // element.  A thread owns the columns t, t + 256, ... over all of its rows and
 // keeps their share of dw in shared memory, or in its row of `partial` where
 // that does not fit (the launch then asks for no shared memory).
