@@ -24,6 +24,9 @@ import torch.distributed as dist
 from . import _lib
 
 _NORM_TYPES = {2.0: 0, math.inf: 1}
+# Called through map(): one pass over many small tensors is what a call costs.
+_pointer, _numel, _device, _contiguous = (
+    torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous)
 _DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -42,7 +45,7 @@ def _as_list(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], what: str) ->
     for dtype in {t.dtype for t in tensors}:
         if dtype not in _DTYPE_CODES:
             raise ValueError(f"{what}: gradients must be bf16, fp16 or fp32, got {dtype}")
-    if len({t.get_device() for t in tensors}) != 1:
+    if len(set(map(_device, tensors))) != 1:
         raise ValueError(f"{what}: gradients on {sorted({str(t.device) for t in tensors})}")
     _lib.require_cuda(first, "gradients")
     return tensors
@@ -68,8 +71,8 @@ class _Table:
     """The host arrays of one call: pointers, sizes and types."""
 
     def __init__(self, tensors: Sequence[torch.Tensor]):
-        self.pointers = array("Q", [t.data_ptr() for t in tensors])
-        self.sizes = array("q", [t.numel() for t in tensors])
+        self.pointers = array("Q", map(_pointer, tensors))
+        self.sizes = array("q", map(_numel, tensors))
         self.types = array("i", [_DTYPE_CODES[t.dtype] for t in tensors])
         self.count = len(tensors)
 
@@ -90,7 +93,7 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], *, norm_type
     device = tensors[0].device
     with _lib.on_device(device):
         # A view whose elements do not fill one stretch of memory is copied.
-        tensors = [t if _dense(t) else t.contiguous() for t in tensors]
+        tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
         table = _Table(tensors)
         norm = torch.empty((), device=device, dtype=torch.float32)
         workspace, nbytes = _workspace(table.count, device)
@@ -108,13 +111,16 @@ def _targets(tensors: list[torch.Tensor], out: Optional[Sequence[torch.Tensor]],
         out = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(out) != len(tensors):
             raise ValueError(f"{what}: {len(out)} outputs for {len(tensors)} gradients")
-        for t, o in zip(tensors, out):
-            if o.shape != t.shape or o.dtype != t.dtype or o.get_device() != t.get_device():
-                raise ValueError(f"{what}: an output is {tuple(o.shape)} {o.dtype} on {o.device}, "
-                                 f"its gradient {tuple(t.shape)} {t.dtype} on {t.device}")
-    for o in out:
-        if not o.is_contiguous() and not _dense(o) and any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
-            raise ValueError(f"{what}: cannot write to an expanded tensor of shape {tuple(o.shape)}")
+        if ([o.shape for o in out] != [t.shape for t in tensors] or [o.dtype for o in out] != [t.dtype for t in tensors]
+                or set(map(_device, out)) != set(map(_device, tensors))):
+            for t, o in zip(tensors, out):
+                if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
+                    raise ValueError(f"{what}: an output is {tuple(o.shape)} {o.dtype} on {o.device}, "
+                                     f"its gradient {tuple(t.shape)} {t.dtype} on {t.device}")
+    if not all(map(_contiguous, out)):
+        for o in out:
+            if not _dense(o) and any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+                raise ValueError(f"{what}: cannot write to an expanded tensor of shape {tuple(o.shape)}")
     return out
 
 
@@ -150,12 +156,12 @@ def clip_grad_norm(
         # Views that do not fill one stretch of memory, or whose output lies in
         # another order, pass through a contiguous copy.
         src, dst, direct = tensors, out, None
-        if not (all(t.is_contiguous() for t in tensors) and all(o.is_contiguous() for o in out)):
+        if not (all(map(_contiguous, tensors)) and all(map(_contiguous, out))):
             direct = [_dense(t) and _dense(o) and _same_order(t, o) for t, o in zip(tensors, out)]
             src = [t if d else t.contiguous() for t, d in zip(tensors, direct)]
             dst = [o if d else torch.empty_like(t) for t, o, d in zip(src, out, direct)]
         table = _Table(src)
-        targets = array("Q", [t.data_ptr() for t in dst])
+        targets = array("Q", map(_pointer, dst))
         pointers, targets_at = table.pointers.buffer_info()[0], targets.buffer_info()[0]
         stream = _lib.stream_ptr(device)
         if group is None and not error_if_nonfinite:
