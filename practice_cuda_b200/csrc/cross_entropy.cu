@@ -52,21 +52,15 @@ bool store_map(CUtensorMap* map, void* base, int dt, int64_t inner, int64_t oute
 
 constexpr int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <int MODE, bool PAIR>
-int launch_product_as(const loss::Params& p, cudaStream_t s) {
-  auto kernel = loss::vocab_product_kernel<MODE, PAIR>;
-  if constexpr (MODE != loss::kProducts) {
-    // These kernels re-split their registers with setmaxnreg, which is only
-    // valid when the launch holds exactly kLaunchRegs per thread (otherwise
-    // setmaxnreg.inc could never be satisfied).
-    static const int num_regs = [&] {
-      cudaFuncAttributes fa{};
-      return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : -1;
-    }();
-    if (num_regs != loss::kLaunchRegs)
-      return fail(PCB_ERR_UNSUPPORTED, "cross entropy kernel register count differs from its setmaxnreg split");
-  }
-  constexpr int smem = loss::Smem<PAIR>::ALLOC;
+// Launch of one of the tcgen05 kernels over `workers` CTAs or pairs.  They
+// re-split their registers with setmaxnreg, which is only valid when the launch
+// holds exactly kLaunchRegs per thread (otherwise setmaxnreg.inc could never be
+// satisfied).
+template <bool PAIR>
+int launch_tiles(void (*kernel)(loss::Params), int num_regs, int smem, const loss::Params& p, cudaStream_t s,
+                 const char* what) {
+  if (num_regs != loss::kLaunchRegs)
+    return fail(PCB_ERR_UNSUPPORTED, "cross entropy kernel register count differs from its setmaxnreg split");
   ensure_smem_attr(kernel, smem);
   const int sms = device_info().sm_count;
   cudaLaunchConfig_t cfg = {};
@@ -75,7 +69,7 @@ int launch_product_as(const loss::Params& p, cudaStream_t s) {
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
-  // griddepcontrol.wait precedes every global access of the kernel.
+  // griddepcontrol.wait precedes every global access of the kernels.
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -85,18 +79,32 @@ int launch_product_as(const loss::Params& p, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = PAIR ? 2 : 1;
   cudaLaunchKernelEx(&cfg, kernel, p);
-  return check_launch("vocab_product_kernel");
+  return check_launch(what);
+}
+
+int regs_of(const void* kernel) {
+  cudaFuncAttributes fa{};
+  return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? fa.numRegs : -1;
+}
+
+template <int MODE, bool PAIR>
+int launch_logits_as(const loss::Params& p, cudaStream_t s) {
+  static const int regs = regs_of((const void*)loss::logits_kernel<MODE, PAIR>);
+  return launch_tiles<PAIR>(loss::logits_kernel<MODE, PAIR>, regs, loss::Smem<PAIR>::ALLOC, p, s, "logits_kernel");
+}
+
+template <int MODE>
+int launch_logits(const loss::Params& p, bool pair, cudaStream_t s) {
+  return pair ? launch_logits_as<MODE, true>(p, s) : launch_logits_as<MODE, false>(p, s);
+}
+
+int launch_grad_products(const loss::Params& p, cudaStream_t s) {
+  static const int regs = regs_of((const void*)loss::grad_products_kernel);
+  return launch_tiles<true>(loss::grad_products_kernel, regs, loss::ProductSmem::ALLOC, p, s, "grad_products_kernel");
 }
 
 // Up to 128 tokens a CTA has a tile to itself.
 bool on_pairs(int64_t tokens) { return tokens > loss::BM; }
-
-template <int MODE>
-int launch_product(const loss::Params& p, bool pair, cudaStream_t s) {
-  if constexpr (MODE != loss::kProducts)
-    if (!pair) return launch_product_as<MODE, false>(p, s);
-  return launch_product_as<MODE, true>(p, s);
-}
 
 // Columns of a logit tile.  On single CTAs: the vocabulary in as few rounds
 // over the SMs as 256-column tiles need, and evenly so (a multiple of 16, the
@@ -196,18 +204,18 @@ struct BwdPlan {
     pieces = up(vocab, cols);
     pitch = std::min(cols, up(vocab, 64) * 64);
     splits = 1;
-    const int64_t dx_tiles = up(tokens, loss::TILE) * up(dim, loss::TILE);
+    const int64_t dx_tiles = up(tokens, loss::TILE) * up(dim, loss::WIDE);
     if (want_dx && pieces == 1) {
       // dX's tiles are few and long where tokens are few: cut them along the
       // vocabulary so that none is longer than a quarter of an SM pair's share.
       const int64_t stages = up(vocab, loss::BK);
-      const int64_t all = dx_tiles * stages + up(vocab, loss::TILE) * up(dim, loss::TILE) * up(tokens, loss::BK);
+      const int64_t all = dx_tiles * stages + up(vocab, loss::TILE) * up(dim, loss::WIDE) * up(tokens, loss::BK);
       const int64_t longest = std::max<int64_t>(16, all / (4 * std::max(1, device_info().sm_count / 2)));
       splits = (int)std::min<int64_t>(std::max<int64_t>(1, stages / longest), 64);
     }
     Cut c;
     g = c.take(tokens * pitch * 2);
-    acc = c.take(want_dx && (pieces > 1 || splits > 1) ? dx_tiles * splits * loss::TILE * loss::TILE * 4 : 0);
+    acc = c.take(want_dx && (pieces > 1 || splits > 1) ? dx_tiles * splits * loss::TILE * loss::WIDE * 4 : 0);
     weight = c.take(tokens * 4);
     alpha = c.take(4);
     bytes = c.at;
@@ -281,7 +289,7 @@ int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw,
   p.partial = reinterpret_cast<float2*>(ws + plan.partial);
   p.target_logit = reinterpret_cast<float*>(ws + plan.target_logit);
   p.ticket = reinterpret_cast<unsigned*>(ws + plan.ticket);
-  if (int st = launch_product<loss::kStats>(p, pair, s)) return st;
+  if (int st = launch_logits<loss::kStats>(p, pair, s)) return st;
   loss::RowArgs r{p.partial, p.target_logit, p.target, ignore_index, vocab, (int)tokens, 2 * q.n_blocks, reduction,
                   stats, loss_out, count, reinterpret_cast<double*>(ws + plan.sums), p.ticket};
   return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), loss::kRowWarps * 32, s, r);
@@ -344,14 +352,13 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     q.scm = plan.pitch;
     p.num_tiles = q.tiles;
     if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-    if (int st = launch_product<loss::kGradient>(p, pair, s)) return st;
+    if (int st = launch_logits<loss::kGradient>(p, pair, s)) return st;
 
     p = base;
-    p.tile_n = loss::TILE;
     int n = 0;
     if (dx) {
       loss::Problem& d = p.prob[n++];
-      shape(d, tokens, dim, cols, plan.splits);
+      shape(d, tokens, dim, cols, plan.splits, true, loss::WIDE);
       ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, d.a_rows);
       ok &= load_b(d, w, dtype, dim, cols, sw);
       d.acc = acc;
@@ -366,7 +373,7 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
       loss::Problem& d = p.prob[n++];
       ok &= slab_map(&d.a, g, dtype, plan.pitch / 64, tokens, plan.pitch);  // rows of dW beyond cols are not stored
       ok &= load_b(d, x, dtype, dim, tokens, sx);
-      shape(d, cols, dim, tokens, 1);
+      shape(d, cols, dim, tokens, 1, true, loss::WIDE);
       d.a_mn = 1;
       char* out = static_cast<char*>(dw) + col0 * sdw * 2;
       d.c = out;
@@ -382,12 +389,12 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
       if (left > 0 && p.num_tiles >= pairs)
         p.extra = std::min(p.prob[0].split_stages / p.prob[1].k_stages, p.prob[1].tiles / (pairs - left));
     }
-    if (int st = launch_product<loss::kProducts>(p, true, s)) return st;
+    if (int st = launch_grad_products(p, s)) return st;
     if (dx && plan.splits > 1) {
       const loss::Problem& d = p.prob[0];
       const loss::JoinArgs j{acc, d.m, d.n, d.m_blocks, d.n_blocks, d.splits, p.fmt, static_cast<uint16_t*>(dx), sdx};
       if (int st = launch_after(loss::loss_join_kernel, "loss_join_kernel",
-                                (int64_t)d.m_blocks * d.n_blocks * 2 * loss::kAccVec, 256, s, j, p))
+                                (int64_t)d.m_blocks * d.n_blocks * 4 * loss::kAccVec, 256, s, j, p))
         return st;
     }
   }

@@ -4,16 +4,17 @@
 //   m_i = max_j l_ij, s_i = sum_j exp(l_ij - m_i), nll_i = (m_i - l_i,target) + log s_i
 //   G_ij = (exp(l_ij - m_i) / s_i - [j = target_i]) w_i,  dX = a G W,  dW = a G^T X
 //
-// One tcgen05 product kernel in three forms:
-//   kStats     a tile of logits leaves the tensor memory as the maximum and the
-//              sum of exponentials of each row's 128 columns, and the target's
-//              logit; the logits are never written.
-//   kGradient  the logits of one piece of the vocabulary again, leaving as G in
-//              the operands' 16-bit type (the one rounding that a tensor-core
-//              product of G asks for; w_i and a are split so that it is of the
-//              order of 1 and the loss's scale stays in fp32).
-//   kProducts  dX += G W and dW = G^T X of that piece in one launch: the tiles
-//              of both share the grid, so neither leaves SMs idle at its end.
+// Two tcgen05 kernels, the first of them in two forms:
+//   logits_kernel<kStats>     a tile of logits leaves the tensor memory as the
+//              maximum and the sum of exponentials of each row's 128 columns, and
+//              the target's logit; the logits are never written.
+//   logits_kernel<kGradient>  the logits of one piece of the vocabulary again,
+//              leaving as G in the operands' 16-bit type (the one rounding that a
+//              tensor-core product of G asks for; w_i and a are split so that it
+//              is of the order of 1 and the loss's scale stays in fp32).
+//   grad_products_kernel      dX += G W and dW = G^T X of that piece in one launch:
+//              the tiles of both share the grid, so neither leaves SMs idle at its
+//              end.
 // Logits, softmax statistics and every sum are fp32.  m and log2 s are kept apart:
 // their sum would lose the small part of a sure token's probability beside a large
 // logit.  The tensor cores truncate as they accumulate, which moves a logit of 4096
@@ -33,7 +34,7 @@
 namespace pcb {
 namespace loss {
 
-enum Mode : int { kStats = 0, kGradient = 1, kProducts = 2 };
+enum Mode : int { kStats = 0, kGradient = 1 };
 enum Acc : int { kAccNone = 0, kAccWrite = 1, kAccAdd = 2, kAccLast = 3, kAccSlab = 4 };
 
 constexpr int BM = 128;            // rows of the tile per CTA
@@ -42,7 +43,10 @@ constexpr int BK = 64;             // K elements of a stage: one 128-byte swizzl
 constexpr int UMMA_K = 16;
 constexpr int kChunkStages = 8;    // stages between two promotions of a logit's accumulator, about
 constexpr int A_BYTES = BM * BK * 2;
-constexpr int SLAB = 64 * BK * 2;           // 64 MN elements x 64 K rows of an MN-major operand
+constexpr int SLAB = 64 * BK * 2;  // 64 MN elements x 64 K rows of an MN-major operand
+constexpr uint32_t K_STEP = UMMA_K * 2 >> 4;     // an instruction's K: 32 bytes along a K-major row,
+constexpr uint32_t MN_STEP = UMMA_K * 128 >> 4;  // or 16 K rows of an MN-major slab
+constexpr int WIDE = 2 * TILE;  // tile columns of the products of G
 constexpr int NACC = 2;
 constexpr int kThreads = 384;
 constexpr int kEpiWarp0 = 4;
@@ -74,6 +78,18 @@ struct Smem {
   static_assert(ALLOC <= 232448, "shared memory per CTA");
 };
 
+// The products of G: 48 KB stages of A and of two 128-column parts of B per CTA.
+struct ProductSmem {
+  static constexpr int STAGES = 4;
+  static constexpr int B_BYTES = 2 * 2 * SLAB;
+  static constexpr int OFF_B = STAGES * A_BYTES;
+  static constexpr int OFF_CSTG = OFF_B + STAGES * B_BYTES;  // 4 KB per epilogue warp
+  static constexpr int OFF_BAR = OFF_CSTG + 8 * 4096;
+  static constexpr int OFF_MISC = OFF_BAR + (2 * STAGES + 4) * 8;
+  static constexpr int ALLOC = OFF_MISC + 16 + 1024;
+  static_assert(ALLOC <= 232448, "shared memory per CTA");
+};
+
 enum Site : int { SITE_LOSS_PRODUCER = 16, SITE_LOSS_MMA = 17, SITE_LOSS_EPILOGUE = 18, SITE_LOSS_TARGET = 19 };
 
 // One matrix product C [m, n] = A B of a launch.
@@ -85,8 +101,9 @@ struct Problem {
   int k_stages, split_stages;
   int chunk_stages;  // of the logits: stages between two promotions
   int a_rows;        // rows of A that a load brings (K-major A)
-  int a_mn;   // A is M-major (kProducts; B is N-major there)
-  int b_slabs;  // B's map takes both of a CTA's 64-column slabs in one load
+  // products of G, where B is N-major:
+  int a_mn;     // A is M-major
+  int b_slabs;  // B's map takes both 64-column slabs of a 128-column part in one load
   int c_tma;  // C leaves through TMA stores
   void* c;
   long long scm;
@@ -248,12 +265,10 @@ __device__ __forceinline__ void store_box(const Problem& q, const uint32_t (&w)[
 }
 
 template <int MODE, bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid_constant__ Params p) {
-  static_assert(PAIR || MODE != kProducts, "the products of G run on CTA pairs");
+__global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_constant__ Params p) {
   using S = Smem<PAIR>;
   constexpr int STAGES = S::STAGES;
   constexpr int TILE_M = PAIR ? TILE : BM;
-  constexpr bool CHUNKED = MODE != kProducts;
   // Bytes of a stage on the (leader's) full barrier.
   // The rows of A below a_rows are loaded; those of the tile beyond it hold
   // whatever was there and reach no row that is stored.
@@ -306,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
   if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
 
   if (warp < kEpiWarp0) {
-    if constexpr (CHUNKED) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
     if (warp == 0) {
       // ------------------------------ TMA producer ------------------------------
       if (lane == 0) {
@@ -318,8 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
           const Problem& q = p.prob[t.prob];
           const int a_row = t.mb * TILE_M + (int)rank * BM;
           const int b_col = PAIR ? t.nb * TILE + (int)rank * (TILE / 2) : t.nb * p.tile_n;
-          const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
-          for (int ks = t.split * q.split_stages; ks < ks1; ++ks) {
+          for (int ks = 0; ks < q.k_stages; ++ks) {
             if (!mbar_spin_bounded(bar_empty + 8 * stage, phase ^ 1, abort_flag, SITE_LOSS_PRODUCER)) {
               ok = false;
               break;
@@ -327,23 +341,11 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
             const uint32_t fb = bar_full + 8 * stage;
             const uint32_t a_dst = s_base + stage * A_BYTES;
             const uint32_t b_dst = s_base + S::OFF_B + stage * S::B_BYTES;
-            const uint32_t a_bytes = (uint32_t)(PAIR ? 2 : 1) * (MODE == kProducts && q.a_mn ? A_BYTES : q.a_rows * BK * 2);
-            if (leader) mbar_arrive_expect_tx(fb, a_bytes + b_bytes);
+            if (leader) mbar_arrive_expect_tx(fb, (uint32_t)(PAIR ? 2 : 1) * q.a_rows * BK * 2 + b_bytes);
             if constexpr (PAIR) {
               const uint32_t fbl = gemm::mapa_shared(fb, 0);
-              if (MODE == kProducts && q.a_mn) {
-                gemm::tma_load_3d_pair(a_dst, &q.a, fbl, 0, ks * BK, a_row / 64);
-              } else {
-                gemm::tma_load_3d_pair(a_dst, &q.a, fbl, ks * BK, a_row, 0);
-              }
-              if (MODE == kProducts && q.b_slabs) {
-                gemm::tma_load_3d_pair(b_dst, &q.b, fbl, 0, ks * BK, b_col / 64);
-              } else if (MODE == kProducts) {
-                gemm::tma_load_3d_pair(b_dst, &q.b, fbl, b_col, ks * BK, 0);
-                gemm::tma_load_3d_pair(b_dst + SLAB, &q.b, fbl, b_col + 64, ks * BK, 0);
-              } else {
-                gemm::tma_load_3d_pair(b_dst, &q.b, fbl, ks * BK, b_col, 0);
-              }
+              gemm::tma_load_3d_pair(a_dst, &q.a, fbl, ks * BK, a_row, 0);
+              gemm::tma_load_3d_pair(b_dst, &q.b, fbl, ks * BK, b_col, 0);
             } else {
               gemm::tma_load_3d(a_dst, &q.a, fb, ks * BK, a_row, 0);
               gemm::tma_load_3d(b_dst, &q.b, fb, ks * BK, b_col, 0);
@@ -368,40 +370,30 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
         auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
           return mbar_spin_bounded_warp(bar, parity, abort_flag, SITE_LOSS_MMA);
         };
-        const uint64_t k_desc = gemm::make_sw128_desc(s_base, 16u), mn_desc = gemm::make_sw128_desc(s_base, SLAB);
-        constexpr uint32_t K_STEP = UMMA_K * 2 >> 4;     // 32 bytes along a K-major row
-        constexpr uint32_t MN_STEP = UMMA_K * 128 >> 4;  // 16 K rows of an MN-major slab
-        constexpr uint32_t B_STEP = MODE == kProducts ? MN_STEP : K_STEP;
-        const uint64_t b_desc = MODE == kProducts ? mn_desc : k_desc;
+        const uint64_t desc = gemm::make_sw128_desc(s_base, 16u);
+        const uint32_t idesc = gemm::make_idesc(p.tile_n, p.fmt, p.fmt, 0, 0, TILE_M);
         for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
-          const TileAt t = locate(p, tile);
-          const Problem& q = p.prob[t.prob];
-          const bool a_mn = MODE == kProducts && q.a_mn;
-          const uint64_t a_desc = a_mn ? mn_desc : k_desc;
-          const uint32_t a_step = a_mn ? MN_STEP : K_STEP;
-          const uint32_t idesc =
-              gemm::make_idesc(p.tile_n, p.fmt, p.fmt, a_mn ? 1 : 0, MODE == kProducts ? 1 : 0, TILE_M);
-          const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
-          int ks = t.split * q.split_stages;
-          while (ks < ks1 && ok) {
+          const Problem& q = p.prob[0];
+          int ks = 0;
+          while (ks < q.k_stages && ok) {
             const uint32_t abuf = acc_cnt % NACC, d_tmem = tmem_base + abuf * TILE;
             if (!wait(bar_tempty + 8 * abuf, ((acc_cnt / NACC) & 1) ^ 1)) {
               ok = false;
               break;
             }
-            const int stop = CHUNKED ? min(ks1, ks + q.chunk_stages) : ks1;
+            const int stop = min(q.k_stages, ks + q.chunk_stages);
             for (bool fresh = true; ks < stop; ++ks, fresh = false) {
               if (!wait(bar_full + 8 * stage, phase)) {
                 ok = false;
                 break;
               }
               gemm::tc_fence_after();
-              const uint32_t a_lo = (uint32_t)a_desc + (uint32_t)(stage * A_BYTES >> 4);
-              const uint32_t b_lo = (uint32_t)b_desc + (uint32_t)((S::OFF_B + stage * S::B_BYTES) >> 4);
+              const uint32_t a_lo = (uint32_t)desc + (uint32_t)(stage * A_BYTES >> 4);
+              const uint32_t b_lo = (uint32_t)desc + (uint32_t)((S::OFF_B + stage * S::B_BYTES) >> 4);
 #pragma unroll
               for (int kk = 0; kk < BK / UMMA_K; ++kk)
-                umma_f16_elect<PAIR>(d_tmem, a_lo + kk * a_step, (uint32_t)(a_desc >> 32), b_lo + kk * B_STEP,
-                                     (uint32_t)(b_desc >> 32), idesc, (kk > 0 || !fresh) ? 1u : 0u);
+                umma_f16_elect<PAIR>(d_tmem, a_lo + kk * K_STEP, (uint32_t)(desc >> 32), b_lo + kk * K_STEP,
+                                     (uint32_t)(desc >> 32), idesc, (kk > 0 || !fresh) ? 1u : 0u);
               gemm::umma_commit_elect<PAIR>(bar_empty + 8 * stage);  // stage (of both CTAs) free once these retire
               if (++stage == STAGES) {
                 stage = 0;
@@ -417,14 +409,13 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
     }
   } else {
     // -------------------------------- epilogue --------------------------------
-    if constexpr (CHUNKED) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHighRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHighRegs));
     const int ew = warp - kEpiWarp0;  // 0..7
     const int quarter = warp & 3;     // tensor-memory lanes 32 * quarter .. + 31
     const int half = ew >> 2;         // column half
     const int half_cols = PAIR ? EPI_COLS : p.tile_n / 2;
     const uint32_t stg = s_base + S::OFF_CSTG + (uint32_t)ew * 4096u;
     const uint32_t bar_tempty_l = PAIR ? gemm::mapa_shared(bar_tempty, 0) : bar_tempty;
-    const float alpha = MODE == kProducts ? alpha_of(p) : 1.f;
     uint32_t acc_cnt = 0;
     bool ok = true;
     for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
@@ -453,107 +444,31 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
         return tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * TILE + half * half_cols;
       };
 
-      if constexpr (CHUNKED) {
-        // Row values are read before the wait, so their latency is hidden.
-        int target = -1;  // within the piece
-        float top = 0.f, shift = 0.f, weight = 0.f;
-        if (in) {
-          const long long tv = p.target[row];
-          const bool valid = tv != p.ignore_index;
-          if (MODE == kGradient && valid) {
-            top = p.stats[row];
-            shift = (float)kGradShift - p.stats[q.m + row];
-            weight = p.row_weight ? p.row_weight[row] : 1.f;
-            if (tv < 0 || tv >= p.vocab) weight = NAN;  // no such column
-          }
-          if (valid && tv >= p.col0 + col0 && tv < p.col0 + limit) target = (int)(tv - p.col0);
+      // Row values are read before the wait, so their latency is hidden.
+      int target = -1;  // within the piece
+      float top = 0.f, shift = 0.f, weight = 0.f;
+      if (in) {
+        const long long tv = p.target[row];
+        const bool valid = tv != p.ignore_index;
+        if (MODE == kGradient && valid) {
+          top = p.stats[row];
+          shift = (float)kGradShift - p.stats[q.m + row];
+          weight = p.row_weight ? p.row_weight[row] : 1.f;
+          if (tv < 0 || tv >= p.vocab) weight = NAN;  // no such column
         }
-        // The logits: the accumulators of every 512 products, summed.
-        float acc[EPI_COLS];
-        const int chunks = (q.k_stages + q.chunk_stages - 1) / q.chunk_stages;
-        for (int ch = 0; ch < chunks; ++ch, ++acc_cnt) {
-          const uint32_t abuf = acc_cnt % NACC;
-          if (!wait_full(abuf)) {
-            ok = false;
-            break;
-          }
-          const uint32_t taddr = address(abuf);
-          uint32_t v[2][32];
-          gemm::tmem_ld32_nowait(taddr, v[0]);
-          gemm::tmem_wait_ld();
-          gemm::tmem_regs_ready(v[0]);
-#pragma unroll
-          for (int c = 0; c < EPI_COLS / 32; ++c) {
-            if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
-            else release(abuf);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float x = __uint_as_float(v[c & 1][j]);
-              acc[c * 32 + j] = ch == 0 ? x : acc[c * 32 + j] + x;
-            }
-            if (c + 1 < EPI_COLS / 32) {
-              gemm::tmem_wait_ld();
-              gemm::tmem_regs_ready(v[(c + 1) & 1]);
-            }
-          }
-        }
-        if (!ok) break;
-
-        if constexpr (MODE == kStats) {
-          float tl = 0.f;
-          if (target >= 0) {
-#pragma unroll
-            for (int j = 0; j < EPI_COLS; ++j)
-              if (target == col0 + j) tl = acc[j];
-          }
-          if (col0 + EPI_COLS > limit) {  // columns beyond this half, or the vocabulary
-#pragma unroll
-            for (int j = 0; j < EPI_COLS; ++j)
-              if (col0 + j >= limit) acc[j] = -INFINITY;
-          }
-          float mc[4] = {acc[0], acc[1], acc[2], acc[3]};
-#pragma unroll
-          for (int j = 4; j < EPI_COLS; ++j) mc[j & 3] = fmaxf(mc[j & 3], acc[j]);
-          const float m = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
-          const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf: exp(-inf - 0) = 0
-          float sc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < EPI_COLS; ++j) sc[j & 3] += exp2_approx((acc[j] - base) * kLog2e);
-          if (in) {
-            p.partial[(long long)(t.nb * 2 + half) * q.m + row] = make_float2(m, (sc[0] + sc[1]) + (sc[2] + sc[3]));
-            if (target >= 0) p.target_logit[row] = tl;
-          }
-        } else {
-#pragma unroll
-          for (int b = 0; b < EPI_COLS / 64; ++b) {  // boxes of 64 columns
-            uint32_t w[32];
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              acc[b * 64 + j] = exp2_approx(fmaf(acc[b * 64 + j] - top, kLog2e, shift));
-            if (target >= col0 + b * 64 && target < col0 + b * 64 + 64) {
-#pragma unroll
-              for (int j = 0; j < 64; ++j)
-                if (target == col0 + b * 64 + j) acc[b * 64 + j] -= kGradScale;
-            }
-            // Tokens left out get zeros, whatever their logits are.
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              w[j] = weight == 0.f
-                         ? 0u
-                         : pack2(acc[b * 64 + 2 * j] * weight, acc[b * 64 + 2 * j + 1] * weight, p.fmt);
-            if (b * 64 < half_cols) store_box(q, w, stg, lane, row0, col0 + b * 64, limit);
-          }
-        }
-      } else {
+        if (valid && tv >= p.col0 + col0 && tv < p.col0 + limit) target = (int)(tv - p.col0);
+      }
+      // The logits: the accumulators of every 512 products, summed.
+      float acc[EPI_COLS];
+      const int chunks = (q.k_stages + q.chunk_stages - 1) / q.chunk_stages;
+      for (int ch = 0; ch < chunks; ++ch, ++acc_cnt) {
         const uint32_t abuf = acc_cnt % NACC;
-        if (!wait_full(abuf)) break;
-        ++acc_cnt;
+        if (!wait_full(abuf)) {
+          ok = false;
+          break;
+        }
         const uint32_t taddr = address(abuf);
-        float4* acc = nullptr;
-        if (q.acc_mode != kAccNone) acc = q.acc + ((long long)t.index * 2 + rank) * kAccVec * 256 + ew * 32 + lane;
-        const bool add = q.acc_mode == kAccAdd || q.acc_mode == kAccLast;
-        const bool stored = q.acc_mode == kAccNone || q.acc_mode == kAccLast;
-        uint32_t v[2][32], w[32];  // w: 64 packed columns
+        uint32_t v[2][32];
         gemm::tmem_ld32_nowait(taddr, v[0]);
         gemm::tmem_wait_ld();
         gemm::tmem_regs_ready(v[0]);
@@ -561,33 +476,62 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
         for (int c = 0; c < EPI_COLS / 32; ++c) {
           if (c + 1 < EPI_COLS / 32) gemm::tmem_ld32_nowait(taddr + (c + 1) * 32, v[(c + 1) & 1]);
           else release(abuf);
-          uint32_t(&u)[32] = v[c & 1];
-          if (add) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 o = acc[(long long)(c * 8 + j) * 256];
-              u[4 * j] = __float_as_uint(__uint_as_float(u[4 * j]) + o.x);
-              u[4 * j + 1] = __float_as_uint(__uint_as_float(u[4 * j + 1]) + o.y);
-              u[4 * j + 2] = __float_as_uint(__uint_as_float(u[4 * j + 2]) + o.z);
-              u[4 * j + 3] = __float_as_uint(__uint_as_float(u[4 * j + 3]) + o.w);
-            }
-          }
-          if (stored) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              w[(c & 1) * 16 + j] = pack2(__uint_as_float(u[2 * j]) * alpha, __uint_as_float(u[2 * j + 1]) * alpha, p.fmt);
-            if (c & 1) store_box(q, w, stg, lane, row0, col0 + (c - 1) * 32, limit);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              acc[(long long)(c * 8 + j) * 256] =
-                  make_float4(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), __uint_as_float(u[4 * j + 2]),
-                              __uint_as_float(u[4 * j + 3]));
+          for (int j = 0; j < 32; ++j) {
+            const float x = __uint_as_float(v[c & 1][j]);
+            acc[c * 32 + j] = ch == 0 ? x : acc[c * 32 + j] + x;
           }
           if (c + 1 < EPI_COLS / 32) {
             gemm::tmem_wait_ld();
             gemm::tmem_regs_ready(v[(c + 1) & 1]);
           }
+        }
+      }
+      if (!ok) break;
+
+      if constexpr (MODE == kStats) {
+        float tl = 0.f;
+        if (target >= 0) {
+#pragma unroll
+          for (int j = 0; j < EPI_COLS; ++j)
+            if (target == col0 + j) tl = acc[j];
+        }
+        if (col0 + EPI_COLS > limit) {  // columns beyond this half, or the vocabulary
+#pragma unroll
+          for (int j = 0; j < EPI_COLS; ++j)
+            if (col0 + j >= limit) acc[j] = -INFINITY;
+        }
+        float mc[4] = {acc[0], acc[1], acc[2], acc[3]};
+#pragma unroll
+        for (int j = 4; j < EPI_COLS; ++j) mc[j & 3] = fmaxf(mc[j & 3], acc[j]);
+        const float m = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3]));
+        const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf: exp(-inf - 0) = 0
+        float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < EPI_COLS; ++j) sc[j & 3] += exp2_approx((acc[j] - base) * kLog2e);
+        if (in) {
+          p.partial[(long long)(t.nb * 2 + half) * q.m + row] = make_float2(m, (sc[0] + sc[1]) + (sc[2] + sc[3]));
+          if (target >= 0) p.target_logit[row] = tl;
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < EPI_COLS / 64; ++b) {  // boxes of 64 columns
+          uint32_t w[32];
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            acc[b * 64 + j] = exp2_approx(fmaf(acc[b * 64 + j] - top, kLog2e, shift));
+          if (target >= col0 + b * 64 && target < col0 + b * 64 + 64) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (target == col0 + b * 64 + j) acc[b * 64 + j] -= kGradScale;
+          }
+          // Tokens left out get zeros, whatever their logits are.
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            w[j] = weight == 0.f
+                       ? 0u
+                       : pack2(acc[b * 64 + 2 * j] * weight, acc[b * 64 + 2 * j + 1] * weight, p.fmt);
+          if (b * 64 < half_cols) store_box(q, w, stg, lane, row0, col0 + b * 64, limit);
         }
       }
     }
@@ -606,6 +550,264 @@ __global__ void __launch_bounds__(kThreads, 1) vocab_product_kernel(const __grid
     gemm::tc_fence_after();
     if (warp == 1) gemm::tmem_dealloc(tmem_base, NACC * TILE);
   }
+}
+
+// dX = G W and dW = G^T X, or what is wanted of them, in one launch.  A CTA
+// pair's tile is 256 x 512: two instructions of N = 256 share the stage of A, so
+// that an SM moves 24 KB of operands for what takes 32 KB in a 256 x 256 tile.
+// That is what bounds these products (the L2's output to the SMs, more so for
+// operands that are not K-major, where 256 x 256 tiles ran at 69 % of the tensor
+// pipe).  The accumulators fill the tensor memory, so the epilogue takes a half
+// into registers at once (128 fp32 a thread) and gives it back before it stores
+// it, and the next tile's first stages are issued for the first half alone while
+// the second is still being read.  A tile at the right edge with no more than 256
+// columns has one half.
+__global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid_constant__ Params p) {
+  using S = ProductSmem;
+  constexpr int STAGES = S::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t s_base = smem_u32(smem);
+  const uint32_t bar_full = s_base + S::OFF_BAR;      // [STAGES]
+  const uint32_t bar_empty = bar_full + 8 * STAGES;   // [STAGES]
+  const uint32_t bar_tfull = bar_empty + 8 * STAGES;  // [2] halves
+  const uint32_t bar_tempty = bar_tfull + 16;         // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::OFF_MISC + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = gemm::cluster_ctarank();
+  const bool leader = rank == 0;
+  const int worker = (int)(blockIdx.x >> 1), workers = (int)(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(bar_tfull + 8 * h, 1);
+      mbar_init(bar_tempty + 8 * h, 16);  // one arrive per epilogue warp of both CTAs
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    gemm::prefetch_tmap(&p.prob[0].a);
+    gemm::prefetch_tmap(&p.prob[0].b);
+  }
+  if (warp == 1) gemm::tmem_alloc_pair(smem_u32(tmem_slot), WIDE);
+  gemm::tc_fence_before();
+  gemm::cluster_sync_all();  // both CTAs' barriers exist before any remote arrive / TMA
+  gemm::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // Nothing global is read or written before the previous kernel has completed.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  if (warp < kEpiWarp0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
+    if (warp == 0) {
+      // ------------------------------ TMA producer ------------------------------
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
+          const TileAt t = locate(p, tile);
+          const Problem& q = p.prob[t.prob];
+          const int a_row = t.mb * TILE + (int)rank * BM;
+          const int b_col = t.nb * WIDE + (int)rank * (TILE / 2);
+          const int halves = t.nb * WIDE + TILE < q.n ? 2 : 1;
+          const uint32_t bytes = 2u * ((q.a_mn ? A_BYTES : q.a_rows * BK * 2) + halves * 2 * SLAB);
+          const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
+          for (int ks = t.split * q.split_stages; ks < ks1; ++ks) {
+            if (!mbar_spin_bounded(bar_empty + 8 * stage, phase ^ 1, abort_flag, SITE_LOSS_PRODUCER)) {
+              ok = false;
+              break;
+            }
+            const uint32_t fb = bar_full + 8 * stage, fbl = gemm::mapa_shared(fb, 0);
+            const uint32_t a_dst = s_base + stage * A_BYTES;
+            const uint32_t b_dst = s_base + S::OFF_B + stage * S::B_BYTES;
+            if (leader) mbar_arrive_expect_tx(fb, bytes);
+            if (q.a_mn) gemm::tma_load_3d_pair(a_dst, &q.a, fbl, 0, ks * BK, a_row / 64);
+            else gemm::tma_load_3d_pair(a_dst, &q.a, fbl, ks * BK, a_row, 0);
+            for (int h = 0; h < halves; ++h) {
+              const uint32_t dst = b_dst + h * 2 * SLAB;
+              const int col = b_col + h * TILE;
+              if (q.b_slabs) {
+                gemm::tma_load_3d_pair(dst, &q.b, fbl, 0, ks * BK, col / 64);
+              } else {
+                gemm::tma_load_3d_pair(dst, &q.b, fbl, col, ks * BK, 0);
+                gemm::tma_load_3d_pair(dst + SLAB, &q.b, fbl, col + 64, ks * BK, 0);
+              }
+            }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        if (!ok) {
+          // Let the copies already issued land before the CTA can exit.
+          for (int s = 0; s < STAGES; ++s) mbar_wait_bounded(bar_full + 8 * s, 0, abort_flag, SITE_LOSS_PRODUCER);
+        }
+      }
+    } else if (warp == 1 && leader) {
+      // ------------------------------- MMA issuer -------------------------------
+      int stage = 0;
+      uint32_t phase = 0, used[2] = {0, 0};  // tiles that have filled each half
+      auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+        return mbar_spin_bounded_warp(bar, parity, abort_flag, SITE_LOSS_MMA);
+      };
+      const uint64_t k_desc = gemm::make_sw128_desc(s_base, 16u), mn_desc = gemm::make_sw128_desc(s_base, SLAB);
+      for (int i = 0, tile; (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
+        const TileAt t = locate(p, tile);
+        const Problem& q = p.prob[t.prob];
+        const uint64_t a_desc = q.a_mn ? mn_desc : k_desc;
+        const uint32_t a_step = q.a_mn ? MN_STEP : K_STEP;
+        const uint32_t idesc = gemm::make_idesc(TILE, p.fmt, p.fmt, q.a_mn, 1, 2 * BM);
+        const int stages = min(q.k_stages, (t.split + 1) * q.split_stages) - t.split * q.split_stages;
+        const bool wide = t.nb * WIDE + TILE < q.n;
+        auto issue = [&](int st, int h, bool fresh) {
+          const uint32_t a_lo = (uint32_t)a_desc + (uint32_t)(st * A_BYTES >> 4);
+          const uint32_t b_lo = (uint32_t)mn_desc + (uint32_t)((S::OFF_B + st * S::B_BYTES + h * 2 * SLAB) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk)
+            umma_f16_elect<true>(tmem_base + h * TILE, a_lo + kk * a_step, (uint32_t)(a_desc >> 32),
+                                 b_lo + kk * MN_STEP, (uint32_t)(mn_desc >> 32), idesc, (kk > 0 || !fresh) ? 1u : 0u);
+        };
+        auto advance = [&] {
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        };
+        if (!wait(bar_tempty, (used[0] & 1) ^ 1)) break;
+        bool ok = true;
+        int done = 0;
+        if (wide) {
+          // The first stages for the first half, then for the second.
+          const int head = min(stages, STAGES), stage0 = stage;
+          const uint32_t phase0 = phase;
+          for (int s = 0; s < head && ok; ++s) {
+            ok = wait(bar_full + 8 * stage, phase);
+            if (!ok) break;
+            gemm::tc_fence_after();
+            issue(stage, 0, s == 0);
+            advance();
+          }
+          if (!ok) break;
+          if (head == stages) gemm::umma_commit_elect<true>(bar_tfull);
+          if (!wait(bar_tempty + 8, (used[1] & 1) ^ 1)) break;
+          gemm::tc_fence_after();
+          stage = stage0;
+          phase = phase0;
+          for (int s = 0; s < head; ++s) {
+            issue(stage, 1, s == 0);
+            gemm::umma_commit_elect<true>(bar_empty + 8 * stage);  // stage (of both CTAs) free once these retire
+            advance();
+          }
+          done = head;
+        }
+        for (; done < stages; ++done) {
+          ok = wait(bar_full + 8 * stage, phase);
+          if (!ok) break;
+          gemm::tc_fence_after();
+          issue(stage, 0, done == 0);
+          if (done + 1 == stages) gemm::umma_commit_elect<true>(bar_tfull);
+          if (wide) issue(stage, 1, false);
+          gemm::umma_commit_elect<true>(bar_empty + 8 * stage);
+          advance();
+        }
+        if (!ok) break;
+        ++used[0];
+        if (wide) {
+          gemm::umma_commit_elect<true>(bar_tfull + 8);
+          ++used[1];
+        }
+      }
+    }
+  } else {
+    // -------------------------------- epilogue --------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kHighRegs));
+    const int ew = warp - kEpiWarp0;  // 0..7
+    const int quarter = warp & 3;     // tensor-memory lanes 32 * quarter .. + 31
+    const int part = ew >> 2;         // 128 of a half's 256 columns
+    const uint32_t stg = s_base + S::OFF_CSTG + (uint32_t)ew * 4096u;
+    const uint32_t bar_tempty_l = gemm::mapa_shared(bar_tempty, 0);
+    const float alpha = alpha_of(p);
+    uint32_t used[2] = {0, 0};
+    bool ok = true;
+    for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
+      const TileAt t = locate(p, tile);
+      const Problem& q = p.prob[t.prob];
+      const int row0 = t.mb * TILE + (int)rank * BM + quarter * 32;  // of the warp
+      const int halves = t.nb * WIDE + TILE < q.n ? 2 : 1;
+      const bool add = q.acc_mode == kAccAdd || q.acc_mode == kAccLast;
+      const bool stored = q.acc_mode == kAccNone || q.acc_mode == kAccLast;
+      for (int h = 0; h < halves; ++h) {
+        const int col0 = t.nb * WIDE + h * TILE + part * EPI_COLS;
+        if (!mbar_spin_bounded_warp(bar_tfull + 8 * h, used[h] & 1, abort_flag, SITE_LOSS_EPILOGUE)) {
+          ok = false;
+          break;
+        }
+        ++used[h];
+        gemm::tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + h * TILE + part * EPI_COLS;
+        uint32_t v[EPI_COLS / 32][32];
+#pragma unroll
+        for (int c = 0; c < EPI_COLS / 32; ++c) gemm::tmem_ld32_nowait(taddr + c * 32, v[c]);
+        gemm::tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < EPI_COLS / 32; ++c) gemm::tmem_regs_ready(v[c]);
+        gemm::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) gemm::mbar_arrive_cluster(bar_tempty_l + 8 * h);
+
+        float4* acc = nullptr;
+        if (q.acc_mode != kAccNone)
+          acc = q.acc + (((long long)t.index * 2 + rank) * 2 + h) * kAccVec * 256 + ew * 32 + lane;
+        if (add) {
+#pragma unroll
+          for (int c = 0; c < EPI_COLS / 32; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 o = acc[(long long)(c * 8 + j) * 256];
+              v[c][4 * j] = __float_as_uint(__uint_as_float(v[c][4 * j]) + o.x);
+              v[c][4 * j + 1] = __float_as_uint(__uint_as_float(v[c][4 * j + 1]) + o.y);
+              v[c][4 * j + 2] = __float_as_uint(__uint_as_float(v[c][4 * j + 2]) + o.z);
+              v[c][4 * j + 3] = __float_as_uint(__uint_as_float(v[c][4 * j + 3]) + o.w);
+            }
+        }
+        if (stored) {
+#pragma unroll
+          for (int b = 0; b < EPI_COLS / 64; ++b) {
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              w[j] = pack2(__uint_as_float(v[2 * b + j / 16][2 * j % 32]) * alpha,
+                           __uint_as_float(v[2 * b + j / 16][2 * j % 32 + 1]) * alpha, p.fmt);
+            store_box(q, w, stg, lane, row0, col0 + b * 64, q.n);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < EPI_COLS / 32; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              acc[(long long)(c * 8 + j) * 256] =
+                  make_float4(__uint_as_float(v[c][4 * j]), __uint_as_float(v[c][4 * j + 1]),
+                              __uint_as_float(v[c][4 * j + 2]), __uint_as_float(v[c][4 * j + 3]));
+        }
+      }
+    }
+    // The staging buffers stay valid until every issued store has completed.
+    if (lane == 0) gemm::bulk_wait_all();
+  }
+
+  __syncwarp();
+  gemm::tc_fence_before();
+  gemm::cluster_sync_all();  // no CTA leaves while its peer may still touch its smem / barriers
+  gemm::tc_fence_after();
+  if (warp == 1) gemm::tmem_dealloc_pair(tmem_base, WIDE);
 }
 
 // ---------------------------------------------------------------------------
@@ -791,16 +993,17 @@ struct JoinArgs {
 __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs p, const __grid_constant__ Params pp) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float alpha = alpha_of(pp);
-  // blockIdx.x: (tile of the first part, CTA of the pair, float4 of the thread)
-  const int i = blockIdx.x % kAccVec, rank = blockIdx.x / kAccVec % 2, index = blockIdx.x / kAccVec / 2;
+  // blockIdx.x: (tile of the first part, CTA of the pair, half, float4 of the thread)
+  const int i = blockIdx.x % kAccVec, h = blockIdx.x / kAccVec % 2, rank = blockIdx.x / kAccVec / 2 % 2;
+  const int index = blockIdx.x / kAccVec / 4;
   const int ew = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TileAt t = locate(pp, index);
   const int row = t.mb * TILE + rank * BM + (ew & 3) * 32 + lane;
-  const int col = t.nb * TILE + (ew >> 2) * EPI_COLS + i * 4;
+  const int col = t.nb * WIDE + h * TILE + (ew >> 2) * EPI_COLS + i * 4;
   if (row >= p.m || col >= p.n) return;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  const long long part = (long long)p.m_blocks * p.n_blocks * 2 * kAccVec * 256;
-  const float4* a = p.acc + (((long long)index * 2 + rank) * kAccVec + i) * 256 + threadIdx.x;
+  const long long part = (long long)p.m_blocks * p.n_blocks * 4 * kAccVec * 256;
+  const float4* a = p.acc + ((((long long)index * 2 + rank) * 2 + h) * kAccVec + i) * 256 + threadIdx.x;
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float4 o = a[s * part];
