@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -106,6 +107,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss):
         x2, w2, target, stats = ctx.saved_tensors
         ignore_index, reduction, piece = ctx.args
@@ -145,8 +147,8 @@ def linear_cross_entropy(
 
     ``reduction``, ``ignore_index`` and the mean over no token at all (NaN,
     with zero gradients) are those of ``torch.nn.functional.cross_entropy``.
-    Differentiable in ``x`` and ``weight``; a gradient that is not needed is
-    not computed.  ``vocab_piece`` bounds the columns of the logits' gradient
+    Differentiable (once) in ``x`` and ``weight``; a gradient that is not needed
+    is not computed.  ``vocab_piece`` bounds the columns of the logits' gradient
     that exist at a time in the backward pass (rounded down to a multiple of
     256, at least 256; default: as many as fit 128 MiB, at least 2048).
 

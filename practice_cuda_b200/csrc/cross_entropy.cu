@@ -138,7 +138,8 @@ void shape(loss::Problem& q, int64_t m, int64_t n, int64_t k, int splits, bool p
   q.m_blocks = (int)up(m, pair ? loss::TILE : loss::BM);
   q.n_blocks = (int)up(n, tile_n);
   q.k_stages = (int)up(k, loss::BK);
-  const int chunks = std::max(1, (q.k_stages + loss::kChunkStages / 2) / loss::kChunkStages);
+  const int target = pair ? loss::kChunkStages : loss::kChunkStagesSingle;
+  const int chunks = std::max(1, (q.k_stages + target / 2) / target);
   q.chunk_stages = (int)up(q.k_stages, chunks);  // even chunks: a last one of a stage or two would stall the others
   q.a_rows = (int)std::min<int64_t>(loss::BM, up(m, 8) * 8);
   q.split_stages = (int)up(q.k_stages, splits);

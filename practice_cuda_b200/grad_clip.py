@@ -184,6 +184,8 @@ def clip_grad_norm(
             for t, o, d in zip(dst, out, direct):
                 if not d:
                     o.copy_(t)
+        if any([o.requires_grad for o in out]):  # part of a graph: what it has saved of them is now stale
+            torch.autograd.graph.increment_version(out)
     return norm
 
 

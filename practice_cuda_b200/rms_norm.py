@@ -18,6 +18,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .registry import QuantResult
@@ -212,6 +213,7 @@ class _RMSNorm(torch.autograd.Function):
         return r.y, r.residual if residual is not None else None, q, scale
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh, _dq, _dscale):
         h, weight, rstd = ctx.saved_tensors
         if dy is None:  # y was not used: h alone carries a gradient
@@ -230,7 +232,7 @@ def rms_norm(
     fp8_dtype: torch.dtype = torch.float8_e4m3fn,
     pow2_scales: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor, Optional[QuantResult]]:
-    """Differentiable norm: ``(y, h, quant)``.
+    """Differentiable (once) norm: ``(y, h, quant)``.
 
     ``y`` and ``h`` (``x + residual``, or ``x``) carry gradients; ``quant`` is
     the FP8 quantization of ``y`` for the linears that read it (``None``

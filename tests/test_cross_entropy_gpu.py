@@ -93,6 +93,8 @@ SHAPES = [
     (1, 1, 8), (1, 2, 16), (3, 127, 64), (2, 128, 72), (7, 129, 136), (128, 256, 64), (129, 257, 128), (256, 512, 256),
     (300, 1000, 200), (257, 4099, 520), (1000, 777, 1024), (1, 40000, 256), (33, 20011, 512), (600, 300, 8),
     (5, 300, 1), (6, 301, 7), (130, 259, 65), (40, 1001, 333),  # widths that are not multiples of 16 bytes
+    (800, 515, 72), (900, 300, 77),  # many tokens on rows that do not start on lines
+    (300, 600, 768), (300, 600, 776), (140, 1500, 1288),  # tiles of one half, and a ragged second one
 ]
 
 
@@ -209,6 +211,15 @@ def test_only_the_gradients_that_are_needed():
     assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, w, target), w)[0], dw)
     with torch.no_grad():
         assert not linear_cross_entropy(x, w, target).requires_grad
+
+
+@gpu
+def test_differentiable_once():
+    x, w, target = _inputs(16, 64, 32, BF16, seed=17)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(linear_cross_entropy(x, w, target), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
 
 
 @gpu

@@ -185,6 +185,16 @@ def test_parameters_and_repeatability():
 
 
 @gpu
+def test_clipping_inside_a_graph_is_seen():
+    x = torch.ones(64, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    loss = (g * g).sum()  # keeps g
+    clip_grad_norm([g], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@gpu
 def test_stream_and_graph():
     g = _tensors([4097, 100], (F32,), seed=11)
     before = [t.clone() for t in g]
