@@ -15,8 +15,10 @@ bool fits_units(const void* p, int64_t row_stride, int es) {
 template <int XT, int YT, int LANES, int NV, int MAX_THREADS>
 int launch_norm_fwd(const norm::FwdArgs& p, int threads, cudaStream_t s) {
   const int64_t rows = LANES ? MAX_THREADS / (LANES ? LANES : 1) : 1;  // per CTA
-  norm::rms_norm_fwd_kernel<XT, YT, LANES, NV, MAX_THREADS>
-      <<<(unsigned)((p.rows + rows - 1) / rows), LANES ? MAX_THREADS : threads, 0, s>>>(p);
+  const unsigned grid = (unsigned)((p.rows + rows - 1) / rows);
+  const int block = LANES ? MAX_THREADS : threads;
+  if (p.res) norm::rms_norm_fwd_kernel<XT, YT, LANES, NV, MAX_THREADS, true><<<grid, block, 0, s>>>(p);
+  else norm::rms_norm_fwd_kernel<XT, YT, LANES, NV, MAX_THREADS, false><<<grid, block, 0, s>>>(p);
   return check_launch("rms_norm_fwd_kernel");
 }
 

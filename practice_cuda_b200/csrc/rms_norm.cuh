@@ -252,7 +252,7 @@ __device__ __forceinline__ float quant_factor(uint32_t amax_bits, const FwdArgs&
 // loaded with the row instead of where they are used, which costs registers: 122).
 // Bound by HBM traffic where all outputs are wanted (606 MB in 98 us, 6.2 TB/s), by
 // instruction issue where one FP8 byte is written for two bytes read.
-template <int XT, int YT, int LANES, int NV, int MAX_THREADS>
+template <int XT, int YT, int LANES, int NV, int MAX_THREADS, bool RES>
 __global__ void __launch_bounds__(MAX_THREADS) rms_norm_fwd_kernel(const FwdArgs p) {
   using T = typename InType<XT>::T;
   constexpr int ROWS = LANES ? MAX_THREADS / (LANES ? LANES : 1) : 1;  // per CTA
@@ -261,14 +261,15 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_norm_fwd_kernel(const FwdArgs
   const long long row = (long long)blockIdx.x * ROWS + (LANES ? threadIdx.x / (LANES ? LANES : 1) : 0);
   const bool live = row < p.rows;  // the lanes of a warp stay together for its shuffles
   const int units = live ? p.dim / kUnit : 0;
-  Raw8<T> hv[NV], rv[NV];
+  Raw8<T> hv[NV], rv[RES ? NV : 1];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int u = lane + i * lanes;
-    hv[i].zero(), rv[i].zero();
+    hv[i].zero();
+    if (RES) rv[RES ? i : 0].zero();
     if (u < units) {
       hv[i].load(static_cast<const T*>(p.x) + row * p.sx + u * kUnit);
-      if (p.res) rv[i].load(static_cast<const T*>(p.res) + row * p.sr + u * kUnit);
+      if (RES && p.res) rv[RES ? i : 0].load(static_cast<const T*>(p.res) + row * p.sr + u * kUnit);
     }
   }
   float2 ss2 = make_float2(0.f, 0.f);
@@ -278,9 +279,9 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_norm_fwd_kernel(const FwdArgs
     const int u = lane + i * lanes;
     float f[8];
     hv[i].unpack(f);
-    if (p.res) {
+    if (RES && p.res) {  // tested although it always holds: without it ptxas gives the loads more registers (133 us, not 97)
       float g[8];
-      rv[i].unpack(g);
+      rv[RES ? i : 0].unpack(g);
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
         const float2 t = __fadd2_rn(make_float2(f[k], f[k + 1]), make_float2(g[k], g[k + 1]));
