@@ -272,7 +272,8 @@ __device__ __forceinline__ void store_box(const Problem& q, const uint32_t (&w)[
 // bound by the tensor cores' operand stream: at 4096 tokens, 16384 columns and dim
 // 4096 on a B200, kStats takes 334 us (1.64 PFLOP/s, tensor pipe 92 % busy),
 // kGradient, which writes 134 MB of G beside it, 364 us (83 %).  On single CTAs
-// bound by reading W: 8 tokens of 32000 x 4096 in 47 us (5.6 TB/s).
+// bound by reading W: 8 tokens of 32000 x 4096 in 51 us with loss_rows_kernel
+// behind it (5.1 TB/s).
 template <int MODE, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_constant__ Params p) {
   using S = Smem<PAIR>;

@@ -8,8 +8,11 @@
 // the second sums the partials in a fixed order in every CTA (so no CTA waits
 // for another and nothing depends on the order of atomics) before it scales.
 // The second kernel walks the chunks from the last to the first: the end of
-// what the first one read is still in L2.  Bound by HBM traffic: each gradient
-// is read twice, less what L2 holds, and written once.
+// what the first one read is still in L2 (47 million bf16 values on a B200: 51.7 us,
+// from the first to the last 53.4 us).  Bound by HBM traffic, each gradient being
+// read twice, less what L2 holds, and written once: 2.2 billion bf16 values in
+// 2064 us (6.4 TB/s of 13.25 GB), 93 million in 100 us (5.6 TB/s), and by the call
+// itself below a few million values.
 //
 // Squares are summed in fp32 over the 16 or 32 elements that a thread loads
 // at a time and in fp64 from there on; a group whose fp32 sum is not finite
