@@ -156,7 +156,8 @@ int check_shapes(int dtype, int64_t tokens, int64_t vocab, int64_t dim, int redu
     return fail(PCB_ERR_INVALID, "linear cross entropy: reduction must be 0 (none), 1 (sum) or 2 (mean)");
   if (tokens > (1 << 26) || vocab > (1 << 26) || dim > (1 << 26))
     return fail(PCB_ERR_UNSUPPORTED, "linear cross entropy: dimension too large");
-  if (up(tokens, loss::TILE) * up(vocab, loss::TILE) > (1 << 30))
+  if (up(tokens, loss::TILE) * up(vocab, loss::TILE) > (1 << 30) ||
+      up(std::max(tokens, vocab), loss::TILE) * up(dim, loss::WIDE) > (1 << 24))  // (times at most 64 splits)
     return fail(PCB_ERR_UNSUPPORTED, "linear cross entropy: too many tiles");
   return PCB_OK;
 }

@@ -187,6 +187,8 @@ class FP8BlockLinear(nn.Linear):
         if quantized is not None:
             x_data, x_scale = quantized.tensor, quantized.dequant_scale
             blocks = (x2d.shape[0], -(-x2d.shape[1] // 128))
+            if self.scaling == "e8m0" and quantized.meta.get("scale_format") != "e8m0":
+                raise ValueError("an e8m0 linear needs its quantized input with power-of-two scales")
             if x_data.shape != x2d.shape or x_data.dtype != E4M3 or tuple(x_scale.shape) != blocks:
                 raise ValueError(f"quantized input must be e4m3 {tuple(x2d.shape)} with 1x128 scales {blocks}, got "
                                  f"{x_data.dtype} {tuple(x_data.shape)} with {tuple(x_scale.shape)}")

@@ -134,7 +134,8 @@ def rms_norm_quant(
     if x2 is not x:
         y = y.view(x.shape) if y is not None else None
         h = h.view(x.shape) if h is not None else None
-    return RMSNormResult(y, _quant_result(q, scale, quant) if q is not None else None, h if h is not None else x, rstd)
+    return RMSNormResult(y, _quant_result(q, scale, quant, pow2_scales) if q is not None else None,
+                         h if h is not None else x, rstd)
 
 
 def _like(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -144,8 +145,10 @@ def _like(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     return t.new_empty(t.shape) if dtype is None else t.new_empty(t.shape, dtype=dtype)
 
 
-def _quant_result(q: torch.Tensor, scale: torch.Tensor, quant: str) -> QuantResult:
+def _quant_result(q: torch.Tensor, scale: torch.Tensor, quant: str, pow2_scales: bool) -> QuantResult:
     meta = {"logical_shape": tuple(q.shape), "fp8_dtype": str(q.dtype)}
+    if pow2_scales:
+        meta["scale_format"] = "e8m0"
     if quant == "block":
         meta.update(block_m=1, block_n=_BLOCK)
         return QuantResult(q, scale, "b200_rms_norm", "block", meta)
@@ -239,5 +242,5 @@ def rms_norm(
     unless ``quant`` names a scheme), through which no gradient flows.
     """
     y, h, q, scale = _RMSNorm.apply(x, weight, residual, eps, quant, fp8_dtype, pow2_scales)
-    result = _quant_result(q, scale, quant) if q is not None else None
+    result = _quant_result(q, scale, quant, pow2_scales) if q is not None else None
     return y, h if h is not None else x, result

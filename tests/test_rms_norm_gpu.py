@@ -104,11 +104,26 @@ def test_forward_widths(rows, dim, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,dim", [(5, 512), (3, 4096), (9, 515), (2, 16392), (2, 20001)])
+@pytest.mark.parametrize("dtype,wdtype", [(BF16, F16), (F16, BF16), (F32, BF16), (F32, F16), (F16, F32)])
+def test_weights_of_another_type(rows, dim, dtype, wdtype):
+    x, r, w = _inputs(rows, dim, dtype, seed=rows * dim)
+    w = w.to(wdtype)
+    _check_forward(x, r, w, "block", E4M3, what="block")
+    res = _check_forward(x, None, w, "row", E4M3, what="row")
+    dx, dw = rms_norm_backward(r, x, w, res.rstd)
+    dx64, dw64, dx_terms, dw_terms = _backward_reference(r, x, w, res.rstd, None)
+    _close(dx, dx64, UNIT[dtype] * (1 + 1e-3), TINY[dtype] + RTOL32 * dx_terms, "dx")
+    _close(dw, dw64, UNIT[wdtype] * (1 + 1e-3), TINY[wdtype] + RTOL32 * dw_terms, "dw")
+
+
+@gpu
 @pytest.mark.parametrize("dim", [256, 1000, 129])
 @pytest.mark.parametrize("fp8", [E4M3, E5M2])
 def test_forward_power_of_two_scales(dim, fp8):
     x, r, w = _inputs(33, dim, BF16, seed=dim)
     res = _check_forward(x, r, w, "block", fp8, pow2=True, what="pow2")
+    assert res.quant.meta["scale_format"] == "e8m0"
     mantissa = res.quant.dequant_scale.view(torch.int32) & 0x7FFFFF
     assert int(mantissa.max()) == 0
 

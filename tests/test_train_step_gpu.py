@@ -88,6 +88,11 @@ def test_linear_with_a_quantized_input():
                 b200_per_block_quant(x.detach(), block_m=1, block_n=128, fp8_dtype=torch.float8_e5m2)):
         with pytest.raises(ValueError):
             lin(x, bad)
+    lin.scaling = "e8m0"  # whose GEMM reads the exponents of the scales alone
+    with pytest.raises(ValueError, match="power-of-two"):
+        lin(x, q)
+    q2 = b200_per_block_quant(x.detach(), block_m=1, block_n=128, pow2_scales=True)
+    assert torch.equal(lin(x, q2), lin(x))
 
 
 def test_no_layers():
