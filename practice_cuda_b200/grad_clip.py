@@ -37,18 +37,20 @@ def _norm_code(norm_type: float, what: str) -> int:
         raise ValueError(f"{what}: norm_type must be 2 or inf, got {norm_type!r}") from None
 
 
-def _as_list(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], what: str) -> list[torch.Tensor]:
+def _as_list(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], what: str):
+    """The tensors and their types."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         raise ValueError(f"{what}: no tensors (their device is where the norm goes)")
     first = tensors[0]
-    for dtype in {t.dtype for t in tensors}:
+    dtypes = [t.dtype for t in tensors]
+    for dtype in set(dtypes):
         if dtype not in _DTYPE_CODES:
             raise ValueError(f"{what}: gradients must be bf16, fp16 or fp32, got {dtype}")
     if len(set(map(_device, tensors))) != 1:
         raise ValueError(f"{what}: gradients on {sorted({str(t.device) for t in tensors})}")
     _lib.require_cuda(first, "gradients")
-    return tensors
+    return tensors, dtypes
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -70,10 +72,10 @@ def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
 class _Table:
     """The host arrays of one call: pointers, sizes and types."""
 
-    def __init__(self, tensors: Sequence[torch.Tensor]):
+    def __init__(self, tensors: Sequence[torch.Tensor], dtypes: Sequence[torch.dtype]):
         self.pointers = array("Q", map(_pointer, tensors))
         self.sizes = array("q", map(_numel, tensors))
-        self.types = array("i", [_DTYPE_CODES[t.dtype] for t in tensors])
+        self.types = array("i", [_DTYPE_CODES[t] for t in dtypes])
         self.count = len(tensors)
 
     def args(self) -> tuple[int, int, int]:
@@ -89,12 +91,12 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], *, norm_type
     """The norm over all tensors: a 0-dim fp32 tensor on their device."""
     what = "grad_norm"
     code = _norm_code(norm_type, what)
-    tensors = _as_list(tensors, what)
+    tensors, dtypes = _as_list(tensors, what)
     device = tensors[0].device
     with _lib.on_device(device):
         # A view whose elements do not fill one stretch of memory is copied.
         tensors = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in tensors]
-        table = _Table(tensors)
+        table = _Table(tensors, dtypes)
         norm = torch.empty((), device=device, dtype=torch.float32)
         workspace, nbytes = _workspace(table.count, device)
         status = _lib.lib().pcb_grad_norm(table.pointers.buffer_info()[0], *table.args(), code, norm.data_ptr(),
@@ -104,24 +106,23 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], *, norm_type
     return norm
 
 
-def _targets(tensors: list[torch.Tensor], out: Optional[Sequence[torch.Tensor]], what: str) -> list[torch.Tensor]:
-    if out is None:
-        out = tensors
-    else:
-        out = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(out) != len(tensors):
-            raise ValueError(f"{what}: {len(out)} outputs for {len(tensors)} gradients")
-        if ([o.shape for o in out] != [t.shape for t in tensors] or [o.dtype for o in out] != [t.dtype for t in tensors]
-                or set(map(_device, out)) != set(map(_device, tensors))):
-            for t, o in zip(tensors, out):
-                if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
-                    raise ValueError(f"{what}: an output is {tuple(o.shape)} {o.dtype} on {o.device}, "
-                                     f"its gradient {tuple(t.shape)} {t.dtype} on {t.device}")
-    if not all(map(_contiguous, out)):
-        for o in out:
-            if not _dense(o) and any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
-                raise ValueError(f"{what}: cannot write to an expanded tensor of shape {tuple(o.shape)}")
+def _targets(tensors, dtypes, out: Sequence[torch.Tensor], what: str) -> list[torch.Tensor]:
+    out = [out] if isinstance(out, torch.Tensor) else list(out)
+    if len(out) != len(tensors):
+        raise ValueError(f"{what}: {len(out)} outputs for {len(tensors)} gradients")
+    if ([o.shape for o in out] != [t.shape for t in tensors] or [o.dtype for o in out] != dtypes
+            or set(map(_device, out)) != {tensors[0].get_device()}):
+        for t, o in zip(tensors, out):
+            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device:
+                raise ValueError(f"{what}: an output is {tuple(o.shape)} {o.dtype} on {o.device}, "
+                                 f"its gradient {tuple(t.shape)} {t.dtype} on {t.device}")
     return out
+
+
+def _check_writable(out: Sequence[torch.Tensor], what: str) -> None:
+    for o in out:
+        if not _dense(o) and any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+            raise ValueError(f"{what}: cannot write to an expanded tensor of shape {tuple(o.shape)}")
 
 
 def clip_grad_norm(
@@ -148,20 +149,22 @@ def clip_grad_norm(
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"{what}: max_norm must not be negative, got {max_norm}")
-    tensors = _as_list(tensors, what)
-    out = _targets(tensors, out, what)
+    tensors, dtypes = _as_list(tensors, what)
+    in_place = out is None
+    out = tensors if in_place else _targets(tensors, dtypes, out, what)
     device = tensors[0].device
     lib = _lib.lib()
     with _lib.on_device(device):
         # Views that do not fill one stretch of memory, or whose output lies in
         # another order, pass through a contiguous copy.
         src, dst, direct = tensors, out, None
-        if not (all(map(_contiguous, tensors)) and all(map(_contiguous, out))):
+        if not (all(map(_contiguous, out)) and (in_place or all(map(_contiguous, tensors)))):
+            _check_writable(out, what)
             direct = [_dense(t) and _dense(o) and _same_order(t, o) for t, o in zip(tensors, out)]
             src = [t if d else t.contiguous() for t, d in zip(tensors, direct)]
             dst = [o if d else torch.empty_like(t) for t, o, d in zip(src, out, direct)]
-        table = _Table(src)
-        targets = array("Q", map(_pointer, dst))
+        table = _Table(src, dtypes)
+        targets = table.pointers if dst is src else array("Q", map(_pointer, dst))
         pointers, targets_at = table.pointers.buffer_info()[0], targets.buffer_info()[0]
         stream = _lib.stream_ptr(device)
         if group is None and not error_if_nonfinite:
