@@ -192,11 +192,50 @@ struct FwdPlan {
   }
 };
 
+// Short tiles that workers with one long tile less take in its place.
+int extra_of(int long_tiles, int long_stages, int short_tiles, int short_stages, int workers) {
+  const int left = long_tiles % workers;
+  if (left == 0 || short_tiles == 0 || long_tiles + short_tiles < workers) return 0;
+  return std::min(long_stages / short_stages, short_tiles / (workers - left));
+}
+
+// Parts that dX's K (the vocabulary) is cut into.  Its tiles are few and long
+// where tokens are few; more parts even out the pairs' shares and cost the
+// writing and reading of their fp32 accumulators.  The shares are counted in
+// stages (0.27 us of the tensor cores) as the kernel hands them out: a tile's
+// epilogue is worth about six stages, a stage's time about 1.7 MB of traffic, and
+// the joining kernel about ten stages of its own.
+int split_of(int64_t tokens, int64_t vocab, int64_t dim, bool want_dw) {
+  const int workers = std::max(1, device_info().sm_count / 2);
+  const int64_t cols = up(dim, loss::WIDE), stages = up(vocab, loss::BK), halves = dim > loss::TILE ? 2 : 1;
+  const int64_t dx_tiles = up(tokens, loss::TILE) * cols, dw_tiles = want_dw ? up(vocab, loss::TILE) * cols : 0;
+  const int64_t dw_stages = up(tokens, loss::BK);
+  if (dx_tiles >= 8 * workers) return 1;  // long rounds already come out nearly even
+  int best = 1;
+  double least = 0;
+  for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (stages / s < 4 && s > 1) break;
+    const int part = (int)up(stages, s), t0 = (int)(dx_tiles * up(stages, part));
+    const int extra = extra_of(t0, part, (int)dw_tiles, (int)dw_stages, workers);
+    int64_t longest = 0;
+    for (int w = 0; w < workers; ++w) {
+      int64_t longs = (t0 - w + workers - 1) / workers;
+      const int r = t0 % workers;
+      int64_t left = dw_tiles - (r > 0 ? (int64_t)extra * (workers - r) : 0), shorts = r > 0 && w >= r ? extra : 0;
+      shorts += std::max<int64_t>(0, (left - (w >= r ? w - r : w - r + workers) + workers - 1) / workers);
+      longest = std::max(longest, longs * (part * halves + 6) + shorts * (dw_stages * halves + 6));
+    }
+    const double cost = (double)longest + (s > 1 ? 10 + (double)s * tokens * dim * 8 / 1.7e6 : 0);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
+}
+
 struct BwdPlan {
   int64_t cols, pieces, pitch;  // of G
   int splits;                   // parts of K of dX
   int64_t g, acc, weight, alpha, bytes;
-  BwdPlan(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, bool want_dx) {
+  BwdPlan(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, bool want_dx, bool want_dw) {
     // G of one piece takes 128 MiB at most (and is no narrower than 2048
     // columns): pieces of even width, whole tiles each.
     if (piece <= 0) piece = std::max<int64_t>(2048, ((int64_t)128 << 20) / 2 / tokens);
@@ -205,16 +244,8 @@ struct BwdPlan {
     cols = up(up(vocab, pieces), loss::TILE) * loss::TILE;
     pieces = up(vocab, cols);
     pitch = std::min(cols, up(vocab, 64) * 64);
-    splits = 1;
     const int64_t dx_tiles = up(tokens, loss::TILE) * up(dim, loss::WIDE);
-    if (want_dx && pieces == 1) {
-      // dX's tiles are few and long where tokens are few: cut them along the
-      // vocabulary so that none is longer than a quarter of an SM pair's share.
-      const int64_t stages = up(vocab, loss::BK);
-      const int64_t all = dx_tiles * stages + up(vocab, loss::TILE) * up(dim, loss::WIDE) * up(tokens, loss::BK);
-      const int64_t longest = std::max<int64_t>(16, all / (4 * std::max(1, device_info().sm_count / 2)));
-      splits = (int)std::min<int64_t>(std::max<int64_t>(1, stages / longest), 64);
-    }
+    splits = want_dx && pieces == 1 ? split_of(tokens, vocab, dim, want_dw) : 1;
     Cut c;
     g = c.take(tokens * pitch * 2);
     acc = c.take(want_dx && (pieces > 1 || splits > 1) ? dx_tiles * splits * loss::TILE * loss::WIDE * 4 : 0);
@@ -297,9 +328,10 @@ int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw,
   return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), loss::kRowWarps * 32, s, r);
 }
 
-int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx) {
+int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx,
+                                          int want_dw) {
   if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
-  return BwdPlan(tokens, vocab, dim, piece, want_dx != 0).bytes;
+  return BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0).bytes;
 }
 
 int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
@@ -315,7 +347,7 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
   }
   if (!dx && !dw) return PCB_OK;
   if (!target || !stats || !count || !dloss) return fail(PCB_ERR_INVALID, "null pointer");
-  const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr);
+  const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr, dw != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
     return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
   if (int st = check_operands(x, sx, weight, sw)) return st;
@@ -386,17 +418,17 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
     if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
     p.num_tiles = p.prob[0].tiles;
     if (n > 1) {
-      const int pairs = device_info().sm_count / 2, left = p.prob[0].tiles % pairs;
       p.num_tiles += p.prob[1].tiles;
-      if (left > 0 && p.num_tiles >= pairs)
-        p.extra = std::min(p.prob[0].split_stages / p.prob[1].k_stages, p.prob[1].tiles / (pairs - left));
+      p.extra = extra_of(p.prob[0].tiles, p.prob[0].split_stages, p.prob[1].tiles, p.prob[1].k_stages,
+                         device_info().sm_count / 2);
     }
     if (int st = launch_grad_products(p, s)) return st;
     if (dx && plan.splits > 1) {
       const loss::Problem& d = p.prob[0];
-      const loss::JoinArgs j{acc, d.m, d.n, d.m_blocks, d.n_blocks, d.splits, p.fmt, static_cast<uint16_t*>(dx), sdx};
+      const loss::JoinArgs j{acc, d.m, d.n, d.m_blocks, d.n_blocks, d.splits, p.fmt, static_cast<uint16_t*>(dx), sdx,
+                             d.c_tma};
       if (int st = launch_after(loss::loss_join_kernel, "loss_join_kernel",
-                                (int64_t)d.m_blocks * d.n_blocks * 4 * loss::kAccVec, 256, s, j, p))
+                                (int64_t)d.m_blocks * d.n_blocks * 4 * loss::kJoinParts, 256, s, j, p))
         return st;
     }
   }

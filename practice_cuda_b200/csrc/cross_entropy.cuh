@@ -186,26 +186,28 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, int fmt) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The tile that worker `w` of `workers` (CTAs or pairs) takes in turn `i`, or -1.
-// Workers take turns.  Where prob[0]'s long tiles do not come out even, the
-// workers with one less of them take `extra` of prob[1]'s short ones in its
-// place, and the turns go on from there.
-__device__ __forceinline__ int tile_of(const Params& p, int w, int workers, int i) {
-  const int t0 = p.prob[0].tiles;
+// The tile that worker `w` of `workers` (CTAs or pairs) takes in turn `i`, or -1:
+// of t0 long tiles and then total - t0 short ones.  Workers take turns.  Where the
+// long tiles do not come out even, the workers with one less of them take `extra`
+// short ones in its place, and the turns go on, beginning with them.
+__host__ __device__ __forceinline__ int tile_of(int t0, int total, int extra, int w, int workers, int i) {
   const int own = (t0 - w + workers - 1) / workers;
   if (i < own) return i * workers + w;
   i -= own;
-  int at = t0;
   const int r = t0 % workers;
-  if (p.extra) {  // only where r > 0
+  int at = t0;
+  if (r > 0) {
     if (w >= r) {
-      if (i < p.extra) return t0 + i * (workers - r) + (w - r);
-      i -= p.extra;
+      if (i < extra) return t0 + i * (workers - r) + (w - r);
+      i -= extra;
     }
-    at += p.extra * (workers - r);
+    at += extra * (workers - r);
   }
-  const int tile = at + i * workers + w;
-  return tile < p.num_tiles ? tile : -1;
+  const int tile = at + i * workers + (w >= r ? w - r : w - r + workers);
+  return tile < total ? tile : -1;
+}
+__device__ __forceinline__ int tile_of(const Params& p, int w, int workers, int i) {
+  return tile_of(p.prob[0].tiles, p.num_tiles, p.extra, w, workers, i);
 }
 
 struct TileAt {
@@ -778,7 +780,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
         float4* acc = nullptr;
         if (q.acc_mode != kAccNone)
           acc = q.acc + (((long long)t.index * 2 + rank) * 2 + h) * kAccVec * 256 + ew * 32 + lane;
-        if (add) {
+        const bool in = row0 + lane < q.m;
+        if (add && in) {
 #pragma unroll
           for (int c = 0; c < EPI_COLS / 32; ++c)
 #pragma unroll
@@ -800,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
                            __uint_as_float(v[2 * b + j / 16][2 * j % 32 + 1]) * alpha, p.fmt);
             store_box(q, w, stg, lane, row0, col0 + b * 64, q.n);
           }
-        } else {
+        } else if (in) {
 #pragma unroll
           for (int c = 0; c < EPI_COLS / 32; ++c)
 #pragma unroll
@@ -995,37 +998,56 @@ __global__ void __launch_bounds__(256) repack_rows_kernel(const uint16_t* src, l
   }
 }
 
-// dX from the parts of K: the fp32 accumulators of every part summed in order.
+// dX from the parts of K: the fp32 accumulators of all parts summed in order.
+// A thread has 32 columns of a row, 64 bytes of what it writes.
 struct JoinArgs {
   const float4* acc;
   int m, n, m_blocks, n_blocks, splits, fmt;
   uint16_t* out;
   long long stride;
+  int vec;  // rows of out start on 16 bytes
 };
+constexpr int kJoinVecs = 8;                       // float4s of a thread
+constexpr int kJoinParts = kAccVec / kJoinVecs;    // of an epilogue thread's share of a half
 __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs p, const __grid_constant__ Params pp) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float alpha = alpha_of(pp);
-  // blockIdx.x: (tile of the first part, CTA of the pair, half, float4 of the thread)
-  const int i = blockIdx.x % kAccVec, h = blockIdx.x / kAccVec % 2, rank = blockIdx.x / kAccVec / 2 % 2;
-  const int index = blockIdx.x / kAccVec / 4;
+  // blockIdx.x: (tile of the first part, CTA of the pair, half, 32 of a thread's 128 columns)
+  const int g = blockIdx.x % kJoinParts, h = blockIdx.x / kJoinParts % 2, rank = blockIdx.x / kJoinParts / 2 % 2;
+  const int index = blockIdx.x / kJoinParts / 4;
   const int ew = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TileAt t = locate(pp, index);
   const int row = t.mb * TILE + rank * BM + (ew & 3) * 32 + lane;
-  const int col = t.nb * WIDE + h * TILE + (ew >> 2) * EPI_COLS + i * 4;
+  const int col = t.nb * WIDE + h * TILE + (ew >> 2) * EPI_COLS + g * kJoinVecs * 4;
   if (row >= p.m || col >= p.n) return;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 v[kJoinVecs];
+#pragma unroll
+  for (int j = 0; j < kJoinVecs; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
   const long long part = (long long)p.m_blocks * p.n_blocks * 4 * kAccVec * 256;
-  const float4* a = p.acc + ((((long long)index * 2 + rank) * 2 + h) * kAccVec + i) * 256 + threadIdx.x;
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const float4 o = a[s * part];
-    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+  const float4* a = p.acc + ((((long long)index * 2 + rank) * 2 + h) * kAccVec + g * kJoinVecs) * 256 + threadIdx.x;
+  for (int s = 0; s < p.splits; ++s, a += part) {
+#pragma unroll
+    for (int j = 0; j < kJoinVecs; ++j) {
+      const float4 o = a[j * 256];
+      v[j].x += o.x, v[j].y += o.y, v[j].z += o.z, v[j].w += o.w;
+    }
   }
-  const float f[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
   uint16_t* out = p.out + (long long)row * p.stride + col;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (col + k < p.n) out[k] = (uint16_t)pack2(f[k], 0.f, p.fmt);
+  for (int j = 0; j < kJoinVecs; j += 2) {
+    const float4 x = v[j], y = v[j + 1];
+    const uint4 w = make_uint4(pack2(x.x * alpha, x.y * alpha, p.fmt), pack2(x.z * alpha, x.w * alpha, p.fmt),
+                               pack2(y.x * alpha, y.y * alpha, p.fmt), pack2(y.z * alpha, y.w * alpha, p.fmt));
+    const int c = 4 * j;
+    if (p.vec && col + c + 8 <= p.n) {
+      *reinterpret_cast<uint4*>(out + c) = w;
+    } else {
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col + c + k < p.n) out[c + k] = (uint16_t)(u[k / 2] >> (16 * (k & 1)));
+    }
+  }
 }
 
 }  // namespace loss

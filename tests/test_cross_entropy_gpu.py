@@ -342,6 +342,6 @@ def test_entry_points_reject_bad_arguments_without_gpu():
     assert forward(tokens=0) == _lib.PCB_OK
     assert forward(sx=17) == _lib.PCB_ERR_LAYOUT and forward(x=264) == _lib.PCB_ERR_LAYOUT
     assert forward(vocab=1 << 40) == _lib.PCB_ERR_UNSUPPORTED
-    need = lib.pcb_linear_ce_bwd_workspace_bytes(4096, 32000, 4096, 0, 1)
+    need = lib.pcb_linear_ce_bwd_workspace_bytes(4096, 32000, 4096, 0, 1, 1)
     # one piece of G (at most 128 MiB) and dX's accumulators, not the logits of the whole vocabulary
     assert need < (128 << 20) + 4096 * 4096 * 4 + (1 << 20)
