@@ -415,6 +415,27 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
                       int64_t sdw, int64_t piece, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * The same two passes, which spend nothing on the products of tokens that are
+ * left out: the others are packed in front, in their order, and only they are
+ * multiplied.  How many there are is known to the device alone.  `packed` is
+ * device state of pcb_linear_ce_packed_bytes() bytes, 256-byte aligned, that the
+ * forward pass writes (each token's place, and a copy of x in that order) and the
+ * backward pass reads; stats are then in that order too.  Where the products are
+ * too small to gain from it, that size is 0, `packed` must be NULL and the passes
+ * are the plain ones.
+ */
+int64_t pcb_linear_ce_packed_bytes(int64_t tokens, int64_t vocab, int64_t dim);
+int pcb_linear_ce_packed_fwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                             int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                             float* loss, float* stats, float* count, void* packed, int64_t packed_bytes,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+int pcb_linear_ce_packed_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                             int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                             const float* stats, const float* count, const void* packed, int64_t packed_bytes,
+                             const float* dloss, void* dx, int64_t sdx, void* dw, int64_t sdw, int64_t piece,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Copy of [rows, cols] 16-bit elements between row strides (in elements;
  * columns contiguous on both sides): what gives pcb_linear_ce_* rows that
  * start on 16-byte boundaries, or on 128-byte lines.  dst: 4-byte aligned, an

@@ -155,6 +155,20 @@ _SIGNATURES = {
          _vp, _i64, _vp, _i64, _i64,  # dx, dw, piece
          _vp, _i64, _vp],
     ),
+    "pcb_linear_ce_packed_bytes": (_i64, [_i64, _i64, _i64]),
+    "pcb_linear_ce_packed_fwd": (
+        _i,
+        [_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64,  # x, weight, dtype, tokens, vocab, dim
+         _vp, _i64, _i, _vp, _vp, _vp,  # target, ignore index, reduction, loss, stats, count
+         _vp, _i64, _vp, _i64, _vp],  # packed, workspace
+    ),
+    "pcb_linear_ce_packed_bwd": (
+        _i,
+        [_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64,  # x, weight, dtype, tokens, vocab, dim
+         _vp, _i64, _i, _vp, _vp, _vp, _i64, _vp,  # target, ignore index, reduction, stats, count, packed, dloss
+         _vp, _i64, _vp, _i64, _i64,  # dx, dw, piece
+         _vp, _i64, _vp],
+    ),
     "pcb_pack_u8": (_i, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp]),
 }
 

@@ -89,27 +89,30 @@ def _forward(x, weight, target, ignore_index, reduction, train):
         nbytes = lib.pcb_linear_ce_fwd_workspace_bytes(tokens, vocab)
         workspace = x.new_empty((nbytes,), dtype=torch.uint8)
         at = stats.data_ptr()
-        status = lib.pcb_linear_ce_fwd(
+        packed_bytes = lib.pcb_linear_ce_packed_bytes(tokens, vocab, dim)
+        packed = x.new_empty((packed_bytes,), dtype=torch.uint8) if packed_bytes else None
+        status = lib.pcb_linear_ce_packed_fwd(
             x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x.dtype], tokens, vocab, dim,
             target.data_ptr(), ignore_index, reduction, loss.data_ptr(), at, at + 8 * tokens,
+            packed.data_ptr() if packed_bytes else None, packed_bytes,
             workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
         if status:
-            _lib.check(status, "pcb_linear_ce_fwd")
-    return loss, x2, w2, stats
+            _lib.check(status, "pcb_linear_ce_packed_fwd")
+    return loss, x2, w2, stats, packed
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction, piece):
-        loss, x2, w2, stats = _forward(x, weight, target, ignore_index, reduction, True)
-        ctx.save_for_backward(x2, w2, target, stats)
+        loss, x2, w2, stats, packed = _forward(x, weight, target, ignore_index, reduction, True)
+        ctx.save_for_backward(x2, w2, target, stats, packed)
         ctx.args = (ignore_index, reduction, piece)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x2, w2, target, stats = ctx.saved_tensors
+        x2, w2, target, stats, packed = ctx.saved_tensors
         ignore_index, reduction, piece = ctx.args
         tokens, dim = x2.shape
         vocab = w2.shape[0]
@@ -123,13 +126,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
             nbytes = lib.pcb_linear_ce_bwd_workspace_bytes(tokens, vocab, dim, piece, want_dx, want_dw)
             workspace = x2.new_empty((nbytes,), dtype=torch.uint8)
             at = stats.data_ptr()
-            status = lib.pcb_linear_ce_bwd(
+            status = lib.pcb_linear_ce_packed_bwd(
                 x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _lib.PCB_DTYPE[x2.dtype], tokens, vocab, dim,
-                target.data_ptr(), ignore_index, reduction, at, at + 8 * tokens, dloss.data_ptr(),
-                dx.data_ptr() if want_dx else None, dim, dw.data_ptr() if want_dw else None, dim, piece,
-                workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
+                target.data_ptr(), ignore_index, reduction, at, at + 8 * tokens,
+                packed.data_ptr() if packed is not None else None, packed.numel() if packed is not None else 0,
+                dloss.data_ptr(), dx.data_ptr() if want_dx else None, dim, dw.data_ptr() if want_dw else None, dim,
+                piece, workspace.data_ptr(), nbytes, _lib.stream_ptr(device))
             if status:
-                _lib.check(status, "pcb_linear_ce_bwd")
+                _lib.check(status, "pcb_linear_ce_packed_bwd")
         return dx, dw, None, None, None, None
 
 
@@ -151,6 +155,10 @@ def linear_cross_entropy(
     is not computed.  ``vocab_piece`` bounds the columns of the logits' gradient
     that exist at a time in the backward pass (rounded down to a multiple of
     256, at least 256; default: as many as fit 128 MiB, at least 2048).
+
+    Tokens left out of large products (512 tokens or more, ``tokens * vocab * dim``
+    of 2^36 or more) take no part in them: the others are packed, which keeps a
+    copy of ``x`` until the backward pass.
 
     A target outside the vocabulary that is not ``ignore_index`` makes its
     loss NaN and sets the device error word (``_lib.device_error``).

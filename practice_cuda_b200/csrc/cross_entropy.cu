@@ -42,9 +42,10 @@ bool slab_map(CUtensorMap* map, const void* base, int dt, int64_t slabs, int64_t
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // B of a product of G: [rows, dim], dim contiguous.
-bool load_b(loss::Problem& q, const void* base, int dt, int64_t dim, int64_t rows, int64_t stride) {
+bool load_b(CUtensorMap* map, loss::Problem& q, const void* base, int dt, int64_t dim, int64_t rows, int64_t stride) {
   q.b_slabs = dim % 64 == 0 ? 1 : 0;
-  return q.b_slabs ? slab_map(&q.b, base, dt, dim / 64, rows, stride) : load_map(&q.b, base, dt, dim, rows, stride, loss::BK);
+  if (q.b_slabs) return slab_map(map, base, dt, dim / 64, rows, stride);
+  return load_map(map, base, dt, dim, rows, stride, loss::BK);
 }
 bool store_map(CUtensorMap* map, void* base, int dt, int64_t inner, int64_t outer, int64_t stride) {
   return make_map(map, base, dt, inner, outer, stride, 32, CU_TENSOR_MAP_L2_PROMOTION_NONE);
@@ -180,6 +181,41 @@ struct Cut {
   }
 };
 
+// Where the logits take about 90 us or more, tokens that are left out are packed
+// away.  Packed and as they are, on a B200, loss / loss and gradients in us: 1021
+// tokens of 50001 x 2056 fp16 with 30 % left out 154 / 760 and 216 / 889, with 60 %
+// 121 / 598 and 216 / 864, with none 204 / 809 and 199 / 802; 4096 tokens of 32000 x
+// 4096 with 30 % 668 / 2456 and 833 / 3150; 2048 tokens of 8192 x 4096 with 30 % 121 /
+// 384 and 136 / 469.  It costs three launches, 5 to 10 us, where no token is left
+// out, and below this size that is more than most masks save.  The gain comes
+// in whole tiles of 256 tokens: 768 tokens with 30 % left out keep their three (180
+// / 653 and 177 / 671), hence no fewer than two of them.
+bool packs(int64_t tokens, int64_t vocab, int64_t dim) {
+  return tokens >= 512 && (double)tokens * vocab * dim >= (double)(1ll << 36);
+}
+
+// What the forward pass leaves for the backward pass of packed tokens.  G takes
+// their order too, so dX leaves the products' kernel row by row to its own places
+// (16 bytes a lane); the copy of x is what dW's product reads.
+struct Order {
+  int64_t live, order, target, x, stride, bytes;
+  Order(int64_t tokens, int64_t vocab, int64_t dim) {
+    Cut c;
+    stride = up(dim, 64) * 64;  // elements
+    live = c.take(4);
+    order = c.take(tokens * 4);
+    target = c.take(tokens * 8);
+    x = c.take(tokens * stride * 2);
+    bytes = packs(tokens, vocab, dim) ? c.at : 0;
+  }
+  void use(loss::Params& p, const void* state) const {
+    const char* s = static_cast<const char*>(state);
+    p.live = reinterpret_cast<const int*>(s + live);
+    p.order = reinterpret_cast<const int*>(s + order);
+    p.target_packed = reinterpret_cast<const long long*>(s + target);
+  }
+};
+
 struct FwdPlan {
   int64_t partial, target_logit, sums, ticket, bytes;
   FwdPlan(int64_t tokens, int64_t vocab) {
@@ -191,13 +227,6 @@ struct FwdPlan {
     bytes = c.at;
   }
 };
-
-// Short tiles that workers with one long tile less take in its place.
-int extra_of(int long_tiles, int long_stages, int short_tiles, int short_stages, int workers) {
-  const int left = long_tiles % workers;
-  if (left == 0 || short_tiles == 0 || long_tiles + short_tiles < workers) return 0;
-  return std::min(long_stages / short_stages, short_tiles / (workers - left));
-}
 
 // Parts that dX's K (the vocabulary) is cut into.  Its tiles are few and long
 // where tokens are few; more parts even out the pairs' shares and cost the
@@ -216,7 +245,7 @@ int split_of(int64_t tokens, int64_t vocab, int64_t dim, bool want_dw) {
   for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
     if (stages / s < 4 && s > 1) break;
     const int part = (int)up(stages, s), t0 = (int)(dx_tiles * up(stages, part));
-    const int extra = extra_of(t0, part, (int)dw_tiles, (int)dw_stages, workers);
+    const int extra = loss::extra_of(t0, part, (int)dw_tiles, (int)dw_stages, workers);
     int64_t longest = 0;
     for (int w = 0; w < workers; ++w) {
       int64_t longs = (t0 - w + workers - 1) / workers;
@@ -255,14 +284,192 @@ struct BwdPlan {
   }
 };
 
-loss::Params base_params(int dtype, int64_t vocab, const int64_t* target, int64_t ignore_index) {
+loss::Params base_params(int dtype, int64_t tokens, int64_t vocab, const int64_t* target, int64_t ignore_index) {
   loss::Params p;
   std::memset(&p, 0, sizeof(p));
   p.fmt = dtype == PCB_DTYPE_BF16 ? 1 : 0;
+  p.tokens = (int)tokens;
   p.target = reinterpret_cast<const long long*>(target);
   p.ignore_index = ignore_index;
   p.vocab = vocab;
   return p;
+}
+
+// The entry points' own argument of packed tokens.
+int check_packed(int dtype, int64_t tokens, int64_t vocab, int64_t dim, int reduction, const void* packed,
+                 int64_t packed_bytes) {
+  if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
+  const int64_t need = tokens > 0 ? Order(tokens, vocab, dim).bytes : 0;
+  if (need ? !packed || !aligned(packed, 256) || packed_bytes < need : packed != nullptr)
+    return fail(PCB_ERR_INVALID, "linear cross entropy: packed state missing, too small, misaligned or not needed");
+  return PCB_OK;
+}
+
+// `order` (null: every token is multiplied, in its own place) is the state that
+// the forward pass leaves for the backward pass of packed tokens.
+int forward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                      int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                      float* loss_out, float* stats, float* count, void* order, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
+  if (tokens == 0) return PCB_OK;
+  if (!target || !loss_out || !stats || !count) return fail(PCB_ERR_INVALID, "null pointer");
+  const FwdPlan plan(tokens, vocab);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
+    return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
+  if (int st = check_operands(x, sx, weight, sw)) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  char* ws = static_cast<char*>(workspace);
+  loss::Params p = base_params(dtype, tokens, vocab, target, ignore_index);
+  loss::Problem& q = p.prob[0];
+  const Order packed(tokens, vocab, dim);
+  if (order) {
+    char* at = static_cast<char*>(order);
+    int* places = reinterpret_cast<int*>(at + packed.order);
+    int* live = reinterpret_cast<int*>(at + packed.live);
+    if (int st = launch_after(loss::loss_order_kernel, "loss_order_kernel", 1, 1024, s, p.target,
+                              (long long)ignore_index, (int)tokens, places, live))
+      return st;
+    if (int st = launch_after(loss::loss_pack_kernel, "loss_pack_kernel",
+                              std::min<int64_t>(tokens, (int64_t)device_info().sm_count * 8), 256, s,
+                              static_cast<const uint16_t*>(x), (long long)sx, p.target, (const int*)places,
+                              (const int*)live, (int)tokens, (int)dim, reinterpret_cast<uint16_t*>(at + packed.x),
+                              (long long)packed.stride, reinterpret_cast<long long*>(at + packed.target)))
+      return st;
+    packed.use(p, order);
+  }
+  const bool pair = on_pairs(tokens);
+  p.tile_n = logit_tile(tokens, vocab);
+  shape(q, tokens, vocab, dim, 1, pair, p.tile_n);
+  q.m_live = 1;
+  if (order && !load_map(&q.packed, static_cast<char*>(order) + packed.x, dtype, dim, tokens, packed.stride, q.a_rows))
+    return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
+  if (!load_map(&q.a, x, dtype, dim, tokens, sx, q.a_rows) ||
+      !load_map(&q.b, weight, dtype, dim, vocab, sw, pair ? loss::TILE / 2 : p.tile_n))
+    return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
+  p.num_tiles = q.tiles;
+  p.partial = reinterpret_cast<float2*>(ws + plan.partial);
+  p.target_logit = reinterpret_cast<float*>(ws + plan.target_logit);
+  p.ticket = reinterpret_cast<unsigned*>(ws + plan.ticket);
+  if (int st = launch_logits<loss::kStats>(p, pair, s)) return st;
+  loss::RowArgs r{p.live, p.order, p.partial, p.target_logit, p.target, ignore_index, vocab, (int)tokens,
+                  2 * q.n_blocks, reduction, stats, loss_out, count, reinterpret_cast<double*>(ws + plan.sums), p.ticket};
+  return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), loss::kRowWarps * 32, s, r);
+}
+
+int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                      int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                      const float* stats, const float* count, const void* order,
+                      const float* dloss, void* dx, int64_t sdx, void* dw, int64_t sdw, int64_t piece, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (tokens == 0) {
+    if (dw && cudaMemset2DAsync(dw, (size_t)sdw * 2, 0, (size_t)dim * 2, (size_t)vocab, s) != cudaSuccess)
+      return check_launch("linear cross entropy dw");
+    return PCB_OK;
+  }
+  if (!dx && !dw) return PCB_OK;
+  if (!target || !stats || !count || !dloss) return fail(PCB_ERR_INVALID, "null pointer");
+  const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr, dw != nullptr);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
+    return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
+  if (int st = check_operands(x, sx, weight, sw)) return st;
+  char* ws = static_cast<char*>(workspace);
+  void* g = ws + plan.g;
+  float4* acc = reinterpret_cast<float4*>(ws + plan.acc);
+  loss::Params base = base_params(dtype, tokens, vocab, target, ignore_index);
+  base.stats = stats;
+  const Order packed(tokens, vocab, dim);
+  const void* packed_x = nullptr;
+  if (order) {
+    packed.use(base, order);
+    packed_x = static_cast<const char*>(order) + packed.x;
+    if (dx)
+      if (int st = launch_after(loss::loss_zero_rows_kernel, "loss_zero_rows_kernel",
+                                std::min<int64_t>(tokens, (int64_t)device_info().sm_count * 8), 256, s, base.order,
+                                base.live, (int)tokens, (int)dim, static_cast<uint16_t*>(dx), (long long)sdx,
+                                aligned(dx, 16) && sdx % 8 == 0 ? 1 : 0))
+        return st;
+  }
+  if (reduction == loss::kNone) {
+    float* row_weight = reinterpret_cast<float*>(ws + plan.weight);
+    float* alpha = reinterpret_cast<float*>(ws + plan.alpha);
+    if (int st = launch_after(loss::loss_weights_kernel, "loss_weights_kernel", 1, 1024, s, dloss, base.target,
+                              (long long)ignore_index, (int)tokens, base.live, base.order, row_weight, alpha))
+      return st;
+    base.row_weight = row_weight;
+    base.alpha = alpha;
+  } else {
+    base.dloss = dloss;
+    base.count = reduction == loss::kMean ? count : nullptr;
+  }
+  for (int64_t i = 0; i < plan.pieces; ++i) {
+    const int64_t col0 = i * plan.cols, cols = std::min(plan.cols, vocab - col0);
+    const char* w = static_cast<const char*>(weight) + col0 * sw * 2;
+    bool ok = true;
+    loss::Params p = base;
+    p.col0 = (int)col0;
+    const bool pair = on_pairs(tokens);
+    p.tile_n = logit_tile(tokens, cols);
+    loss::Problem& q = p.prob[0];
+    shape(q, tokens, cols, dim, 1, pair, p.tile_n);
+    q.m_live = 1;
+    ok &= load_map(&q.a, x, dtype, dim, tokens, sx, q.a_rows);
+    if (packed_x) ok &= load_map(&q.packed, packed_x, dtype, dim, tokens, packed.stride, q.a_rows);
+    ok &= load_map(&q.b, w, dtype, dim, cols, sw, pair ? loss::TILE / 2 : p.tile_n);
+    ok &= store_map(&q.c_box, g, dtype, cols, tokens, plan.pitch);
+    q.c_tma = pair;  // a single CTA's column halves need not be whole 64-column boxes
+    q.c = g;
+    q.scm = plan.pitch;
+    p.num_tiles = q.tiles;
+    if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
+    if (int st = launch_logits<loss::kGradient>(p, pair, s)) return st;
+
+    p = base;
+    int n = 0;
+    if (dx) {
+      loss::Problem& d = p.prob[n++];
+      shape(d, tokens, dim, cols, plan.splits, true, loss::WIDE);
+      ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, d.a_rows);
+      ok &= load_b(&d.b, d, w, dtype, dim, cols, sw);
+      d.acc = acc;
+      if (plan.splits > 1) d.acc_mode = loss::kAccSlab;
+      else if (plan.pieces > 1) d.acc_mode = i == 0 ? loss::kAccWrite : i + 1 < plan.pieces ? loss::kAccAdd : loss::kAccLast;
+      d.c = dx;
+      d.scm = sdx;
+      d.c_tma = aligned(dx, 16) && sdx % 8 == 0;
+      if (d.c_tma) ok &= store_map(&d.c_box, dx, dtype, dim, tokens, sdx);
+      d.m_live = 1;
+    }
+    if (dw) {
+      loss::Problem& d = p.prob[n++];
+      ok &= slab_map(&d.a, g, dtype, plan.pitch / 64, tokens, plan.pitch);  // rows of dW beyond cols are not stored
+      ok &= load_b(&d.b, d, x, dtype, dim, tokens, sx);
+      if (packed_x) ok &= load_b(&d.packed, d, packed_x, dtype, dim, tokens, packed.stride);
+      shape(d, cols, dim, tokens, 1, true, loss::WIDE);
+      d.k_live = 1;
+      d.a_mn = 1;
+      char* out = static_cast<char*>(dw) + col0 * sdw * 2;
+      d.c = out;
+      d.scm = sdw;
+      d.c_tma = aligned(out, 16) && sdw % 8 == 0;
+      if (d.c_tma) ok &= store_map(&d.c_box, out, dtype, dim, cols, sdw);
+    }
+    if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
+    p.num_tiles = p.prob[0].tiles;
+    if (n > 1) p.num_tiles += p.prob[1].tiles;
+    if (int st = launch_grad_products(p, s)) return st;
+    if (dx && plan.splits > 1) {
+      const loss::Problem& d = p.prob[0];
+      const loss::JoinArgs j{acc, d.n, d.n_blocks, d.splits, p.fmt, static_cast<uint16_t*>(dx), sdx,
+                             d.c_tma};
+      if (int st = launch_after(loss::loss_join_kernel, "loss_join_kernel",
+                                (int64_t)d.m_blocks * d.n_blocks * 4 * loss::kJoinParts, 256, s, j, p))
+        return st;
+    }
+  }
+  return PCB_OK;
 }
 
 }  // namespace
@@ -292,6 +499,11 @@ int pcb_repack_u16(const void* src, int64_t rows, int64_t cols, int64_t src_stri
   return check_launch("repack_rows_kernel");
 }
 
+int64_t pcb_linear_ce_packed_bytes(int64_t tokens, int64_t vocab, int64_t dim) {
+  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  return Order(tokens, vocab, dim).bytes;
+}
+
 int64_t pcb_linear_ce_fwd_workspace_bytes(int64_t tokens, int64_t vocab) {
   if (tokens <= 0 || vocab <= 0) return 0;
   return FwdPlan(tokens, vocab).bytes;
@@ -301,31 +513,17 @@ int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
                       float* loss_out, float* stats, float* count, void* workspace, int64_t workspace_bytes,
                       void* stream) {
-  if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
-  if (tokens == 0) return PCB_OK;
-  if (!target || !loss_out || !stats || !count) return fail(PCB_ERR_INVALID, "null pointer");
-  const FwdPlan plan(tokens, vocab);
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
-    return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
-  if (int st = check_operands(x, sx, weight, sw)) return st;
-  cudaStream_t s = (cudaStream_t)stream;
-  char* ws = static_cast<char*>(workspace);
-  loss::Params p = base_params(dtype, vocab, target, ignore_index);
-  loss::Problem& q = p.prob[0];
-  const bool pair = on_pairs(tokens);
-  p.tile_n = logit_tile(tokens, vocab);
-  shape(q, tokens, vocab, dim, 1, pair, p.tile_n);
-  if (!load_map(&q.a, x, dtype, dim, tokens, sx, q.a_rows) ||
-      !load_map(&q.b, weight, dtype, dim, vocab, sw, pair ? loss::TILE / 2 : p.tile_n))
-    return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-  p.num_tiles = q.tiles;
-  p.partial = reinterpret_cast<float2*>(ws + plan.partial);
-  p.target_logit = reinterpret_cast<float*>(ws + plan.target_logit);
-  p.ticket = reinterpret_cast<unsigned*>(ws + plan.ticket);
-  if (int st = launch_logits<loss::kStats>(p, pair, s)) return st;
-  loss::RowArgs r{p.partial, p.target_logit, p.target, ignore_index, vocab, (int)tokens, 2 * q.n_blocks, reduction,
-                  stats, loss_out, count, reinterpret_cast<double*>(ws + plan.sums), p.ticket};
-  return launch_after(loss::loss_rows_kernel, "loss_rows_kernel", up(tokens, 32), loss::kRowWarps * 32, s, r);
+  return forward(x, sx, weight, sw, dtype, tokens, vocab, dim, target, ignore_index, reduction, loss_out, stats, count,
+                 nullptr, workspace, workspace_bytes, stream);
+}
+
+int pcb_linear_ce_packed_fwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                             int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                             float* loss_out, float* stats, float* count, void* packed, int64_t packed_bytes,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int st = check_packed(dtype, tokens, vocab, dim, reduction, packed, packed_bytes)) return st;
+  return forward(x, sx, weight, sw, dtype, tokens, vocab, dim, target, ignore_index, reduction, loss_out, stats, count,
+                 packed, workspace, workspace_bytes, stream);
 }
 
 int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx,
@@ -338,101 +536,18 @@ int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
                       const float* stats, const float* count, const float* dloss, void* dx, int64_t sdx, void* dw,
                       int64_t sdw, int64_t piece, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (int st = check_shapes(dtype, tokens, vocab, dim, reduction)) return st;
-  cudaStream_t s = (cudaStream_t)stream;
-  if (tokens == 0) {
-    if (dw && cudaMemset2DAsync(dw, (size_t)sdw * 2, 0, (size_t)dim * 2, (size_t)vocab, s) != cudaSuccess)
-      return check_launch("linear cross entropy dw");
-    return PCB_OK;
-  }
-  if (!dx && !dw) return PCB_OK;
-  if (!target || !stats || !count || !dloss) return fail(PCB_ERR_INVALID, "null pointer");
-  const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr, dw != nullptr);
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
-    return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
-  if (int st = check_operands(x, sx, weight, sw)) return st;
-  char* ws = static_cast<char*>(workspace);
-  void* g = ws + plan.g;
-  float4* acc = reinterpret_cast<float4*>(ws + plan.acc);
-  loss::Params base = base_params(dtype, vocab, target, ignore_index);
-  base.stats = stats;
-  if (reduction == loss::kNone) {
-    float* row_weight = reinterpret_cast<float*>(ws + plan.weight);
-    float* alpha = reinterpret_cast<float*>(ws + plan.alpha);
-    if (int st = launch_after(loss::loss_weights_kernel, "loss_weights_kernel", 1, 1024, s, dloss, base.target,
-                              (long long)ignore_index, (int)tokens, row_weight, alpha))
-      return st;
-    base.row_weight = row_weight;
-    base.alpha = alpha;
-  } else {
-    base.dloss = dloss;
-    base.count = reduction == loss::kMean ? count : nullptr;
-  }
-  for (int64_t i = 0; i < plan.pieces; ++i) {
-    const int64_t col0 = i * plan.cols, cols = std::min(plan.cols, vocab - col0);
-    const char* w = static_cast<const char*>(weight) + col0 * sw * 2;
-    bool ok = true;
-    loss::Params p = base;
-    p.col0 = (int)col0;
-    const bool pair = on_pairs(tokens);
-    p.tile_n = logit_tile(tokens, cols);
-    loss::Problem& q = p.prob[0];
-    shape(q, tokens, cols, dim, 1, pair, p.tile_n);
-    ok &= load_map(&q.a, x, dtype, dim, tokens, sx, q.a_rows);
-    ok &= load_map(&q.b, w, dtype, dim, cols, sw, pair ? loss::TILE / 2 : p.tile_n);
-    ok &= store_map(&q.c_box, g, dtype, cols, tokens, plan.pitch);
-    q.c_tma = pair;  // a single CTA's column halves need not be whole 64-column boxes
-    q.c = g;
-    q.scm = plan.pitch;
-    p.num_tiles = q.tiles;
-    if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-    if (int st = launch_logits<loss::kGradient>(p, pair, s)) return st;
+  return backward(x, sx, weight, sw, dtype, tokens, vocab, dim, target, ignore_index, reduction, stats, count, nullptr,
+                  dloss, dx, sdx, dw, sdw, piece, workspace, workspace_bytes, stream);
+}
 
-    p = base;
-    int n = 0;
-    if (dx) {
-      loss::Problem& d = p.prob[n++];
-      shape(d, tokens, dim, cols, plan.splits, true, loss::WIDE);
-      ok &= load_map(&d.a, g, dtype, cols, tokens, plan.pitch, d.a_rows);
-      ok &= load_b(d, w, dtype, dim, cols, sw);
-      d.acc = acc;
-      if (plan.splits > 1) d.acc_mode = loss::kAccSlab;
-      else if (plan.pieces > 1) d.acc_mode = i == 0 ? loss::kAccWrite : i + 1 < plan.pieces ? loss::kAccAdd : loss::kAccLast;
-      d.c = dx;
-      d.scm = sdx;
-      d.c_tma = aligned(dx, 16) && sdx % 8 == 0;
-      if (d.c_tma) ok &= store_map(&d.c_box, dx, dtype, dim, tokens, sdx);
-    }
-    if (dw) {
-      loss::Problem& d = p.prob[n++];
-      ok &= slab_map(&d.a, g, dtype, plan.pitch / 64, tokens, plan.pitch);  // rows of dW beyond cols are not stored
-      ok &= load_b(d, x, dtype, dim, tokens, sx);
-      shape(d, cols, dim, tokens, 1, true, loss::WIDE);
-      d.a_mn = 1;
-      char* out = static_cast<char*>(dw) + col0 * sdw * 2;
-      d.c = out;
-      d.scm = sdw;
-      d.c_tma = aligned(out, 16) && sdw % 8 == 0;
-      if (d.c_tma) ok &= store_map(&d.c_box, out, dtype, dim, cols, sdw);
-    }
-    if (!ok) return fail(PCB_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the operand layout");
-    p.num_tiles = p.prob[0].tiles;
-    if (n > 1) {
-      p.num_tiles += p.prob[1].tiles;
-      p.extra = extra_of(p.prob[0].tiles, p.prob[0].split_stages, p.prob[1].tiles, p.prob[1].k_stages,
-                         device_info().sm_count / 2);
-    }
-    if (int st = launch_grad_products(p, s)) return st;
-    if (dx && plan.splits > 1) {
-      const loss::Problem& d = p.prob[0];
-      const loss::JoinArgs j{acc, d.m, d.n, d.m_blocks, d.n_blocks, d.splits, p.fmt, static_cast<uint16_t*>(dx), sdx,
-                             d.c_tma};
-      if (int st = launch_after(loss::loss_join_kernel, "loss_join_kernel",
-                                (int64_t)d.m_blocks * d.n_blocks * 4 * loss::kJoinParts, 256, s, j, p))
-        return st;
-    }
-  }
-  return PCB_OK;
+int pcb_linear_ce_packed_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
+                             int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
+                             const float* stats, const float* count, const void* packed, int64_t packed_bytes,
+                             const float* dloss, void* dx, int64_t sdx, void* dw, int64_t sdw, int64_t piece,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int st = check_packed(dtype, tokens, vocab, dim, reduction, packed, packed_bytes)) return st;
+  return backward(x, sx, weight, sw, dtype, tokens, vocab, dim, target, ignore_index, reduction, stats, count, packed,
+                  dloss, dx, sdx, dw, sdw, piece, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -101,12 +101,14 @@ enum Site : int { SITE_LOSS_PRODUCER = 16, SITE_LOSS_MMA = 17, SITE_LOSS_EPILOGU
 // One matrix product C [m, n] = A B of a launch.
 struct Problem {
   CUtensorMap a, b, c_box;
+  CUtensorMap packed;  // takes the place of a (logits) or b (dW) where tokens are left out
   int m, n;
   int m_blocks, n_blocks, splits;  // splits: parts of K, each a tile of its own
   int tiles;                       // m_blocks * n_blocks * splits
   int k_stages, split_stages;
   int chunk_stages;  // of the logits: stages between two promotions
   int a_rows;        // rows of A that a load brings (K-major A)
+  int m_live, k_live;  // m or k is the tokens: only those in Live count
   // products of G, where B is N-major:
   int a_mn;     // A is M-major
   int b_slabs;  // B's map takes both 64-column slabs of a 128-column part in one load
@@ -120,9 +122,15 @@ struct Problem {
 struct Params {
   Problem prob[2];
   int num_tiles;
-  int extra;   // tiles of prob[1] that the workers with one tile less of prob[0] take first
   int tile_n;  // tile columns (TILE on a CTA pair)
   int fmt;  // 0 fp16, 1 bf16
+  // Tokens that are left out: `order` puts the others first, `*live` says how
+  // many they are, and target_packed holds the targets in that order (null: every
+  // token is taken, in its own place).
+  int tokens;
+  const int* live;
+  const int* order;
+  const long long* target_packed;
   // rows
   const long long* target;
   long long ignore_index;
@@ -208,8 +216,39 @@ __host__ __device__ __forceinline__ int tile_of(int t0, int total, int extra, in
   const int tile = at + i * workers + (w >= r ? w - r : w - r + workers);
   return tile < total ? tile : -1;
 }
-__device__ __forceinline__ int tile_of(const Params& p, int w, int workers, int i) {
-  return tile_of(p.prob[0].tiles, p.num_tiles, p.extra, w, workers, i);
+// Short tiles that workers with one long tile less take in its place.
+__host__ __device__ __forceinline__ int extra_of(int long_tiles, int long_stages, int short_tiles, int short_stages,
+                                                 int workers) {
+  const int left = long_tiles % workers;
+  if (left == 0 || short_tiles == 0 || long_tiles + short_tiles < workers) return 0;
+  const int most = short_tiles / (workers - left), fit = long_stages / short_stages;
+  return most < fit ? most : fit;
+}
+
+// What a launch has to do once it is known how many tokens count.
+struct Live {
+  int rows;       // those tokens
+  bool dense;     // all of them: nothing is packed
+  int m_blocks;   // of prob[0]
+  int tiles;      // of prob[0]
+  int total, extra;
+  int token_stages;  // of a product over the tokens
+};
+__device__ __forceinline__ Live live_of(const Params& p, int tile_m, int workers) {
+  Live l;
+  const Problem& q = p.prob[0];
+  l.rows = p.live ? *p.live : p.tokens;
+  l.dense = l.rows == p.tokens;
+  const int rows = max(l.rows, 1);  // without any, one row of zeros in G
+  l.m_blocks = q.m_live ? (rows + tile_m - 1) / tile_m : q.m_blocks;
+  l.tiles = l.m_blocks * q.n_blocks * q.splits;
+  l.total = l.tiles + p.num_tiles - q.tiles;
+  l.token_stages = (rows + BK - 1) / BK;
+  l.extra = l.total > l.tiles ? extra_of(l.tiles, q.split_stages, l.total - l.tiles, l.token_stages, workers) : 0;
+  return l;
+}
+__device__ __forceinline__ int tile_of(const Live& l, int w, int workers, int i) {
+  return tile_of(l.tiles, l.total, l.extra, w, workers, i);
 }
 
 struct TileAt {
@@ -217,29 +256,30 @@ struct TileAt {
 };
 // Tiles in groups of kGroupM tile rows, rows fastest: the tiles in flight share
 // few columns of B, and a group's rows of A stay in L2.
-__device__ __forceinline__ TileAt locate(const Params& p, int tile) {
+__device__ __forceinline__ TileAt locate(const Params& p, const Live& l, int tile) {
   TileAt t;
-  t.prob = tile >= p.prob[0].tiles ? 1 : 0;
+  t.prob = tile >= l.tiles ? 1 : 0;
   const Problem& q = p.prob[t.prob];
-  int i = tile - (t.prob ? p.prob[0].tiles : 0);
+  int i = tile - (t.prob ? l.tiles : 0);
   t.index = i;
-  const int area = q.m_blocks * q.n_blocks;
+  const int m_blocks = t.prob ? q.m_blocks : l.m_blocks;
+  const int area = m_blocks * q.n_blocks;
   t.split = i / area;
   i -= t.split * area;
   const int group = i / (kGroupM * q.n_blocks);
-  const int rows = min(kGroupM, q.m_blocks - group * kGroupM);
+  const int rows = min(kGroupM, m_blocks - group * kGroupM);
   i -= group * kGroupM * q.n_blocks;
   t.nb = i / rows;
   t.mb = group * kGroupM + i - t.nb * rows;
   return t;
 }
 
-// 64 columns of a warp's 32 rows: every lane packs its row's 128 bytes into the
-// warp's staging buffer (128-byte swizzle), from where one TMA store takes
-// the box, or, where C's rows do not suit TMA, the warp writes row by row
-// (columns below `limit`).
-__device__ __forceinline__ void store_box(const Problem& q, const uint32_t (&w)[32], uint32_t stg, int lane, int row0,
-                                          int col, int limit) {
+// 64 columns of a warp's 32 rows of the first m: every lane packs its row's 128
+// bytes into the warp's staging buffer (128-byte swizzle), from where one TMA store
+// takes the box.  Where C's rows do not suit TMA, or go to the places in `order`
+// (not null), the warp writes row by row (columns below `limit`).
+__device__ __forceinline__ void store_box(const Problem& q, const int* order, int m, const uint32_t (&w)[32],
+                                          uint32_t stg, int lane, int row0, int col, int limit) {
   if (lane == 0) gemm::bulk_wait_read<0>();
   __syncwarp();
   const uint32_t swz = (uint32_t)(lane & 7);
@@ -250,23 +290,41 @@ __device__ __forceinline__ void store_box(const Problem& q, const uint32_t (&w)[
                  "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
                  : "memory");
   }
-  if (q.c_tma) {
+  if (!order && q.c_tma) {
     gemm::fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0 && row0 < q.m && col < q.n) gemm::tma_store_3d(&q.c_box, stg, col, row0, 0);
+    if (lane == 0 && row0 < m && col < q.n) gemm::tma_store_3d(&q.c_box, stg, col, row0, 0);
     return;
   }
   __syncwarp();
   uint16_t* c = static_cast<uint16_t*>(q.c);
-  const int rows = min(32, q.m - row0);
+  const int rows = min(32, m - row0);
+  const int place = order && lane < rows ? order[row0 + lane] : row0 + lane;  // C's row
+  if (q.c_tma && limit % 8 == 0) {  // 16 bytes a lane, four rows at a time
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3), u = lane & 7;
+      const long long at = __shfl_sync(0xffffffffu, place, r);
+      uint4 v;
+      const uint32_t src = stg + (uint32_t)r * 128u + (((uint32_t)u ^ ((uint32_t)r & 7u)) << 4);
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "r"(src)
+                   : "memory");
+      if (r < rows && col + u * 8 < limit) *reinterpret_cast<uint4*>(c + at * q.scm + col + u * 8) = v;
+    }
+    __syncwarp();
+    return;
+  }
   for (int r = 0; r < rows; ++r) {
+    const long long at = __shfl_sync(0xffffffffu, place, r);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int e = h * 32 + lane;  // column within the box
       uint16_t v;
       const uint32_t src = stg + (uint32_t)r * 128u + ((((uint32_t)e >> 3) ^ ((uint32_t)r & 7u)) << 4) + ((uint32_t)e & 7u) * 2u;
       asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src) : "memory");
-      if (col + e < limit) c[(long long)(row0 + r) * q.scm + col + e] = v;
+      if (col + e < limit) c[at * q.scm + col + e] = v;
     }
   }
   __syncwarp();
@@ -333,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
   // read or written before that kernel has completed.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
+  const Live live = live_of(p, TILE_M, workers);
 
   if (warp < kEpiWarp0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
@@ -342,11 +401,12 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
-          const TileAt t = locate(p, tile);
+        for (int i = 0, tile; ok && (tile = tile_of(live, worker, workers, i)) >= 0; ++i) {
+          const TileAt t = locate(p, live, tile);
           const Problem& q = p.prob[t.prob];
           const int a_row = t.mb * TILE_M + (int)rank * BM;
           const int b_col = PAIR ? t.nb * TILE + (int)rank * (TILE / 2) : t.nb * p.tile_n;
+          const CUtensorMap* a_map = live.dense ? &q.a : &q.packed;
           for (int ks = 0; ks < q.k_stages; ++ks) {
             if (!mbar_spin_bounded(bar_empty + 8 * stage, phase ^ 1, abort_flag, SITE_LOSS_PRODUCER)) {
               ok = false;
@@ -358,10 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
             if (leader) mbar_arrive_expect_tx(fb, (uint32_t)(PAIR ? 2 : 1) * q.a_rows * BK * 2 + b_bytes);
             if constexpr (PAIR) {
               const uint32_t fbl = gemm::mapa_shared(fb, 0);
-              gemm::tma_load_3d_pair(a_dst, &q.a, fbl, ks * BK, a_row, 0);
+              gemm::tma_load_3d_pair(a_dst, a_map, fbl, ks * BK, a_row, 0);
               gemm::tma_load_3d_pair(b_dst, &q.b, fbl, ks * BK, b_col, 0);
             } else {
-              gemm::tma_load_3d(a_dst, &q.a, fb, ks * BK, a_row, 0);
+              gemm::tma_load_3d(a_dst, a_map, fb, ks * BK, a_row, 0);
               gemm::tma_load_3d(b_dst, &q.b, fb, ks * BK, b_col, 0);
             }
             if (++stage == STAGES) {
@@ -386,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
         };
         const uint64_t desc = gemm::make_sw128_desc(s_base, 16u);
         const uint32_t idesc = gemm::make_idesc(p.tile_n, p.fmt, p.fmt, 0, 0, TILE_M);
-        for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
+        for (int i = 0, tile; ok && (tile = tile_of(live, worker, workers, i)) >= 0; ++i) {
           const Problem& q = p.prob[0];
           int ks = 0;
           while (ks < q.k_stages && ok) {
@@ -432,14 +492,14 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
     const uint32_t bar_tempty_l = PAIR ? gemm::mapa_shared(bar_tempty, 0) : bar_tempty;
     uint32_t acc_cnt = 0;
     bool ok = true;
-    for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
-      const TileAt t = locate(p, tile);
+    for (int i = 0, tile; ok && (tile = tile_of(live, worker, workers, i)) >= 0; ++i) {
+      const TileAt t = locate(p, live, tile);
       const Problem& q = p.prob[t.prob];
       const int row0 = t.mb * TILE_M + (int)rank * BM + quarter * 32;  // of the warp
       const int row = row0 + lane;
       const int col0 = t.nb * (PAIR ? TILE : p.tile_n) + half * half_cols;
       const int limit = min(q.n, col0 + half_cols);  // columns of this half
-      const bool in = row < q.m;
+      const bool in = row < live.rows;
       auto wait_full = [&](uint32_t abuf) -> bool {
         if (!mbar_spin_bounded_warp(bar_tfull + 8 * abuf, (acc_cnt / NACC) & 1, abort_flag, SITE_LOSS_EPILOGUE))
           return false;
@@ -462,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
       int target = -1;  // within the piece
       float top = 0.f, shift = 0.f, weight = 0.f;
       if (in) {
-        const long long tv = p.target[row];
+        const long long tv = live.dense ? p.target[row] : p.target_packed[row];
         const bool valid = tv != p.ignore_index;
         if (MODE == kGradient && valid) {
           top = p.stats[row];
@@ -545,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
             w[j] = weight == 0.f
                        ? 0u
                        : pack2(acc[b * 64 + 2 * j] * weight, acc[b * 64 + 2 * j + 1] * weight, p.fmt);
-          if (b * 64 < half_cols) store_box(q, w, stg, lane, row0, col0 + b * 64, limit);
+          if (b * 64 < half_cols) store_box(q, nullptr, q.m, w, stg, lane, row0, col0 + b * 64, limit);
         }
       }
     }
@@ -618,6 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
   const uint32_t tmem_base = *tmem_slot;
   // Nothing global is read or written before the previous kernel has completed.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Live live = live_of(p, TILE, workers);
 
   if (warp < kEpiWarp0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLowRegs));
@@ -627,15 +688,17 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
-          const TileAt t = locate(p, tile);
+        for (int i = 0, tile; ok && (tile = tile_of(live, worker, workers, i)) >= 0; ++i) {
+          const TileAt t = locate(p, live, tile);
           const Problem& q = p.prob[t.prob];
+          const CUtensorMap* b_map = q.k_live && !live.dense ? &q.packed : &q.b;
           const int a_row = t.mb * TILE + (int)rank * BM;
           const int b_col = t.nb * WIDE + (int)rank * (TILE / 2);
           const int halves = t.nb * WIDE + TILE < q.n ? 2 : 1;
           const uint32_t bytes = 2u * ((q.a_mn ? A_BYTES : q.a_rows * BK * 2) + halves * 2 * SLAB);
-          const int ks1 = min(q.k_stages, (t.split + 1) * q.split_stages);
-          for (int ks = t.split * q.split_stages; ks < ks1; ++ks) {
+          const int ks0 = t.split * q.split_stages;
+          const int ks1 = q.k_live ? live.token_stages : min(q.k_stages, ks0 + q.split_stages);
+          for (int ks = ks0; ks < ks1; ++ks) {
             if (!mbar_spin_bounded(bar_empty + 8 * stage, phase ^ 1, abort_flag, SITE_LOSS_PRODUCER)) {
               ok = false;
               break;
@@ -650,10 +713,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
               const uint32_t dst = b_dst + h * 2 * SLAB;
               const int col = b_col + h * TILE;
               if (q.b_slabs) {
-                gemm::tma_load_3d_pair(dst, &q.b, fbl, 0, ks * BK, col / 64);
+                gemm::tma_load_3d_pair(dst, b_map, fbl, 0, ks * BK, col / 64);
               } else {
-                gemm::tma_load_3d_pair(dst, &q.b, fbl, col, ks * BK, 0);
-                gemm::tma_load_3d_pair(dst + SLAB, &q.b, fbl, col + 64, ks * BK, 0);
+                gemm::tma_load_3d_pair(dst, b_map, fbl, col, ks * BK, 0);
+                gemm::tma_load_3d_pair(dst + SLAB, b_map, fbl, col + 64, ks * BK, 0);
               }
             }
             if (++stage == STAGES) {
@@ -675,13 +738,14 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
         return mbar_spin_bounded_warp(bar, parity, abort_flag, SITE_LOSS_MMA);
       };
       const uint64_t k_desc = gemm::make_sw128_desc(s_base, 16u), mn_desc = gemm::make_sw128_desc(s_base, SLAB);
-      for (int i = 0, tile; (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
-        const TileAt t = locate(p, tile);
+      for (int i = 0, tile; (tile = tile_of(live, worker, workers, i)) >= 0; ++i) {
+        const TileAt t = locate(p, live, tile);
         const Problem& q = p.prob[t.prob];
         const uint64_t a_desc = q.a_mn ? mn_desc : k_desc;
         const uint32_t a_step = q.a_mn ? MN_STEP : K_STEP;
         const uint32_t idesc = gemm::make_idesc(TILE, p.fmt, p.fmt, q.a_mn, 1, 2 * BM);
-        const int stages = min(q.k_stages, (t.split + 1) * q.split_stages) - t.split * q.split_stages;
+        const int ks0 = t.split * q.split_stages;
+        const int stages = q.k_live ? live.token_stages : min(q.k_stages, ks0 + q.split_stages) - ks0;
         const bool wide = t.nb * WIDE + TILE < q.n;
         auto issue = [&](int st, int h, bool fresh) {
           const uint32_t a_lo = (uint32_t)a_desc + (uint32_t)(st * A_BYTES >> 4);
@@ -753,13 +817,15 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
     const float alpha = alpha_of(p);
     uint32_t used[2] = {0, 0};
     bool ok = true;
-    for (int i = 0, tile; ok && (tile = tile_of(p, worker, workers, i)) >= 0; ++i) {
-      const TileAt t = locate(p, tile);
+    for (int i = 0, tile; ok && (tile = tile_of(live, worker, workers, i)) >= 0; ++i) {
+      const TileAt t = locate(p, live, tile);
       const Problem& q = p.prob[t.prob];
       const int row0 = t.mb * TILE + (int)rank * BM + quarter * 32;  // of the warp
       const int halves = t.nb * WIDE + TILE < q.n ? 2 : 1;
       const bool add = q.acc_mode == kAccAdd || q.acc_mode == kAccLast;
       const bool stored = q.acc_mode == kAccNone || q.acc_mode == kAccLast;
+      const int m = q.m_live ? live.rows : q.m;
+      const int* order = q.m_live && !live.dense ? p.order : nullptr;
       for (int h = 0; h < halves; ++h) {
         const int col0 = t.nb * WIDE + h * TILE + part * EPI_COLS;
         if (!mbar_spin_bounded_warp(bar_tfull + 8 * h, used[h] & 1, abort_flag, SITE_LOSS_EPILOGUE)) {
@@ -782,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
         float4* acc = nullptr;
         if (q.acc_mode != kAccNone)
           acc = q.acc + (((long long)t.index * 2 + rank) * 2 + h) * kAccVec * 256 + ew * 32 + lane;
-        const bool in = row0 + lane < q.m;
+        const bool in = row0 + lane < m;
         if (add && in) {
 #pragma unroll
           for (int c = 0; c < EPI_COLS / 32; ++c)
@@ -803,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
             for (int j = 0; j < 32; ++j)
               w[j] = pack2(__uint_as_float(v[2 * b + j / 16][2 * j % 32]) * alpha,
                            __uint_as_float(v[2 * b + j / 16][2 * j % 32 + 1]) * alpha, p.fmt);
-            store_box(q, w, stg, lane, row0, col0 + b * 64, q.n);
+            store_box(q, order, m, w, stg, lane, row0, col0 + b * 64, q.n);
           }
         } else if (in) {
 #pragma unroll
@@ -835,6 +901,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
 enum Reduction : int { kNone = 0, kSum = 1, kMean = 2 };
 
 struct RowArgs {
+  const int* live;  // tokens that count, and the order that puts them first; null: every token in its place
+  const int* order;
   const float2* partial;
   const float* target_logit;
   const long long* target;
@@ -855,8 +923,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
+  const int live = p.live ? *p.live : p.tokens;
   float m = -INFINITY, s = 0.f;
-  if (row < p.tokens) {
+  if (row < live) {
     for (int i = warp; i < p.parts; i += kRowWarps * kRowLoads) {
       float2 o[kRowLoads];
 #pragma unroll
@@ -889,7 +958,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
     const float log_sum = logf(sum);
     p.stats[row] = base;
     p.stats[p.tokens + row] = log2f(sum);
-    const long long t = p.target[row];
+    const int at = live < p.tokens ? p.order[row] : row;  // the token's own place
+    const long long t = p.target[at];
     float v = 0.f;
     if (t != p.ignore_index) {
       valid = 1.0;
@@ -901,7 +971,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
       }
       nll = (double)v;
     }
-    if (p.reduction == kNone) p.loss[row] = v;
+    if (p.reduction == kNone) p.loss[at] = v;
   }
   if (p.reduction == kNone) return;
   if (warp == 0) {
@@ -940,12 +1010,96 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
   }
 }
 
+// Tokens that are left out cost nothing where there are many: the others are
+// packed in front, in their order, and only they are multiplied.  order[i] is the
+// token in place i, those left out behind the others; *live how many others there
+// are.  One CTA: a count and a position for 1024 tokens at a time.
+__global__ void __launch_bounds__(1024) loss_order_kernel(const long long* target, long long ignore_index, int tokens,
+                                                          int* order, int* live) {
+  __shared__ int sums[33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // First the number of tokens that count, then the places.
+  int mine = 0;
+  for (int i = threadIdx.x; i < tokens; i += 1024) mine += target[i] != ignore_index;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) sums[warp] = mine;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) total += sums[i];
+  if (threadIdx.x == 0) *live = total;
+  int taken = 0, left_out = total;  // next place of either kind
+  for (int i0 = 0; i0 < tokens; i0 += 1024) {
+    const int i = i0 + threadIdx.x;
+    const bool takes = i < tokens && target[i] != ignore_index;
+    const unsigned votes = __ballot_sync(0xffffffffu, takes);
+    __syncthreads();
+    if (lane == 0) sums[warp] = __popc(votes);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      before += w < warp ? sums[w] : 0;
+      all += sums[w];
+    }
+    before += __popc(votes & ((1u << lane) - 1u));
+    if (takes) order[taken + before] = i;
+    else if (i < tokens) order[left_out + (int)threadIdx.x - before] = i;
+    taken += all;
+    left_out += min(1024, tokens - i0) - all;
+  }
+}
+
+// The rows of x and the targets in that order; zeros for the rows that a
+// tile or a stage reads beyond them.  Nothing where every token counts.
+__global__ void __launch_bounds__(256) loss_pack_kernel(const uint16_t* x, long long sx, const long long* target,
+                                                        const int* order, const int* live, int tokens, int dim,
+                                                        uint16_t* packed, long long stride, long long* target_packed) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int rows = *live;
+  if (rows == tokens) return;
+  const int end = min(tokens, (max(rows, 1) + TILE - 1) / TILE * TILE), units = (int)(stride / 8);
+  for (int row = blockIdx.x; row < tokens; row += gridDim.x) {
+    const int at = order[row];
+    if (threadIdx.x == 0) target_packed[row] = target[at];
+    if (row >= end) continue;
+    const uint4* src = reinterpret_cast<const uint4*>(x + (long long)at * sx);
+    uint4* dst = reinterpret_cast<uint4*>(packed + row * stride);
+    for (int u = threadIdx.x; u < units; u += 256) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < rows && u * 8 + 8 <= dim) {
+        v = src[u];
+      } else if (row < rows && u * 8 < dim) {  // the row's last elements
+        alignas(16) uint16_t e[8] = {};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (u * 8 + k < dim) e[k] = x[(long long)at * sx + u * 8 + k];
+        v = *reinterpret_cast<const uint4*>(e);
+      }
+      dst[u] = v;
+    }
+  }
+}
+
+// Zeros for the rows of dX of tokens that are left out.
+__global__ void __launch_bounds__(256) loss_zero_rows_kernel(const int* order, const int* live, int tokens, int dim,
+                                                             uint16_t* dx, long long sdx, int vec) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int row = *live + blockIdx.x; row < tokens; row += gridDim.x) {
+    uint16_t* dst = dx + (long long)order[row] * sdx;
+    const int units = vec ? dim / 8 : 0;
+    for (int u = threadIdx.x; u < units; u += 256) reinterpret_cast<uint4*>(dst)[u] = make_uint4(0, 0, 0, 0);
+    for (int c = units * 8 + threadIdx.x; c < dim; c += 256) dst[c] = 0;
+  }
+}
+
 // Losses that are not reduced: their gradients g_i as weights w_i = g_i / A of
 // at most 1 in magnitude and the factor A (a power of two), so that G is
 // rounded at the same place whatever the scale.  One CTA.
 __global__ void __launch_bounds__(1024) loss_weights_kernel(const float* dloss, const long long* target,
-                                                            long long ignore_index, int tokens, float* weight,
-                                                            float* alpha) {
+                                                            long long ignore_index, int tokens, const int* live,
+                                                            const int* order, float* weight, float* alpha) {
   __shared__ uint32_t top[32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   uint32_t m = 0;
@@ -961,7 +1115,8 @@ __global__ void __launch_bounds__(1024) loss_weights_kernel(const float* dloss, 
   const bool usable = e >= 2 && e < 253;
   const float up = usable ? __uint_as_float((uint32_t)(e + 1) << 23) : 1.f;     // 2^(e + 1) > max
   const float down = usable ? __uint_as_float((uint32_t)(253 - e) << 23) : 1.f; // 1 / up
-  for (int i = threadIdx.x; i < tokens; i += 1024) weight[i] = dloss[i] * down;
+  const bool packed = live && *live < tokens;
+  for (int i = threadIdx.x; i < tokens; i += 1024) weight[i] = dloss[packed ? order[i] : i] * down;
   if (threadIdx.x == 0) *alpha = up * (1.f / kGradScale);
 }
 
@@ -1004,7 +1159,7 @@ __global__ void __launch_bounds__(256) repack_rows_kernel(const uint16_t* src, l
 // A thread has 32 columns of a row, 64 bytes of what it writes.
 struct JoinArgs {
   const float4* acc;
-  int m, n, m_blocks, n_blocks, splits, fmt;
+  int n, n_blocks, splits, fmt;
   uint16_t* out;
   long long stride;
   int vec;  // rows of out start on 16 bytes
@@ -1014,18 +1169,20 @@ constexpr int kJoinParts = kAccVec / kJoinVecs;    // of an epilogue thread's sh
 __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs p, const __grid_constant__ Params pp) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float alpha = alpha_of(pp);
+  const Live live = live_of(pp, TILE, 1);
   // blockIdx.x: (tile of the first part, CTA of the pair, half, 32 of a thread's 128 columns)
   const int g = blockIdx.x % kJoinParts, h = blockIdx.x / kJoinParts % 2, rank = blockIdx.x / kJoinParts / 2 % 2;
   const int index = blockIdx.x / kJoinParts / 4;
   const int ew = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TileAt t = locate(pp, index);
+  if (index >= live.m_blocks * p.n_blocks) return;
+  const TileAt t = locate(pp, live, index);
   const int row = t.mb * TILE + rank * BM + (ew & 3) * 32 + lane;
   const int col = t.nb * WIDE + h * TILE + (ew >> 2) * EPI_COLS + g * kJoinVecs * 4;
-  if (row >= p.m || col >= p.n) return;
+  if (row >= live.rows || col >= p.n) return;
   float4 v[kJoinVecs];
 #pragma unroll
   for (int j = 0; j < kJoinVecs; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const long long part = (long long)p.m_blocks * p.n_blocks * 4 * kAccVec * 256;
+  const long long part = (long long)live.m_blocks * p.n_blocks * 4 * kAccVec * 256;
   const float4* a = p.acc + ((((long long)index * 2 + rank) * 2 + h) * kAccVec + g * kJoinVecs) * 256 + threadIdx.x;
   for (int s = 0; s < p.splits; ++s, a += part) {
 #pragma unroll
@@ -1034,7 +1191,7 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const JoinArgs p, const 
       v[j].x += o.x, v[j].y += o.y, v[j].z += o.z, v[j].w += o.w;
     }
   }
-  uint16_t* out = p.out + (long long)row * p.stride + col;
+  uint16_t* out = p.out + (long long)(live.dense ? row : pp.order[row]) * p.stride + col;
 #pragma unroll
   for (int j = 0; j < kJoinVecs; j += 2) {
     const float4 x = v[j], y = v[j + 1];

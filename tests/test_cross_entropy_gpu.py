@@ -345,3 +345,114 @@ def test_entry_points_reject_bad_arguments_without_gpu():
     need = lib.pcb_linear_ce_bwd_workspace_bytes(4096, 32000, 4096, 0, 1, 1)
     # one piece of G (at most 128 MiB) and dX's accumulators, not the logits of the whole vocabulary
     assert need < (128 << 20) + 4096 * 4096 * 4 + (1 << 20)
+
+
+def test_packed_state_is_checked_without_gpu():
+    lib = _lib.lib()
+    assert lib.pcb_linear_ce_packed_bytes(0, 32000, 4096) == 0
+    assert lib.pcb_linear_ce_packed_bytes(511, 1 << 20, 4096) == 0  # too few tokens
+    assert lib.pcb_linear_ce_packed_bytes(4096, 1000, 1024) == 0  # too small a product
+    need = lib.pcb_linear_ce_packed_bytes(4096, 32000, 4096)
+    assert 4096 * (4096 * 2 + 12) <= need <= 4096 * (4096 * 2 + 12) + 4 * 256
+
+    def forward(tokens, packed, nbytes):
+        return lib.pcb_linear_ce_packed_fwd(256, 4096, 256, 4096, 2, tokens, 32000, 4096, 256, IGNORE, 2, 256, 256, 256,
+                                            packed, nbytes, 256, 1 << 40, None)
+
+    def backward(tokens, packed, nbytes):
+        return lib.pcb_linear_ce_packed_bwd(256, 4096, 256, 4096, 2, tokens, 32000, 4096, 256, IGNORE, 2, 256, 256,
+                                            packed, nbytes, 256, 256, 4096, None, 4096, 0, 256, 1 << 40, None)
+
+    for call in (forward, backward):
+        assert call(4096, None, need) == _lib.PCB_ERR_INVALID
+        assert call(4096, 128, need) == _lib.PCB_ERR_INVALID
+        assert call(4096, 256, need - 1) == _lib.PCB_ERR_INVALID
+        assert call(8, 256, need) == _lib.PCB_ERR_INVALID  # state that nothing would write
+        assert call(0, None, 0) == _lib.PCB_OK
+
+
+def _mask(name, tokens):
+    """Tokens that are left out."""
+    out = torch.zeros(tokens, dtype=torch.bool)
+    if name == "first":
+        out[0] = True
+    elif name == "last":
+        out[-1] = True
+    elif name == "scattered":
+        out = torch.rand(tokens, generator=torch.Generator().manual_seed(17)) < 0.4
+    elif name == "one tile left":
+        out[256:] = True
+    elif name == "one more than a tile left":
+        out[:tokens - 257] = True
+    elif name == "one left":
+        out[:] = True
+        out[tokens // 2] = False
+    elif name == "all":
+        out[:] = True
+    return out.cuda()
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,dim", [(515, 33001, 4104), (2100, 8200, 4032)])
+@pytest.mark.parametrize("mask", ["none", "first", "last", "scattered", "one tile left", "one more than a tile left",
+                                  "one left"])
+def test_tokens_left_out_of_large_products(tokens, vocab, dim, mask):
+    x, w, target = _inputs(tokens, vocab, dim, BF16, seed=tokens)
+    left_out = _mask(mask, tokens)
+    target[left_out] = IGNORE
+    assert _lib.lib().pcb_linear_ce_packed_bytes(tokens, vocab, dim) > 0
+    for reduction, piece in (("mean", None), ("none", None), ("sum", 2048)):
+        loss, dx, dw = _check(x, w, target, reduction, piece=piece, what=reduction)
+        assert int(dx[left_out].count_nonzero()) == 0
+        if reduction == "none":
+            assert int(loss[left_out].count_nonzero()) == 0
+    score = linear_cross_entropy(x, w, target, reduction="none")
+    assert torch.equal(score, linear_cross_entropy(x.requires_grad_(), w, target, reduction="none").detach())
+
+
+@gpu
+def test_large_product_of_no_token():
+    x, w, target = _inputs(600, 30000, 4096, F16, seed=6)
+    target.fill_(IGNORE)
+    assert _lib.lib().pcb_linear_ce_packed_bytes(600, 30000, 4096) > 0
+    x.requires_grad_(), w.requires_grad_()
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(x, w, target, reduction=reduction)
+        assert bool(torch.isnan(loss)) if reduction == "mean" else int(loss.count_nonzero()) == 0
+        dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+        assert int(dx.count_nonzero()) == 0 and int(dw.count_nonzero()) == 0
+
+
+@gpu
+def test_gradients_of_large_products_on_rows_of_other_strides():
+    """dX whose rows do not suit TMA (a C caller's), one gradient at a time, an output of odd stride."""
+    tokens, vocab, dim = 700, 24001, 4104
+    x, w, target = _inputs(tokens, vocab, dim, BF16, seed=3, ignored=0.5)
+    _, dx, dw = _check(x, w, target, "mean")
+    x1, w1 = x.detach().requires_grad_(), w.detach().requires_grad_()
+    only_x, = torch.autograd.grad(linear_cross_entropy(x1, w, target), x1)
+    only_w, = torch.autograd.grad(linear_cross_entropy(x, w1, target), w1)
+    (_, _), (ex, ox), (ew, ow) = _reference(x, w, target, "mean", torch.tensor(1.0, device="cuda"))
+    _within(only_x, ex, ox, "dx alone")
+    _within(only_w, ew, ow, "dw alone")
+    lib, code = _lib.lib(), _lib.PCB_DTYPE[BF16]
+    stream = torch.cuda.current_stream().cuda_stream
+    packed = torch.empty(lib.pcb_linear_ce_packed_bytes(tokens, vocab, dim), dtype=torch.uint8, device="cuda")
+    stats, count = torch.empty(2 * tokens, device="cuda"), torch.empty(1, device="cuda")
+    loss, one = torch.empty((), device="cuda"), torch.ones((), device="cuda")
+    ws = torch.empty(lib.pcb_linear_ce_fwd_workspace_bytes(tokens, vocab), dtype=torch.uint8, device="cuda")
+    args = (x.data_ptr(), dim, w.data_ptr(), dim, code, tokens, vocab, dim, target.data_ptr(), IGNORE, 2)
+    forward = lambda nbytes: lib.pcb_linear_ce_packed_fwd(
+        *args, loss.data_ptr(), stats.data_ptr(), count.data_ptr(), packed.data_ptr(), nbytes, ws.data_ptr(),
+        ws.numel(), stream)
+    assert forward(packed.numel() - 1) != 0  # refused before anything runs
+    assert forward(packed.numel()) == 0
+    for piece in (0, 4096):
+        out = torch.full((tokens, dim + 1), 7.0, dtype=BF16, device="cuda")
+        ws2 = torch.empty(lib.pcb_linear_ce_bwd_workspace_bytes(tokens, vocab, dim, piece, 1, 0), dtype=torch.uint8,
+                          device="cuda")
+        assert lib.pcb_linear_ce_packed_bwd(
+            *args, stats.data_ptr(), count.data_ptr(), packed.data_ptr(), packed.numel(), one.data_ptr(),
+            out.data_ptr(), dim + 1, None, dim, piece, ws2.data_ptr(), ws2.numel(), stream) == 0
+        _within(out[:, :dim], ex, ox, f"dx of stride {dim + 1}, piece {piece}")
+        assert bool((out[:, dim] == 7.0).all())
