@@ -407,7 +407,9 @@ int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t
  * x's type.  dloss: [tokens] or [1], as loss.  The vocabulary is taken in
  * pieces of `piece` columns (rounded down to a multiple of 256; <= 0: as many
  * as keep G at 128 MiB, at least 2048), of which only one piece of G exists at
- * a time.  Sums are taken in a fixed order.
+ * a time.  Sums are taken in a fixed order.  What x holds for tokens that are
+ * left out reaches nothing; where pcb_linear_ce_packed_bytes is not 0 it must be
+ * finite for that, or the packed passes be used.
  */
 int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,

@@ -156,6 +156,7 @@ def linear_cross_entropy(
     that exist at a time in the backward pass (rounded down to a multiple of
     256, at least 256; default: as many as fit 128 MiB, at least 2048).
 
+    What ``x`` holds for tokens that are left out (NaN, say) reaches nothing.
     Tokens left out of large products (512 tokens or more, ``tokens * vocab * dim``
     of 2^36 or more) take no part in them: the others are packed, which keeps a
     copy of ``x`` until the backward pass.

@@ -263,7 +263,7 @@ int split_of(int64_t tokens, int64_t vocab, int64_t dim, bool want_dw) {
 struct BwdPlan {
   int64_t cols, pieces, pitch;  // of G
   int splits;                   // parts of K of dX
-  int64_t g, acc, weight, alpha, bytes;
+  int64_t g, acc, weight, alpha, x, pitch_x, bytes;
   BwdPlan(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, bool want_dx, bool want_dw) {
     // G of one piece takes 128 MiB at most (and is no narrower than 2048
     // columns): pieces of even width, whole tiles each.
@@ -280,6 +280,8 @@ struct BwdPlan {
     acc = c.take(want_dx && (pieces > 1 || splits > 1) ? dx_tiles * splits * loss::TILE * loss::WIDE * 4 : 0);
     weight = c.take(tokens * 4);
     alpha = c.take(4);
+    pitch_x = up(dim, 64) * 64;
+    x = c.take(want_dw && !packs(tokens, vocab, dim) ? tokens * pitch_x * 2 : 0);
     bytes = c.at;
   }
 };
@@ -404,6 +406,14 @@ int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtyp
     base.dloss = dloss;
     base.count = reduction == loss::kMean ? count : nullptr;
   }
+  const bool copies = dw && !packs(tokens, vocab, dim);
+  if (copies)
+    if (int st = launch_after(loss::loss_kept_rows_kernel, "loss_kept_rows_kernel",
+                              std::min<int64_t>(tokens, (int64_t)device_info().sm_count * 8), 256, s,
+                              static_cast<const uint16_t*>(x), (long long)sx, base.target, (long long)ignore_index,
+                              count, (int)tokens, (int)dim, reinterpret_cast<uint16_t*>(ws + plan.x),
+                              (long long)plan.pitch_x))
+      return st;
   for (int64_t i = 0; i < plan.pieces; ++i) {
     const int64_t col0 = i * plan.cols, cols = std::min(plan.cols, vocab - col0);
     const char* w = static_cast<const char*>(weight) + col0 * sw * 2;
@@ -447,6 +457,10 @@ int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtyp
       ok &= slab_map(&d.a, g, dtype, plan.pitch / 64, tokens, plan.pitch);  // rows of dW beyond cols are not stored
       ok &= load_b(&d.b, d, x, dtype, dim, tokens, sx);
       if (packed_x) ok &= load_b(&d.packed, d, packed_x, dtype, dim, tokens, packed.stride);
+      if (copies) {
+        ok &= load_b(&d.packed, d, ws + plan.x, dtype, dim, tokens, plan.pitch_x);
+        p.kept = count;
+      }
       shape(d, cols, dim, tokens, 1, true, loss::WIDE);
       d.k_live = 1;
       d.a_mn = 1;

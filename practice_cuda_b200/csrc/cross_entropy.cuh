@@ -131,6 +131,9 @@ struct Params {
   const int* live;
   const int* order;
   const long long* target_packed;
+  // Where nothing is packed: how many tokens count, if dW's product reads a copy
+  // of X without the others' rows (null: X as it is).
+  const float* kept;
   // rows
   const long long* target;
   long long ignore_index;
@@ -225,10 +228,16 @@ __host__ __device__ __forceinline__ int extra_of(int long_tiles, int long_stages
   return most < fit ? most : fit;
 }
 
+// Whether all tokens count, of which *kept do (beyond 2^24 a float cannot say).
+__device__ __forceinline__ bool all_kept(const float* kept, int tokens) {
+  return tokens < (1 << 24) && *kept == (float)tokens;
+}
+
 // What a launch has to do once it is known how many tokens count.
 struct Live {
   int rows;       // those tokens
   bool dense;     // all of them: nothing is packed
+  bool copied;    // dW reads the copy of X
   int m_blocks;   // of prob[0]
   int tiles;      // of prob[0]
   int total, extra;
@@ -239,6 +248,7 @@ __device__ __forceinline__ Live live_of(const Params& p, int tile_m, int workers
   const Problem& q = p.prob[0];
   l.rows = p.live ? *p.live : p.tokens;
   l.dense = l.rows == p.tokens;
+  l.copied = !l.dense || (p.kept && !all_kept(p.kept, p.tokens));
   const int rows = max(l.rows, 1);  // without any, one row of zeros in G
   l.m_blocks = q.m_live ? (rows + tile_m - 1) / tile_m : q.m_blocks;
   l.tiles = l.m_blocks * q.n_blocks * q.splits;
@@ -691,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_products_kernel(const __grid
         for (int i = 0, tile; ok && (tile = tile_of(live, worker, workers, i)) >= 0; ++i) {
           const TileAt t = locate(p, live, tile);
           const Problem& q = p.prob[t.prob];
-          const CUtensorMap* b_map = q.k_live && !live.dense ? &q.packed : &q.b;
+          const CUtensorMap* b_map = q.k_live && live.copied ? &q.packed : &q.b;
           const int a_row = t.mb * TILE + (int)rank * BM;
           const int b_col = t.nb * WIDE + (int)rank * (TILE / 2);
           const int halves = t.nb * WIDE + TILE < q.n ? 2 : 1;
@@ -973,7 +983,6 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
     }
     if (p.reduction == kNone) p.loss[at] = v;
   }
-  if (p.reduction == kNone) return;
   if (warp == 0) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -1006,7 +1015,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
   if (threadIdx.x == 0) {
     for (int i = 1; i < kRowWarps; ++i) a += total[0][i], b += total[1][i];
     p.count[0] = (float)b;
-    p.loss[0] = (float)(p.reduction == kMean ? a / b : a);  // 0 / 0 where every token is left out
+    if (p.reduction != kNone) p.loss[0] = (float)(p.reduction == kMean ? a / b : a);  // 0 / 0: every token is left out
   }
 }
 
@@ -1051,6 +1060,22 @@ __global__ void __launch_bounds__(1024) loss_order_kernel(const long long* targe
   }
 }
 
+__device__ __forceinline__ void copy_row(const uint16_t* src, uint16_t* dst, int units, int dim, bool zero) {
+  for (int u = threadIdx.x; u < units; u += 256) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (!zero && u * 8 + 8 <= dim) {
+      v = reinterpret_cast<const uint4*>(src)[u];
+    } else if (!zero && u * 8 < dim) {  // the row's last elements
+      alignas(16) uint16_t e[8] = {};
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (u * 8 + k < dim) e[k] = src[u * 8 + k];
+      v = *reinterpret_cast<const uint4*>(e);
+    }
+    reinterpret_cast<uint4*>(dst)[u] = v;
+  }
+}
+
 // The rows of x and the targets in that order; zeros for the rows that a
 // tile or a stage reads beyond them.  Nothing where every token counts.
 __global__ void __launch_bounds__(256) loss_pack_kernel(const uint16_t* x, long long sx, const long long* target,
@@ -1064,22 +1089,20 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const uint16_t* x, long 
     const int at = order[row];
     if (threadIdx.x == 0) target_packed[row] = target[at];
     if (row >= end) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(x + (long long)at * sx);
-    uint4* dst = reinterpret_cast<uint4*>(packed + row * stride);
-    for (int u = threadIdx.x; u < units; u += 256) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < rows && u * 8 + 8 <= dim) {
-        v = src[u];
-      } else if (row < rows && u * 8 < dim) {  // the row's last elements
-        alignas(16) uint16_t e[8] = {};
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (u * 8 + k < dim) e[k] = x[(long long)at * sx + u * 8 + k];
-        v = *reinterpret_cast<const uint4*>(e);
-      }
-      dst[u] = v;
-    }
+    copy_row(x + (long long)at * sx, packed + row * stride, units, dim, row >= rows);
   }
+}
+
+// Where nothing is packed, the X of dW's product, with zeros for the tokens
+// that are left out: their rows of G are zeros, but what they hold may be NaN or
+// infinite.  Nothing where every token counts.
+__global__ void __launch_bounds__(256) loss_kept_rows_kernel(const uint16_t* x, long long sx, const long long* target,
+                                                             long long ignore_index, const float* kept, int tokens,
+                                                             int dim, uint16_t* out, long long stride) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (all_kept(kept, tokens)) return;
+  for (int row = blockIdx.x; row < tokens; row += gridDim.x)
+    copy_row(x + (long long)row * sx, out + row * stride, (int)(stride / 8), dim, target[row] == ignore_index);
 }
 
 // Zeros for the rows of dX of tokens that are left out.

@@ -456,3 +456,28 @@ def test_gradients_of_large_products_on_rows_of_other_strides():
             out.data_ptr(), dim + 1, None, dim, piece, ws2.data_ptr(), ws2.numel(), stream) == 0
         _within(out[:, :dim], ex, ox, f"dx of stride {dim + 1}, piece {piece}")
         assert bool((out[:, dim] == 7.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,dim", [(2, 40, 16), (9, 300, 72), (100, 517, 77), (300, 900, 192),
+                                              (600, 300, 64), (515, 33001, 4104), (900, 700, 260)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_non_finite_rows_left_out_reach_nothing(tokens, vocab, dim, reduction, value):
+    x, w, target = _inputs(tokens, vocab, dim, BF16, seed=dim, ignored=0.5)
+    target[tokens // 2] = IGNORE
+    target[0] = 1
+    left_out = target == IGNORE
+    x[left_out] = 0.0
+    expected = _check(x, w, target, reduction, what="zeros")
+    x[left_out] = value
+    dloss = torch.rand(target.shape, generator=torch.Generator().manual_seed(1)).cuda() + 0.5
+    dloss = dloss if reduction == "none" else torch.tensor(1.0, device="cuda")
+    x1, w1 = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = linear_cross_entropy(x1, w1, target, reduction=reduction)
+    got = (loss.detach(), *torch.autograd.grad(loss, (x1, w1), dloss))
+    for a, b, name in zip(got, expected, ("loss", "dx", "dw")):
+        assert torch.equal(a, b), name
+    loss = linear_cross_entropy(x, w1, target, reduction=reduction)
+    assert torch.equal(torch.autograd.grad(loss, w1, dloss)[0], expected[2])
+    assert _lib.device_error()[0] == 0
