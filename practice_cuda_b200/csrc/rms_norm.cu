@@ -87,6 +87,17 @@ int launch_norm_bwd(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
   return check_launch("rms_norm_bwd_kernel");
 }
 
+// 16-bit rows of at most 512 NV units.
+template <int XT, int NV>
+int launch_norm_bwd_staged(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
+  auto kernel = norm::rms_norm_bwd_staged_kernel<XT, NV>;
+  const int smem = p.dim / norm::kUnit * norm::kStagedBytes;
+  ensure_smem_attr(kernel, smem);
+  parts = norm_bwd_ctas(p.rows, 1, 1);
+  kernel<<<parts, norm::kStagedThreads, smem, s>>>(p);
+  return check_launch("rms_norm_bwd_staged_kernel");
+}
+
 // False: the rows are too wide for these kernels.  Eight columns a thread keep
 // clear of register spills, sixteen take the widths beyond.
 template <int XT, int WT>
@@ -118,8 +129,13 @@ int dispatch_norm_bwd(const norm::BwdArgs& p, bool vec, int& parts, cudaStream_t
     if (units <= 128) return launch_norm_bwd<XT, 128 / NV, NV>(p, parts, s);
     if (units <= 256) return launch_norm_bwd<XT, 256 / NV, NV>(p, parts, s);
     if (units <= 512) return launch_norm_bwd<XT, 512 / NV, NV>(p, parts, s);
-    if (units <= 1024) return launch_norm_bwd<XT, 1024 / NV, NV>(p, parts, s);
-    return launch_norm_bwd<XT, 1024, 2>(p, parts, s);
+    if constexpr (XT == PCB_DTYPE_F32) {
+      if (units <= 1024) return launch_norm_bwd<XT, 1024, 1>(p, parts, s);
+      return launch_norm_bwd<XT, 1024, 2>(p, parts, s);
+    } else {
+      if (units <= 1024) return launch_norm_bwd<XT, 512, 2>(p, parts, s);
+      return launch_norm_bwd_staged<XT, 4>(p, parts, s);
+    }
   }
   const bool same = p.w_dtype == XT, f32 = p.w_dtype == PCB_DTYPE_F32;
   if ((same && launch_norm_bwd_elems<XT, XT>(p, parts, s)) ||

@@ -221,6 +221,24 @@ def test_backward_many_rows(rows, dim):
 
 
 @gpu
+@pytest.mark.parametrize("rows,dim", [(700, 8200), (450, 10240), (297, 16384), (149, 12296), (300, 8192), (300, 16392)])
+@pytest.mark.parametrize("dtype,wdtype", [(BF16, BF16), (F16, F32), (F32, F32)])
+def test_backward_many_wide_rows(rows, dim, dtype, wdtype):
+    h, dh, w = _inputs(rows, dim, dtype, seed=rows + dim)
+    w = w.to(wdtype)
+    wide = synthetic((rows, dim + 24), std=0.1, seed=8, dtype=dtype).cuda()
+    dy = wide[:, 8 : 8 + dim]  # rows of another stride
+    rstd = (h.float().square().mean(1) + EPS).rsqrt()
+    for extra in (dh, None):
+        dx, dw = rms_norm_backward(dy, h, w, rstd, dresidual=extra)
+        dx64, dw64, dx_terms, dw_terms = _backward_reference(dy, h, w, rstd, extra)
+        _close(dx, dx64, UNIT[dtype] * (1 + 1e-3), TINY[dtype] + RTOL32 * dx_terms, "dx")
+        _close(dw, dw64, UNIT[wdtype] * (1 + 1e-3), TINY[wdtype] + RTOL32 * dw_terms, "dw")
+        again = rms_norm_backward(dy, h, w, rstd, dresidual=extra)
+        assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+
+
+@gpu
 def test_backward_strides_and_alignment():
     dim = 256
     base = synthetic((5, 3 * dim + 7), seed=21, dtype=F32).cuda()
