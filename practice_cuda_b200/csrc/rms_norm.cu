@@ -27,16 +27,32 @@ int threads_of(int items, int per_thread, int step) {
   return (t + step - 1) / step * step;
 }
 
-// False: the rows are too wide for these kernels.
+// False: the generic kernel takes the rows.  Columns that a thread has beyond the
+// width cost as much as the others, so a CTA has eight a thread up to 8192 columns
+// (16384 x 1021 bf16 with a residual and y on a B200: 68 us, 115 with sixteen; 16384 x
+// 3001: 193 and 250 us; 8192 x 8191: 330 and 369 us), but for 16-bit rows of 4097
+// to 6144, whose eight columns leave an SM one CTA where sixteen leave it two
+// (12000 x 5001: 344 and 293 us; in fp32, with more registers, 342 and 444 us).
+// Without a residual, whose sum it would read back, the generic kernel is faster
+// beyond 2048 columns (16384 x 4095: 149 us, 211 with eight columns a thread; 16384
+// x 1901: 96 us with eight).
 template <int XT, int YT, int WT>
 bool launch_norm_fwd_elems(const norm::FwdArgs& p, cudaStream_t s) {
-  const int threads = threads_of(p.dim, norm::kElems, 128);
-  if (p.dim <= 32 * norm::kElems)
-    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, true, 256><<<(unsigned)((p.rows + 7) / 8), 256, 0, s>>>(p);
+  constexpr int NE = norm::kElems;
+  const int threads = threads_of(p.dim, 8, 128), wide = threads_of(p.dim, NE, 128);
+  if (p.dim <= 32 * NE)
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, true, NE, 256><<<(unsigned)((p.rows + 7) / 8), 256, 0, s>>>(p);
+  else if (!p.res && p.dim > 2048)
+    return false;
   else if (threads <= 512)
-    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, 512><<<(unsigned)p.rows, threads, 0, s>>>(p);
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, 8, 512><<<(unsigned)p.rows, threads, 0, s>>>(p);
+  else if (XT != PCB_DTYPE_F32 && threads <= 768)
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, XT == PCB_DTYPE_F32 ? 8 : NE, 512>
+        <<<(unsigned)p.rows, wide, 0, s>>>(p);
   else if (threads <= 1024)
-    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, 1024><<<(unsigned)p.rows, threads, 0, s>>>(p);
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, 8, 1024><<<(unsigned)p.rows, threads, 0, s>>>(p);
+  else if (wide <= 1024)
+    norm::rms_norm_fwd_elems_kernel<XT, YT, WT, false, NE, 1024><<<(unsigned)p.rows, wide, 0, s>>>(p);
   else
     return false;
   return true;
@@ -62,7 +78,7 @@ int dispatch_norm_fwd(const norm::FwdArgs& p, bool vec, cudaStream_t s) {
   if ((same && launch_norm_fwd_elems<XT, YT, XT>(p, s)) ||
       (!same && f32 && launch_norm_fwd_elems<XT, YT, PCB_DTYPE_F32>(p, s)))
     return check_launch("rms_norm_fwd_elems_kernel");
-  // Rows too wide, or a weight of the other 16-bit type.
+  // Wide rows, or a weight of the other 16-bit type.
   const int64_t grid = std::min<int64_t>(p.rows, (int64_t)device_info().sm_count * 8);
   norm::rms_norm_fwd_generic_kernel<XT, YT><<<(unsigned)grid, norm::kGenericThreads, 0, s>>>(p);
   return check_launch("rms_norm_fwd_generic_kernel");

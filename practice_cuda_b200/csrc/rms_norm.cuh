@@ -361,16 +361,15 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_norm_fwd_kernel(const FwdArgs
 
 // The same element by element, for rows that do not suit 16-byte loads (odd
 // widths, strides or alignments): a thread holds the columns t, t + threads, ...
-// (NE of them), so every access of a warp is contiguous and all of a row's loads
+// (NE of them at most), so every access of a warp is contiguous and all of a row's loads
 // are in flight together.  A row is a warp's (widths up to 32 NE) or a CTA's,
 // whose threads are a multiple of 128: four warps hold a 128-column block.
 constexpr int kElems = 16;
 // WT is the weight's type: x's or fp32.
-template <int XT, int YT, int WT, bool WARP, int MAX_THREADS>
+template <int XT, int YT, int WT, bool WARP, int NE, int MAX_THREADS>
 __global__ void __launch_bounds__(MAX_THREADS) rms_norm_fwd_elems_kernel(const FwdArgs p) {
   using T = typename InType<XT>::T;
   using W = typename InType<WT>::T;
-  constexpr int NE = kElems;
   const int threads = WARP ? 32 : (int)blockDim.x;
   const int t = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
   const long long row = WARP ? (long long)blockIdx.x * (MAX_THREADS / 32) + (threadIdx.x >> 5) : (long long)blockIdx.x;

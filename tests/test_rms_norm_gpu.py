@@ -104,6 +104,36 @@ def test_forward_widths(rows, dim, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,dim", [(5, 511), (4, 513), (3, 2047), (3, 2049), (2, 4095), (2, 4097), (3, 6143),
+                                      (2, 6145), (2, 8191), (2, 8193), (2, 16383), (1300, 2051)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_forward_odd_widths(rows, dim, dtype):
+    x, r, w = _inputs(rows, dim, dtype, seed=rows + dim)
+    for residual in (r, None):
+        _check_forward(x, residual, w, "block", E4M3, what="block")
+        _check_forward(x, residual, w, "row", E4M3, what="row")
+        _check_forward(x, residual, w.float(), None, E4M3, what="y alone, fp32 weight")
+
+
+@gpu
+@pytest.mark.parametrize("dim", [4101, 8195])
+def test_forward_odd_zero_rows_and_non_finite_values(dim):
+    x, _, w = _inputs(5, dim, BF16, seed=3)
+    x[1] = 0
+    x[2, 5] = float("inf")
+    x[3, 7] = float("nan")
+    for residual in (None, torch.zeros_like(x)):
+        res = rms_norm_quant(x, w, residual, eps=EPS, return_y=True)
+        assert torch.equal(res.y[1], torch.zeros_like(res.y[1]))
+        assert torch.equal(res.quant.tensor[1].float(), torch.zeros(dim, device="cuda"))
+        assert bool(torch.isnan(res.y[3]).all())
+        assert bool(torch.isnan(res.y[2, 5])) and torch.equal(res.y[2, 6:].float(),
+                                                              torch.zeros(dim - 6, device="cuda"))
+        good = [0, 4]
+        _check_forward(x[good], None if residual is None else residual[good], w, "block", E4M3, what="rows beside them")
+
+
+@gpu
 @pytest.mark.parametrize("rows,dim", [(5, 512), (3, 4096), (9, 515), (2, 16392), (2, 20001)])
 @pytest.mark.parametrize("dtype,wdtype", [(BF16, F16), (F16, BF16), (F32, BF16), (F32, F16), (F16, F32)])
 def test_weights_of_another_type(rows, dim, dtype, wdtype):
