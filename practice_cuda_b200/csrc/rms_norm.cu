@@ -115,7 +115,10 @@ int launch_norm_bwd_staged(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
 }
 
 // False: the rows are too wide for these kernels.  Eight columns a thread keep
-// clear of register spills, sixteen take the widths beyond.
+// clear of register spills and let more of a row's loads be on their way (8192 x
+// 7001 bf16 on a B200: 218 us, 253 with sixteen; fp32 241 either way); sixteen take
+// the widths beyond (4096 x 16383 bf16: 292 us with a few registers spilled, 1197 us
+// in the generic kernel, which reads the row again from memory).
 template <int XT, int WT>
 bool launch_norm_bwd_elems(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
   if (p.dim <= 32 * norm::kElems) {
@@ -125,9 +128,12 @@ bool launch_norm_bwd_elems(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
     const int threads = threads_of(p.dim, 8, 32);
     parts = norm_bwd_ctas(p.rows, 1, std::min(kNormBwdMost, 1024 / threads));
     norm::rms_norm_bwd_elems_kernel<XT, WT, false, 8, 512><<<parts, threads, 0, s>>>(p);
-  } else if (p.dim <= 512 * 16) {
+  } else if (p.dim <= 1024 * 8) {
     parts = norm_bwd_ctas(p.rows, 1, 1);
-    norm::rms_norm_bwd_elems_kernel<XT, WT, false, 16, 512><<<parts, threads_of(p.dim, 16, 32), 0, s>>>(p);
+    norm::rms_norm_bwd_elems_kernel<XT, WT, false, 8, 1024><<<parts, threads_of(p.dim, 8, 32), 0, s>>>(p);
+  } else if (p.dim <= 1024 * 16) {
+    parts = norm_bwd_ctas(p.rows, 1, 1);
+    norm::rms_norm_bwd_elems_kernel<XT, WT, false, 16, 1024><<<parts, threads_of(p.dim, 16, 32), 0, s>>>(p);
   } else {
     return false;
   }

@@ -251,7 +251,8 @@ def test_backward_many_rows(rows, dim):
 
 
 @gpu
-@pytest.mark.parametrize("rows,dim", [(700, 8200), (450, 10240), (297, 16384), (149, 12296), (300, 8192), (300, 16392)])
+@pytest.mark.parametrize("rows,dim", [(700, 8200), (450, 10240), (297, 16384), (149, 12296), (300, 8192), (300, 16392),
+                                      (300, 4099), (150, 8191), (297, 8193), (149, 16383), (20, 16385)])
 @pytest.mark.parametrize("dtype,wdtype", [(BF16, BF16), (F16, F32), (F32, F32)])
 def test_backward_many_wide_rows(rows, dim, dtype, wdtype):
     h, dh, w = _inputs(rows, dim, dtype, seed=rows + dim)
