@@ -30,6 +30,7 @@
 #pragma once
 
 #include "gemm_sm100.cuh"
+#include "repack.cuh"
 
 namespace pcb {
 namespace loss {
@@ -1144,33 +1145,33 @@ __global__ void __launch_bounds__(1024) loss_weights_kernel(const float* dloss, 
 }
 
 // Rows copied to another stride, two elements (a word of dst) a thread at a
-// time: a row that starts on an odd element is read as the aligned words around it
-// and shifted, so loads and stores stay whole and contiguous across the warp.
+// time: a row that starts on an odd element is read as the aligned words around its
+// pairs and shifted, so loads and stores stay whole and contiguous across the warp.
 constexpr int kRepackLoads = 8;
+struct RowIn {
+  const uint16_t* e;
+  __device__ __forceinline__ uint32_t pair(int i) const { return __ldg(reinterpret_cast<const uint32_t*>(e + i)); }
+  __device__ __forceinline__ uint16_t half(int i) const { return __ldg(e + i); }
+};
 __global__ void __launch_bounds__(256) repack_rows_kernel(const uint16_t* src, long long rows, int cols,
                                                           long long src_stride, uint32_t* dst, long long dst_words) {
   const int words = (cols + 1) / 2;
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(src + row * src_stride);
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
-    const bool odd = at & 2;
+    const RowIn in{src + row * src_stride};
+    const bool odd = reinterpret_cast<uintptr_t>(in.e) & 2;
     uint32_t* out = dst + row * dst_words;
     for (int j0 = threadIdx.x; j0 < words; j0 += 256 * kRepackLoads) {
-      uint32_t a[kRepackLoads], b[kRepackLoads];
+      WordParts w[kRepackLoads];
 #pragma unroll
       for (int k = 0; k < kRepackLoads; ++k) {
         const int j = j0 + k * 256;
-        a[k] = b[k] = 0;
-        if (j < words) {
-          a[k] = __ldg(w + j);
-          if (odd && 2 * j + 1 < cols) b[k] = __ldg(w + j + 1);
-        }
+        w[k] = j < words ? load_word_parts(in, odd, j, cols) : WordParts{0, 0};
       }
 #pragma unroll
       for (int k = 0; k < kRepackLoads; ++k) {
         const int j = j0 + k * 256;
         if (j >= words) break;
-        const uint32_t v = odd ? __funnelshift_r(a[k], b[k], 16) : a[k];
+        const uint32_t v = join_word_parts(w[k], odd);
         if (2 * j + 1 < cols) out[j] = v;
         else *reinterpret_cast<uint16_t*>(out + j) = (uint16_t)v;
       }
