@@ -355,14 +355,15 @@ int pcb_grad_norm(const void* const* grads, const int64_t* numel, const int* dty
 /*
  * pcb_grad_norm, then out[i] = grads[i] * min(1, max_norm / (norm + eps)),
  * each product rounded once to the tensor's type.  out[i] may be grads[i];
- * tensors must not overlap otherwise.  A NaN norm makes every output NaN.
+ * outputs that overlap one another or a gradient otherwise are refused
+ * (PCB_ERR_INVALID).  A NaN norm makes every output NaN.
  */
 int pcb_grad_clip(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes, int64_t count,
                   int norm_type, float max_norm, float eps, float* norm, void* workspace, int64_t workspace_bytes,
                   void* stream);
 
 /* The scaling of pcb_grad_clip alone, with the norm read from the device
- * (a norm that several processes have joined, say). */
+ * (a norm that several processes have joined, say); it refuses the same. */
 int pcb_grad_scale(const void* const* grads, void* const* out, const int64_t* numel, const int* dtypes, int64_t count,
                    const float* norm, float max_norm, float eps, void* stream);
 

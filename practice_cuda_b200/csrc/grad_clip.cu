@@ -19,6 +19,8 @@
 // (elements above 1.8e19) is summed again in fp64, so the norm overflows only
 // where the result does.
 #include <algorithm>
+#include <new>
+#include <vector>
 
 #include "host.cuh"
 
@@ -320,6 +322,38 @@ int check_list(const List& l, bool scaled) {
   return PCB_OK;
 }
 
+// CTAs scale chunks side by side, so what is written for one tensor must be no
+// other tensor's, neither read nor written; out[i] may be in[i] itself.
+int check_overlap(const List& l) {
+  struct Span {
+    uintptr_t begin, end;
+  };
+  auto span = [&](const void* p, int64_t i) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return Span{at, at + (uintptr_t)l.numel[i] * elem_size(l.dtype[i])};
+  };
+  auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+  std::vector<Span> out;
+  try {
+    out.reserve((size_t)l.count);
+  } catch (const std::bad_alloc&) {
+    return fail(PCB_ERR_UNSUPPORTED, "too many gradients");
+  }
+  for (int64_t i = 0; i < l.count; ++i)
+    if (l.numel[i]) out.push_back(span(l.out[i], i));
+  if (!std::is_sorted(out.begin(), out.end(), before)) std::sort(out.begin(), out.end(), before);
+  bool apart = true;
+  for (size_t k = 1; k < out.size(); ++k) apart &= out[k - 1].end <= out[k].begin;
+  for (int64_t i = 0; apart && i < l.count; ++i) {
+    if (!l.numel[i] || l.in[i] == l.out[i]) continue;
+    const Span in = span(l.in[i], i);
+    // The first written span that ends behind in.begin: they are apart, so their ends are in order too.
+    const auto at = std::partition_point(out.begin(), out.end(), [&](const Span& o) { return o.end <= in.begin; });
+    apart = at == out.end() || at->begin >= in.end;
+  }
+  return apart ? PCB_OK : fail(PCB_ERR_INVALID, "gradients or outputs overlap: each element may be scaled once only");
+}
+
 // Calls f(table, grid) for each table of at most N tensors; empty tensors are left out.
 template <int N, typename F>
 int for_tables(const List& l, F&& f) {
@@ -396,6 +430,8 @@ int entry(const List& l, int norm_type, bool scale, float* norm, float max_norm,
           int64_t workspace_bytes, void* stream) {
   if (norm_type != PCB_GRAD_NORM_L2 && norm_type != PCB_GRAD_NORM_MAX) return fail(PCB_ERR_INVALID, "bad norm type");
   if (int st = check_list(l, scale)) return st;
+  if (scale)
+    if (int st = check_overlap(l)) return st;
   if (!norm || !workspace || !aligned(workspace, 8) || workspace_bytes < pcb_grad_norm_workspace_bytes(l.count))
     return fail(PCB_ERR_INVALID, "gradient norm workspace too small or misaligned");
   double* partial = static_cast<double*>(workspace);
@@ -437,6 +473,7 @@ int pcb_grad_scale(const void* const* grads, void* const* out, const int64_t* nu
   if (!(max_norm >= 0.f)) return fail(PCB_ERR_INVALID, "max_norm must not be negative");
   const List l{grads, out, numel, dtypes, count};
   if (int st = check_list(l, true)) return st;
+  if (int st = check_overlap(l)) return st;
   if (!norm) return fail(PCB_ERR_INVALID, "null pointer");
   float* n = const_cast<float*>(norm);  // read only where no partials are given
   cudaStream_t s = (cudaStream_t)stream;

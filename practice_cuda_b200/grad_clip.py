@@ -125,6 +125,21 @@ def _check_writable(out: Sequence[torch.Tensor], what: str) -> None:
             raise ValueError(f"{what}: cannot write to an expanded tensor of shape {tuple(o.shape)}")
 
 
+def _check_apart(out: Sequence[torch.Tensor], what: str) -> None:
+    """Refuse a tensor that is written twice.  (The library refuses dense tensors that
+    overlap; these, of which some are not, are written one after the other.)"""
+    pointers = [o.data_ptr() for o in out if o.numel()]
+    if len(set(pointers)) != len(pointers):
+        raise ValueError(f"{what}: gradients or outputs overlap: each element may be scaled once only")
+
+
+def _check_status(status: int, entry: str, what: str) -> None:
+    if status == _lib.PCB_ERR_INVALID:
+        raise ValueError(f"{what}: {_lib.lib().pcb_last_error_text().decode()}")
+    if status:
+        _lib.check(status, entry)
+
+
 def clip_grad_norm(
     tensors: Union[torch.Tensor, Iterable[torch.Tensor]],
     max_norm: float,
@@ -138,7 +153,9 @@ def clip_grad_norm(
     """Scale ``tensors`` by ``min(1, max_norm / (norm + eps))`` and return
     the norm before it (0-dim fp32, on the device).
 
-    In place, or into ``out`` (one tensor each, of the same shape and type).
+    In place, or into ``out`` (one tensor each, of the same shape and type).  Each
+    element is scaled once: a tensor that stands in the list twice, tensors that
+    overlap, and outputs that overlap another gradient are refused.
     A non-finite norm makes the gradients NaN or 0, as the product says;
     ``error_if_nonfinite`` raises instead, before anything is written, and
     waits for the GPU to know.  With ``group``, the tensors are this process's
@@ -160,6 +177,7 @@ def clip_grad_norm(
         src, dst, direct = tensors, out, None
         if not (all(map(_contiguous, out)) and (in_place or all(map(_contiguous, tensors)))):
             _check_writable(out, what)
+            _check_apart(out, what)
             direct = [_dense(t) and _dense(o) and _same_order(t, o) for t, o in zip(tensors, out)]
             src = [t if d else t.contiguous() for t, d in zip(tensors, direct)]
             dst = [o if d else torch.empty_like(t) for t, o, d in zip(src, out, direct)]
@@ -173,7 +191,7 @@ def clip_grad_norm(
             status = lib.pcb_grad_clip(pointers, targets_at, *table.args(), code, max_norm, eps, norm.data_ptr(),
                                        workspace.data_ptr(), nbytes, stream)
             if status:
-                _lib.check(status, "pcb_grad_clip")
+                _check_status(status, "pcb_grad_clip", what)
         else:
             norm = grad_norm(src, norm_type=norm_type)
             if group is not None:
@@ -182,7 +200,7 @@ def clip_grad_norm(
                 raise RuntimeError(f"{what}: the gradients' norm is {norm.item()}")
             status = lib.pcb_grad_scale(pointers, targets_at, *table.args(), norm.data_ptr(), max_norm, eps, stream)
             if status:
-                _lib.check(status, "pcb_grad_scale")
+                _check_status(status, "pcb_grad_scale", what)
         if direct is not None:
             for t, o, d in zip(dst, out, direct):
                 if not d:

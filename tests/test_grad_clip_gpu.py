@@ -279,3 +279,76 @@ def test_entry_points_reject_bad_arguments_without_gpu():
                    {"pointer": 0}, {"pointer": 17}, {"norm": None}, {"nbytes": 0}, {"count": -1}):
         assert clip(**kwargs) == _lib.PCB_ERR_INVALID, kwargs
     assert lib.pcb_grad_norm(None, None, None, 1, 0, 16, 16, 1 << 20, None) == _lib.PCB_ERR_INVALID
+
+
+def test_overlapping_tensors_are_refused_without_gpu():
+    """Two CTAs would scale the same elements at once."""
+    import ctypes
+
+    lib = _lib.lib()
+
+    def status(entry, grads, out, numel, dtypes=None):
+        count = len(grads)
+        pointers, targets = (ctypes.c_uint64 * count)(*grads), (ctypes.c_uint64 * count)(*out)
+        sizes, kinds = (ctypes.c_int64 * count)(*numel), (ctypes.c_int * count)(*(dtypes or [0] * count))
+        table = (ctypes.addressof(pointers), ctypes.addressof(targets), ctypes.addressof(sizes), ctypes.addressof(kinds))
+        if entry == "clip":  # a norm that is missing is refused too, but later
+            return lib.pcb_grad_clip(*table, count, 0, 1.0, EPS, None, None, 0, None), lib.pcb_last_error_text().decode()
+        return lib.pcb_grad_scale(*table, count, None, 1.0, EPS, None), lib.pcb_last_error_text().decode()
+
+    bad = [
+        ([64, 64], [64, 64], [4, 4]),  # one tensor twice
+        ([256, 64, 256], [256, 64, 256], [4, 4, 4]),
+        ([64, 72], [64, 72], [4, 4]),  # 16 bytes from 64 on, and from 72 on
+        ([64, 128], [128, 64], [4, 4]),  # outputs changed over
+        ([64, 128], [256, 264], [4, 4]),  # outputs that overlap
+        ([64], [68], [4]),  # an output that is moved by less than its length
+        ([64, 80, 512], [64, 80, 92], [4, 4, 4]),  # an output in another gradient
+    ]
+    good = [
+        ([64, 80], [64, 80], [4, 4]),  # neighbours
+        ([80, 64], [80, 64], [4, 4]),
+        ([64, 64], [256, 512], [4, 4]),  # one gradient into two outputs
+        ([64, 64], [64, 64], [4, 0]),  # an empty tensor
+        ([64, 128], [256, 272], [4, 4]),
+        ([64], [80], [4]),
+        ([64, 80, 512], [64, 80, 96], [4, 4, 4]),
+    ]
+    for entry in ("clip", "scale"):
+        for case in bad:
+            code, text = status(entry, *case)
+            assert code == _lib.PCB_ERR_INVALID and "overlap" in text, case
+        for case in good:
+            assert "overlap" not in status(entry, *case)[1], case
+        assert "overlap" in status(entry, [64, 72], [64, 72], [4, 4], [0, 0])[1]
+        assert "overlap" not in status(entry, [64, 72], [64, 72], [4, 4], [1, 1])[1]  # 8 bytes each
+
+
+@gpu
+def test_overlapping_tensors_are_refused():
+    g = torch.arange(1.0, 101.0, device="cuda").view(10, 10)
+    kept, other = g.clone(), torch.empty_like(g)
+    parameter = torch.nn.Parameter(torch.zeros(10, 10, device="cuda"))
+    parameter.grad = g
+    for bad in (
+        lambda: clip_grad_norm([g, g], 1.0),
+        lambda: clip_grad_norm([g, g], 1.0, error_if_nonfinite=True),
+        lambda: clip_grad_norm([g[:6], g[5:]], 1.0),
+        lambda: clip_grad_norm([g, other], 1.0, out=[other, g]),
+        lambda: clip_grad_norm([g, kept], 1.0, out=[other, other]),
+        lambda: clip_grad_norm([g[:, ::2], g[:, ::2]], 1.0),  # strided ones
+        lambda: clip_grad_norm_([parameter, parameter], 1.0),
+    ):
+        with pytest.raises(ValueError, match="overlap"):
+            bad()
+    assert torch.equal(g, kept)
+    norm64 = _norm64([kept])
+    # Neighbours, columns that take turns, and a gradient that is read twice are fine.
+    clip_grad_norm([g[:5], g[5:]], 0.5 * norm64)
+    _check_clipped([g], [kept], 0.5 * norm64 / (norm64 + EPS))
+    g.copy_(kept)
+    clip_grad_norm([g[:, ::2], g[:, 1::2]], 0.5 * norm64)
+    _check_clipped([g], [kept], 0.5 * norm64 / (norm64 + EPS))
+    twice = [torch.empty_like(g), torch.empty_like(g)]
+    clip_grad_norm([kept, kept], norm64, out=twice)
+    _check_clipped(twice, [kept, kept], norm64 / (math.sqrt(2.0) * norm64 + EPS))
