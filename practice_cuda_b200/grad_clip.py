@@ -205,8 +205,9 @@ def clip_grad_norm(
             for t, o, d in zip(dst, out, direct):
                 if not d:
                     o.copy_(t)
-        if any([o.requires_grad for o in out]):  # part of a graph: what it has saved of them is now stale
-            torch.autograd.graph.increment_version(out)
+        # A graph may have saved any of them, whether or not they require a gradient:
+        # it is to see that they have changed, as after an in-place operation of torch.
+        torch.autograd.graph.increment_version(out)
     return norm
 
 
@@ -243,8 +244,11 @@ def clip_grad_norm_(
     if not grads:
         return torch.zeros(())
     locals_, group = _local_shards(grads, what)
-    return clip_grad_norm(locals_, max_norm, norm_type=norm_type, eps=eps, error_if_nonfinite=error_if_nonfinite,
+    norm = clip_grad_norm(locals_, max_norm, norm_type=norm_type, eps=eps, error_if_nonfinite=error_if_nonfinite,
                           group=group)
+    if group is not None:  # the shards' versions are their own
+        torch.autograd.graph.increment_version(grads)
+    return norm
 
 
 def _local_shards(grads: list[torch.Tensor], what: str):

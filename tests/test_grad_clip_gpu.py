@@ -352,3 +352,55 @@ def test_overlapping_tensors_are_refused():
     twice = [torch.empty_like(g), torch.empty_like(g)]
     clip_grad_norm([kept, kept], norm64, out=twice)
     _check_clipped(twice, [kept, kept], norm64 / (math.sqrt(2.0) * norm64 + EPS))
+
+
+@gpu
+def test_clipping_what_a_graph_has_saved_is_seen():
+    """Gradients do not require a gradient themselves, but a graph may hold them."""
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    plain = lambda: torch.full((8, 8), 3.0, device="cuda")
+    targets = {
+        "in place": lambda g: clip_grad_norm([g], 0.1),
+        "in place, not finite": lambda g: clip_grad_norm([g], 0.1, error_if_nonfinite=True),
+        "an output": lambda g: clip_grad_norm([plain()], 0.1, out=[g]),
+        "detached": lambda g: clip_grad_norm([g.detach()], 0.1),
+        "a view": lambda g: clip_grad_norm([g[2:5]], 0.1),
+        "columns": lambda g: clip_grad_norm([g[:, 2:5]], 0.1),
+        "beside a strided one": lambda g: clip_grad_norm([plain()[:, ::2], g], 0.1),
+    }
+    for name, clip in targets.items():
+        g = plain()
+        loss = (w * g.view(64)).sum()  # keeps g
+        version = g._version
+        clip(g)
+        assert g._version > version, name
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    # What is read alone keeps its version.
+    g, out = plain(), plain()
+    version = g._version
+    clip_grad_norm([g], 0.1, out=[out])
+    grad_norm([g])
+    assert g._version == version
+    with torch.inference_mode():
+        clip_grad_norm([plain()], 0.1)
+
+
+def test_clipping_sharded_gradients_is_seen_without_gpu(tmp_path, monkeypatch):
+    """The DTensor that holds a clipped shard counts the change too."""
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import Shard, distribute_tensor
+
+    from practice_cuda_b200 import grad_clip
+
+    monkeypatch.setattr(grad_clip, "clip_grad_norm", lambda tensors, *args, **kwargs: torch.ones(()))
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cpu", (1,))
+        parameter = torch.nn.Parameter(distribute_tensor(torch.ones(4, 2), mesh, [Shard(0)]))
+        parameter.grad = distribute_tensor(torch.full((4, 2), 3.0), mesh, [Shard(0)])
+        version = parameter.grad._version
+        grad_clip.clip_grad_norm_([parameter], 0.1)
+        assert parameter.grad._version > version
+    finally:
+        dist.destroy_process_group()
