@@ -409,8 +409,7 @@ int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t
  * pieces of `piece` columns (rounded down to a multiple of 256; <= 0: as many
  * as keep G at 128 MiB, at least 2048), of which only one piece of G exists at
  * a time.  Sums are taken in a fixed order.  What x holds for tokens that are
- * left out reaches nothing; where pcb_linear_ce_packed_bytes is not 0 it must be
- * finite for that, or the packed passes be used.
+ * left out reaches nothing.
  */
 int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
@@ -432,6 +431,9 @@ int pcb_linear_ce_packed_fwd(const void* x, int64_t sx, const void* weight, int6
                              int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
                              float* loss, float* stats, float* count, void* packed, int64_t packed_bytes,
                              void* workspace, int64_t workspace_bytes, void* stream);
+/* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_packed_bwd. */
+int64_t pcb_linear_ce_packed_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece,
+                                                 int want_dx, int want_dw);
 int pcb_linear_ce_packed_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,
                              int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
                              const float* stats, const float* count, const void* packed, int64_t packed_bytes,

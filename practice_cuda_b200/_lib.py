@@ -162,6 +162,7 @@ _SIGNATURES = {
          _vp, _i64, _i, _vp, _vp, _vp,  # target, ignore index, reduction, loss, stats, count
          _vp, _i64, _vp, _i64, _vp],  # packed, workspace
     ),
+    "pcb_linear_ce_packed_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i, _i]),
     "pcb_linear_ce_packed_bwd": (
         _i,
         [_vp, _i64, _vp, _i64, _i, _i64, _i64, _i64,  # x, weight, dtype, tokens, vocab, dim

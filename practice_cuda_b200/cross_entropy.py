@@ -123,7 +123,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             dloss = dloss.to(torch.float32).contiguous()
             dx = x2.new_empty((tokens, dim)) if want_dx else None
             dw = x2.new_empty((vocab, dim)) if want_dw else None
-            nbytes = lib.pcb_linear_ce_bwd_workspace_bytes(tokens, vocab, dim, piece, want_dx, want_dw)
+            nbytes = lib.pcb_linear_ce_packed_bwd_workspace_bytes(tokens, vocab, dim, piece, want_dx, want_dw)
             workspace = x2.new_empty((nbytes,), dtype=torch.uint8)
             at = stats.data_ptr()
             status = lib.pcb_linear_ce_packed_bwd(

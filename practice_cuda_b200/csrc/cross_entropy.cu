@@ -264,10 +264,16 @@ struct BwdPlan {
   int64_t cols, pieces, pitch;  // of G
   int splits;                   // parts of K of dX
   int64_t g, acc, weight, alpha, x, pitch_x, bytes;
-  BwdPlan(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, bool want_dx, bool want_dw) {
+  bool copies;  // dW reads a copy of X without the rows of tokens that are left out
+  BwdPlan(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, bool want_dx, bool want_dw, bool packed) {
+    pitch_x = up(dim, 64) * 64;
+    copies = want_dw && !packed;
+    const int64_t copy = copies ? tokens * pitch_x * 2 : 0;
     // G of one piece takes 128 MiB at most (and is no narrower than 2048
-    // columns): pieces of even width, whole tiles each.
-    if (piece <= 0) piece = std::max<int64_t>(2048, ((int64_t)128 << 20) / 2 / tokens);
+    // columns): pieces of even width, whole tiles each.  The copy of X is within
+    // that where it is large.
+    const int64_t budget = ((int64_t)128 << 20) - (packs(tokens, vocab, dim) ? copy : 0);
+    if (piece <= 0) piece = std::max<int64_t>(2048, budget / 2 / tokens);
     piece = std::max<int64_t>(loss::TILE, piece / loss::TILE * loss::TILE);
     pieces = up(vocab, piece);
     cols = up(up(vocab, pieces), loss::TILE) * loss::TILE;
@@ -280,8 +286,7 @@ struct BwdPlan {
     acc = c.take(want_dx && (pieces > 1 || splits > 1) ? dx_tiles * splits * loss::TILE * loss::WIDE * 4 : 0);
     weight = c.take(tokens * 4);
     alpha = c.take(4);
-    pitch_x = up(dim, 64) * 64;
-    x = c.take(want_dw && !packs(tokens, vocab, dim) ? tokens * pitch_x * 2 : 0);
+    x = c.take(copy);
     bytes = c.at;
   }
 };
@@ -373,7 +378,7 @@ int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtyp
   }
   if (!dx && !dw) return PCB_OK;
   if (!target || !stats || !count || !dloss) return fail(PCB_ERR_INVALID, "null pointer");
-  const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr, dw != nullptr);
+  const BwdPlan plan(tokens, vocab, dim, piece, dx != nullptr, dw != nullptr, order != nullptr);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.bytes)
     return fail(PCB_ERR_INVALID, "linear cross entropy workspace too small or misaligned");
   if (int st = check_operands(x, sx, weight, sw)) return st;
@@ -406,8 +411,7 @@ int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtyp
     base.dloss = dloss;
     base.count = reduction == loss::kMean ? count : nullptr;
   }
-  const bool copies = dw && !packs(tokens, vocab, dim);
-  if (copies)
+  if (plan.copies)
     if (int st = launch_after(loss::loss_kept_rows_kernel, "loss_kept_rows_kernel",
                               std::min<int64_t>(tokens, (int64_t)device_info().sm_count * 8), 256, s,
                               static_cast<const uint16_t*>(x), (long long)sx, base.target, (long long)ignore_index,
@@ -457,7 +461,7 @@ int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtyp
       ok &= slab_map(&d.a, g, dtype, plan.pitch / 64, tokens, plan.pitch);  // rows of dW beyond cols are not stored
       ok &= load_b(&d.b, d, x, dtype, dim, tokens, sx);
       if (packed_x) ok &= load_b(&d.packed, d, packed_x, dtype, dim, tokens, packed.stride);
-      if (copies) {
+      if (plan.copies) {
         ok &= load_b(&d.packed, d, ws + plan.x, dtype, dim, tokens, plan.pitch_x);
         p.kept = count;
       }
@@ -543,7 +547,13 @@ int pcb_linear_ce_packed_fwd(const void* x, int64_t sx, const void* weight, int6
 int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx,
                                           int want_dw) {
   if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
-  return BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0).bytes;
+  return BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0, false).bytes;
+}
+
+int64_t pcb_linear_ce_packed_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece,
+                                                 int want_dx, int want_dw) {
+  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  return BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0, packs(tokens, vocab, dim)).bytes;
 }
 
 int pcb_linear_ce_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,

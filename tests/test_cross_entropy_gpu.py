@@ -481,3 +481,42 @@ def test_non_finite_rows_left_out_reach_nothing(tokens, vocab, dim, reduction, v
     loss = linear_cross_entropy(x, w1, target, reduction=reduction)
     assert torch.equal(torch.autograd.grad(loss, w1, dloss)[0], expected[2])
     assert _lib.device_error()[0] == 0
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,dim", [(515, 33001, 4104), (300, 900, 192)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_entry_points_without_packed_state(tokens, vocab, dim, reduction):
+    """pcb_linear_ce_fwd and _bwd, at a size that the packed passes would pack and at one that they would not:
+    what x holds for tokens that are left out reaches nothing."""
+    x, w, target = _inputs(tokens, vocab, dim, BF16, seed=dim, ignored=0.4)
+    left_out = target == IGNORE
+    lib, code = _lib.lib(), _lib.PCB_DTYPE[BF16]
+    assert (lib.pcb_linear_ce_packed_bytes(tokens, vocab, dim) > 0) == (tokens > 500)
+    stream = torch.cuda.current_stream().cuda_stream
+    red = ["none", "sum", "mean"].index(reduction)
+    one = torch.rand(tokens if red == 0 else 1, generator=torch.Generator().manual_seed(1)).cuda() + 0.5
+    ws = torch.empty(lib.pcb_linear_ce_fwd_workspace_bytes(tokens, vocab), dtype=torch.uint8, device="cuda")
+    ws2 = torch.empty(lib.pcb_linear_ce_bwd_workspace_bytes(tokens, vocab, dim, 0, 1, 1), dtype=torch.uint8, device="cuda")
+
+    def run():
+        ws.fill_(0xff), ws2.fill_(0xff)  # NaN, whatever they are read as
+        args = (x.data_ptr(), dim, w.data_ptr(), dim, code, tokens, vocab, dim, target.data_ptr(), IGNORE, red)
+        loss, stats, count = (torch.empty(n, device="cuda") for n in (one.numel(), 2 * tokens, 1))
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        assert lib.pcb_linear_ce_fwd(*args, loss.data_ptr(), stats.data_ptr(), count.data_ptr(), ws.data_ptr(),
+                                     ws.numel(), stream) == 0
+        assert lib.pcb_linear_ce_bwd(*args, stats.data_ptr(), count.data_ptr(), one.data_ptr(), dx.data_ptr(), dim,
+                                     dw.data_ptr(), dim, 0, ws2.data_ptr(), ws2.numel(), stream) == 0
+        return loss, dx, dw
+
+    x[left_out] = 0.0
+    clean = run()
+    expected = _reference(x, w, target, reduction, one if red == 0 else one[0])
+    for got, (value, off), name in zip(clean, expected, ("loss", "dx", "dw")):
+        _within(got.view(value.shape), value, off, name)
+    for value in (float("nan"), float("-inf")):
+        x[left_out] = value
+        for a, b, name in zip(run(), clean, ("loss", "dx", "dw")):
+            assert torch.equal(a, b), f"{name} with {value}"
+    assert _lib.device_error()[0] == 0
