@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -151,8 +152,8 @@ def linear_cross_entropy(
 
     ``reduction``, ``ignore_index`` and the mean over no token at all (NaN,
     with zero gradients) are those of ``torch.nn.functional.cross_entropy``.
-    Differentiable (once) in ``x`` and ``weight``; a gradient that is not needed
-    is not computed.  ``vocab_piece`` bounds the columns of the logits' gradient
+    Differentiable (once, in reverse mode) in ``x`` and ``weight``; a gradient that
+    is not needed is not computed.  ``vocab_piece`` bounds the columns of the logits' gradient
     that exist at a time in the backward pass (rounded down to a multiple of
     256, at least 256; default: as many as fit 128 MiB, at least 2048).
 
@@ -170,7 +171,9 @@ def linear_cross_entropy(
     t = target if target.ndim == 1 else target.reshape(-1)
     t = t.to(torch.int64).contiguous()
     code = _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad):
+    train = torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad)
+    # A tangent of forward mode goes to the autograd function too, which refuses it.
+    if train or unpack_dual(x2).tangent is not None or unpack_dual(weight).tangent is not None:
         loss = _LinearCrossEntropy.apply(x2, weight, t, int(ignore_index), code, int(vocab_piece or 0))
     else:
         loss = _forward(x2, weight, t, int(ignore_index), code, False)[0]

@@ -520,3 +520,21 @@ def test_entry_points_without_packed_state(tokens, vocab, dim, reduction):
         for a, b, name in zip(run(), clean, ("loss", "dx", "dw")):
             assert torch.equal(a, b), f"{name} with {value}"
     assert _lib.device_error()[0] == 0
+
+
+@gpu
+def test_forward_mode_is_refused():
+    """No tangent is dropped without a word, whatever else the call needs."""
+    import torch.autograd.forward_ad as forward_ad
+
+    x, w, target = _inputs(16, 64, 32, BF16, seed=18)
+    tangent = torch.ones_like(x)
+    with forward_ad.dual_level():
+        dual_x, dual_w = forward_ad.make_dual(x, tangent), forward_ad.make_dual(w, torch.ones_like(w))
+        for args in ((dual_x, w), (x, dual_w), (x.clone().requires_grad_(), dual_w),
+                     (forward_ad.make_dual(x.view(2, 8, 32), tangent.view(2, 8, 32)), w)):
+            with pytest.raises(NotImplementedError, match="jvp"):
+                linear_cross_entropy(*args, target.view(args[0].shape[:-1]))
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp"):
+                linear_cross_entropy(*args, target.view(args[0].shape[:-1]))
+        assert not linear_cross_entropy(x, w, target).requires_grad
