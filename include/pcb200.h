@@ -346,8 +346,8 @@ int64_t pcb_grad_norm_workspace_bytes(int64_t count);
  * grads[i] is a device pointer to numel[i] contiguous elements of dtypes[i]
  * (F32/F16/BF16; types may be mixed).  The four arrays are host memory and
  * are read before the call returns.  *norm (device, fp32) gets the norm;
- * squares are summed in fp32 runs of at most 32 and in fp64 from there on, in
- * a fixed order.  No tensors, or only empty ones: 0.
+ * squares are summed in fp32 runs of at most 32 (in fp64 where they leave its
+ * range at either end) and in fp64 from there on, in a fixed order.  No tensors, or only empty ones: 0.
  */
 int pcb_grad_norm(const void* const* grads, const int64_t* numel, const int* dtypes, int64_t count, int norm_type,
                   float* norm, void* workspace, int64_t workspace_bytes, void* stream);

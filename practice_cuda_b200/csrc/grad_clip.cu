@@ -16,8 +16,9 @@
 //
 // Squares are summed in fp32 over the 16 or 32 elements that a thread loads
 // at a time and in fp64 from there on; a group whose fp32 sum is not finite
-// (elements above 1.8e19) is summed again in fp64, so the norm overflows only
-// where the result does.
+// (elements above 1.8e19), or so small that its squares are subnormal or nothing
+// in fp32, is summed again in fp64.  So the norm is as exact for any gradients, and
+// overflows only where the result does.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -143,11 +144,17 @@ struct SquareAcc {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < n; ++i) s = fmaf(f[i], f[i], s);
-    if (s <= 3.4e38f) {
+    // Squares below 2^-126 are off by up to 2^-150 each: 32 of them by 2^-29 of 1e-35.
+    if (s >= 1e-35f && s <= 3.4e38f) {
       v += (double)s;
-    } else {  // overflow, infinity or NaN
-      for (int i = 0; i < n; ++i) v += (double)f[i] * (double)f[i];
+      return;
     }
+    uint32_t any = 0;  // zeros are common, and are not summed again
+#pragma unroll
+    for (int i = 0; i < n; ++i) any |= abs_bits(f[i]);
+    if (any == 0) return;
+#pragma unroll
+    for (int i = 0; i < n; ++i) v += (double)f[i] * (double)f[i];
   }
   __device__ __forceinline__ double value() const { return v; }
   static __device__ __forceinline__ double join(double a, double b) { return a + b; }

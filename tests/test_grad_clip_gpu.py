@@ -404,3 +404,24 @@ def test_clipping_sharded_gradients_is_seen_without_gpu(tmp_path, monkeypatch):
         assert parameter.grad._version > version
     finally:
         dist.destroy_process_group()
+
+
+@gpu
+@pytest.mark.parametrize("value", [1e-18, 1e-20, 1e-23, 1e-30, 1e-36])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_squares_below_the_range_of_fp32(value, dtype):
+    """Gradients whose squares are subnormal or nothing in fp32: the norm has the same accuracy."""
+    for sizes in ([5000], [1], [7, 8193, 40]):
+        small = [synthetic((n,), std=value, seed=n, dtype=dtype).cuda() for n in sizes]
+        expected = _norm64(small)
+        assert abs(grad_norm(small).item() - expected) <= RTOL_NORM * expected
+        before = [t.clone() for t in small]
+        norm = clip_grad_norm(small, 0.5 * expected, eps=0.0)
+        assert abs(norm.item() - expected) <= RTOL_NORM * expected
+        _check_clipped(small, before, 0.5)
+    # Large ones beside them, and zeros.
+    mixed = [torch.full((300,), value, device="cuda", dtype=dtype), torch.zeros(5000, device="cuda", dtype=dtype),
+             torch.ones(3, device="cuda", dtype=dtype)]
+    assert abs(grad_norm(mixed).item() - _norm64(mixed)) <= RTOL_NORM * _norm64(mixed)
+    mixed.pop()
+    assert abs(grad_norm(mixed).item() - _norm64(mixed)) <= RTOL_NORM * _norm64(mixed)
