@@ -66,7 +66,9 @@ const char* pcb_last_error_text(void);
 /* Read and clear the device error word of the current device.  *code is 0
  * when no kernel reported a failure; otherwise a pcb_status (PCB_ERR_TIMEOUT
  * for a bounded wait that ran out), *site the kernel/wait site and *info the
- * block index.  Synchronises the device. */
+ * block index.  The cross entropy's kernels have a word of their own: where they
+ * and another kernel failed, each of two calls reports one.  Synchronises the
+ * device. */
 int pcb_get_device_error(int* code, int* site, int* info);
 
 /* Test hook: the next pcb_bmm_scaled launch makes its kernel report `code`

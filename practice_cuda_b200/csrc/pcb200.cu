@@ -451,9 +451,8 @@ int pcb_get_device_error(int* code, int* site, int* info) {
   const unsigned int zero[3] = {0, 0, 0};
   if (cudaMemcpyToSymbol(pcb::g_device_error, zero, sizeof(zero)) != cudaSuccess)
     return check_launch("pcb_get_device_error clear");
-  unsigned int loss[3] = {0, 0, 0};
-  if (take_loss_device_error(loss) != cudaSuccess) return check_launch("pcb_get_device_error read");
-  if (h[0] == 0) std::memcpy(h, loss, sizeof(h));
+  // The loss has a word of its own: left for the next call where this one has an error to tell.
+  if (h[0] == 0 && take_loss_device_error(h) != cudaSuccess) return check_launch("pcb_get_device_error read");
   if (code) *code = (int)h[0];
   if (site) *site = (int)h[1];
   if (info) *info = (int)h[2];

@@ -538,3 +538,21 @@ def test_forward_mode_is_refused():
             with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp"):
                 linear_cross_entropy(*args, target.view(args[0].shape[:-1]))
         assert not linear_cross_entropy(x, w, target).requires_grad
+
+
+@gpu
+def test_error_of_the_loss_beside_another_kernels():
+    """Two kernels report in one interval: both errors are read, one after the other."""
+    from practice_cuda_b200.registry import get_bmm, get_quant
+
+    _lib.device_error()  # clear
+    a, b = synthetic((1, 128, 128), seed=30).cuda(), synthetic((1, 128, 128), seed=31).cuda()
+    quant = get_quant("b200_per_channel").fn
+    qa, qb = quant(a, channel_axis=-2), quant(b, channel_axis=-1)
+    _lib.check(_lib.lib().pcb_debug_inject_error(_lib.PCB_ERR_TIMEOUT), "inject")
+    get_bmm("b200_per_channel_a_k_b_n").fn(qa, qb)
+    x, w, target = _inputs(10, 300, 64, BF16, seed=14)
+    target[3] = 300
+    linear_cross_entropy(x, w, target)
+    codes = [_lib.device_error()[:2] for _ in range(3)]
+    assert codes == [(_lib.PCB_ERR_TIMEOUT, 4), (_lib.PCB_ERR_INVALID, 19), (0, 0)]
