@@ -148,6 +148,16 @@ void shape(loss::Problem& q, int64_t m, int64_t n, int64_t k, int splits, bool p
   q.tiles = q.m_blocks * q.n_blocks * q.splits;
 }
 
+bool too_large(int64_t tokens, int64_t vocab, int64_t dim) {
+  return tokens > (1 << 26) || vocab > (1 << 26) || dim > (1 << 26) ||
+         up(tokens, loss::TILE) * up(vocab, loss::TILE) > (1 << 30) ||
+         up(std::max(tokens, vocab), loss::TILE) * up(dim, loss::WIDE) > (1 << 24);  // (times at most 64 splits)
+}
+// Sizes that need a workspace: no tokens need none, and what the passes refuse is not computed with.
+bool has_workspace(int64_t tokens, int64_t vocab, int64_t dim) {
+  return tokens > 0 && vocab > 0 && dim > 0 && !too_large(tokens, vocab, dim);
+}
+
 int check_shapes(int dtype, int64_t tokens, int64_t vocab, int64_t dim, int reduction) {
   if (dtype != PCB_DTYPE_F16 && dtype != PCB_DTYPE_BF16)
     return fail(PCB_ERR_INVALID, "linear cross entropy: x and weight must be F16 or BF16");
@@ -155,11 +165,8 @@ int check_shapes(int dtype, int64_t tokens, int64_t vocab, int64_t dim, int redu
     return fail(PCB_ERR_INVALID, "linear cross entropy needs tokens >= 0, vocab > 0 and dim > 0");
   if (reduction < loss::kNone || reduction > loss::kMean)
     return fail(PCB_ERR_INVALID, "linear cross entropy: reduction must be 0 (none), 1 (sum) or 2 (mean)");
-  if (tokens > (1 << 26) || vocab > (1 << 26) || dim > (1 << 26))
-    return fail(PCB_ERR_UNSUPPORTED, "linear cross entropy: dimension too large");
-  if (up(tokens, loss::TILE) * up(vocab, loss::TILE) > (1 << 30) ||
-      up(std::max(tokens, vocab), loss::TILE) * up(dim, loss::WIDE) > (1 << 24))  // (times at most 64 splits)
-    return fail(PCB_ERR_UNSUPPORTED, "linear cross entropy: too many tiles");
+  if (too_large(tokens, vocab, dim))
+    return fail(PCB_ERR_UNSUPPORTED, "linear cross entropy: dimension too large, or too many tiles");
   return PCB_OK;
 }
 
@@ -274,6 +281,7 @@ struct BwdPlan {
     // that where it is large.
     const int64_t budget = ((int64_t)128 << 20) - (packs(tokens, vocab, dim) ? copy : 0);
     if (piece <= 0) piece = std::max<int64_t>(2048, budget / 2 / tokens);
+    piece = std::min(piece, up(vocab, loss::TILE) * loss::TILE);  // whatever a caller names: sums with it stay in range
     piece = std::max<int64_t>(loss::TILE, piece / loss::TILE * loss::TILE);
     pieces = up(vocab, piece);
     cols = up(up(vocab, pieces), loss::TILE) * loss::TILE;
@@ -518,12 +526,12 @@ int pcb_repack_u16(const void* src, int64_t rows, int64_t cols, int64_t src_stri
 }
 
 int64_t pcb_linear_ce_packed_bytes(int64_t tokens, int64_t vocab, int64_t dim) {
-  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  if (!has_workspace(tokens, vocab, dim)) return 0;
   return Order(tokens, vocab, dim).bytes;
 }
 
 int64_t pcb_linear_ce_fwd_workspace_bytes(int64_t tokens, int64_t vocab) {
-  if (tokens <= 0 || vocab <= 0) return 0;
+  if (!has_workspace(tokens, vocab, 1)) return 0;
   return FwdPlan(tokens, vocab).bytes;
 }
 
@@ -546,13 +554,13 @@ int pcb_linear_ce_packed_fwd(const void* x, int64_t sx, const void* weight, int6
 
 int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx,
                                           int want_dw) {
-  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  if (!has_workspace(tokens, vocab, dim)) return 0;
   return BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0, false).bytes;
 }
 
 int64_t pcb_linear_ce_packed_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece,
                                                  int want_dx, int want_dw) {
-  if (tokens <= 0 || vocab <= 0 || dim <= 0) return 0;
+  if (!has_workspace(tokens, vocab, dim)) return 0;
   return BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0, packs(tokens, vocab, dim)).bytes;
 }
 

@@ -556,3 +556,44 @@ def test_error_of_the_loss_beside_another_kernels():
     linear_cross_entropy(x, w, target)
     codes = [_lib.device_error()[:2] for _ in range(3)]
     assert codes == [(_lib.PCB_ERR_TIMEOUT, 4), (_lib.PCB_ERR_INVALID, 19), (0, 0)]
+
+
+def test_workspace_sizes_of_any_arguments_without_gpu():
+    """Sizes whose sums pass 64 bits: no crash, and a piece beyond the vocabulary is the vocabulary."""
+    import subprocess
+    import sys
+
+    program = """
+import ctypes, sys
+lib = ctypes.CDLL(sys.argv[1])
+i64 = ctypes.c_int64
+def sized(name, *args):
+    fn = getattr(lib, name)
+    fn.restype, fn.argtypes = i64, [i64] * len(args)
+    return fn(*args)
+big = 2 ** 63 - 1
+whole = sized("pcb_linear_ce_bwd_workspace_bytes", 300, 1000, 200, 1024, 1, 1)
+assert whole > 0
+for piece in (1025, 10 ** 9, 2 ** 31, 2 ** 62, big - 300, big):
+    assert sized("pcb_linear_ce_bwd_workspace_bytes", 300, 1000, 200, piece, 1, 1) == whole, piece
+    assert sized("pcb_linear_ce_packed_bwd_workspace_bytes", 300, 1000, 200, piece, 1, 1) == whole, piece
+for tokens, vocab, dim in ((big, 1000, 200), (300, big, 200), (300, 1000, big), (big, big, big), (300, big - 100, 64),
+                           (2 ** 27, 1000, 200), (300, 2 ** 27, 200), (2 ** 26, 2 ** 26, 8)):
+    # what the passes refuse needs no room
+    assert sized("pcb_linear_ce_bwd_workspace_bytes", tokens, vocab, dim, 0, 1, 1) == 0, (tokens, vocab, dim)
+    assert sized("pcb_linear_ce_packed_bwd_workspace_bytes", tokens, vocab, dim, 0, 1, 1) == 0, (tokens, vocab, dim)
+    assert sized("pcb_linear_ce_packed_bytes", tokens, vocab, dim) == 0, (tokens, vocab, dim)
+for tokens, vocab in ((big, 1000), (300, big), (big, big), (300, big - 100), (2 ** 27, 10), (10, 2 ** 27), (2 ** 26, 2 ** 26)):
+    assert sized("pcb_linear_ce_fwd_workspace_bytes", tokens, vocab) == 0, (tokens, vocab)
+"""
+    done = subprocess.run([sys.executable, "-c", program, _lib.LIB_PATH], capture_output=True, text=True)
+    assert done.returncode == 0, (done.returncode, done.stderr)
+
+
+@gpu
+def test_a_piece_beyond_the_vocabulary():
+    x, w, target = _inputs(40, 300, 64, BF16, seed=19)
+    first = _check(x, w, target)
+    for piece in (10 ** 6, 2 ** 62, 2 ** 63 - 1):
+        for a, b in zip(_check(x, w, target, piece=piece), first):
+            assert torch.equal(a, b)
