@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
 
       // Row values are read before the wait, so their latency is hidden.
       int target = -1;  // within the piece
-      float top = 0.f, shift = 0.f, weight = 0.f;
+      float top = 0.f, shift = 0.f, weight = 0.f, sure = 0.f;
       if (in) {
         const long long tv = live.dense ? p.target[row] : p.target_packed[row];
         const bool valid = tv != p.ignore_index;
@@ -541,7 +541,10 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
           weight = p.row_weight ? p.row_weight[row] : 1.f;
           if (tv < 0 || tv >= p.vocab) weight = NAN;  // no such column
         }
-        if (valid && tv >= p.col0 + col0 && tv < p.col0 + limit) target = (int)(tv - p.col0);
+        if (valid && tv >= p.col0 + col0 && tv < p.col0 + limit) {
+          target = (int)(tv - p.col0);
+          if (MODE == kGradient) sure = kGradScale * expm1f(-p.stats[q.m + row] / kLog2e);
+        }
       }
       // The logits: the accumulators of all chunks, summed.
       float acc[EPI_COLS];
@@ -608,7 +611,12 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
           if (target >= col0 + b * 64 && target < col0 + b * 64 + 64) {
 #pragma unroll
             for (int j = 0; j < 64; ++j)
-              if (target == col0 + b * 64 + j) acc[b * 64 + j] -= kGradScale;
+              if (target == col0 + b * 64 + j) {
+                // A target with more than half of the probability is the largest logit,
+                // so p - 1 = 1 / s - 1: from log s itself, since in p - 1 little is left of the digits.
+                const float e = acc[b * 64 + j];
+                acc[b * 64 + j] = e > 0.5f * kGradScale ? sure : e - kGradScale;
+              }
           }
           // Tokens left out get zeros, whatever their logits are.
 #pragma unroll
@@ -928,14 +936,18 @@ struct RowArgs {
 
 constexpr int kRowWarps = 32, kRowLoads = 8;
 __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs p) {
-  __shared__ float ms[kRowWarps][32], ss[kRowWarps][32];
+  // Sums of exponentials in fp64: one that is hardly above 1 holds what a sure token's loss
+  // and gradients are made of.
+  __shared__ float ms[kRowWarps][32];
+  __shared__ double ss[kRowWarps][32];
   __shared__ double total[2][kRowWarps];
   __shared__ bool last;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;
   const int live = p.live ? *p.live : p.tokens;
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY;
+  double s = 0.0;
   if (row < live) {
     for (int i = warp; i < p.parts; i += kRowWarps * kRowLoads) {
       float2 o[kRowLoads];
@@ -948,9 +960,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
 #pragma unroll
       for (int j = 0; j < kRowLoads; ++j) mn = fmaxf(mn, o[j].x);
       const float base = mn == -INFINITY ? 0.f : mn;
-      s *= exp2f((m - base) * kLog2e);
+      s *= (double)exp2f((m - base) * kLog2e);
 #pragma unroll
-      for (int j = 0; j < kRowLoads; ++j) s += o[j].y * exp2f((o[j].x - base) * kLog2e);
+      for (int j = 0; j < kRowLoads; ++j) s += (double)(o[j].y * exp2f((o[j].x - base) * kLog2e));
       m = mn;
     }
   }
@@ -963,12 +975,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) loss_rows_kernel(const RowArgs
 #pragma unroll
     for (int i = 1; i < kRowWarps; ++i) top = fmaxf(top, ms[i][lane]);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kRowWarps; ++i) sum += ss[i][lane] * exp2f((ms[i][lane] - base) * kLog2e);
-    const float log_sum = logf(sum);
+    for (int i = 0; i < kRowWarps; ++i) sum += ss[i][lane] * (double)exp2f((ms[i][lane] - base) * kLog2e);
+    const float log_sum = log1pf((float)(sum - 1.0));
     p.stats[row] = base;
-    p.stats[p.tokens + row] = log2f(sum);
+    p.stats[p.tokens + row] = sum < 1.5 ? log_sum * kLog2e : log2f((float)sum);
     const int at = live < p.tokens ? p.order[row] : row;  // the token's own place
     const long long t = p.target[at];
     float v = 0.f;

@@ -597,3 +597,39 @@ def test_a_piece_beyond_the_vocabulary():
     for piece in (10 ** 6, 2 ** 62, 2 ** 63 - 1):
         for a, b in zip(_check(x, w, target, piece=piece), first):
             assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [60, 290])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gradients_of_sure_tokens(tokens, dtype):
+    """Tokens whose target has all but 1e-6 to 1e-3 of the probability keep what is left of the gradient's digits.
+
+    weight is half an identity and a row of x has its target's column, one other, and
+    -400 elsewhere, so a logit is one exact product and a probability of two terms: e in
+    1 + e is rounded once, by 2^-24 at most, and dx is 0.5 G, rounded to the type as G
+    and as dx; RTOL32 covers e's own exponential and the logarithm."""
+    vocab = 256
+    w = (0.5 * torch.eye(vocab)).to(dtype).cuda()
+    x = torch.full((tokens, vocab), -400.0)
+    g = torch.Generator().manual_seed(20)
+    target = torch.randint(0, vocab, (tokens,), generator=g)
+    other = (target + torch.randint(1, vocab, (tokens,), generator=g)) % vocab
+    rows = torch.arange(tokens)
+    x[rows, target] = 10.0
+    x[rows, other] = 10.0 - torch.randint(56, 112, (tokens,), generator=g) / 4  # e of exp(-7) to exp(-13.9)
+    x, target, other, rows = x.to(dtype).cuda().requires_grad_(), target.cuda(), other.cuda(), rows.cuda()
+    for reduction in ("sum", "none"):
+        loss = linear_cross_entropy(x, w, target, reduction=reduction)
+        dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+        logits = 0.5 * x.detach().double()
+        e = torch.exp(logits[rows, other] - logits[rows, target])
+        if reduction == "none":
+            _within(loss.detach(), torch.log1p(e), 2.0 ** -24 + RTOL32 * e, "loss")
+        for column, sign in ((target, -1.0), (other, 1.0)):
+            expected = sign * 0.5 * e / (1 + e)
+            off = 0.5 * 2.0 ** -24 + (2 * UNIT[dtype] * 1.01 + RTOL32) * expected.abs() + TINY[dtype]
+            _within(dx[rows, column], expected, off, f"{reduction} {sign:+.0f}")
+        rest = dx.clone()
+        rest[rows, target] = rest[rows, other] = 0.0
+        assert int(rest.count_nonzero()) == 0
