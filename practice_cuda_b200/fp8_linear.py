@@ -167,11 +167,30 @@ class FP8BlockLinear(nn.Linear):
 
     scaling: str = "fp32"
 
+    def _check_quantized(self, quantized: QuantResult, x2d: torch.Tensor) -> None:
+        data, scale = quantized.tensor, quantized.dequant_scale
+        blocks = (x2d.shape[0], -(-x2d.shape[1] // 128))
+        if self.scaling == "e8m0" and quantized.meta.get("scale_format") != "e8m0":
+            raise ValueError("an e8m0 linear needs its quantized input with power-of-two scales")
+        if data.shape != x2d.shape or data.dtype != E4M3 or tuple(scale.shape) != blocks or scale.dtype != torch.float32:
+            raise ValueError(f"quantized input must be e4m3 {tuple(x2d.shape)} with fp32 1x128 scales {blocks}, got "
+                             f"{data.dtype} {tuple(data.shape)} with {scale.dtype} {tuple(scale.shape)}")
+        if data.device != x2d.device or scale.device != x2d.device:
+            raise ValueError(f"quantized input must be on {x2d.device}, got {data.device} with scales on {scale.device}")
+
     def forward(self, x: torch.Tensor, quantized: Optional[QuantResult] = None) -> torch.Tensor:
         """``quantized``: x's 1x128 quantization with this layer's kind of
         scales, where the caller has it already (the norm before several
         linears, ``rms_norm.rms_norm``); x itself is still what the weight
         gradient quantizes along the tokens."""
+        shape = x.shape
+        x2d = x.reshape(-1, shape[-1])
+        if x2d.stride(-1) != 1:
+            x2d = x2d.contiguous()
+        x_data = x_scale = None
+        if quantized is not None:
+            self._check_quantized(quantized, x2d)
+            x_data, x_scale = quantized.tensor, quantized.dequant_scale
         w = self.weight
         if isinstance(w, BlockFP8Weight):  # unsharded by the FSDP2 FP8 all-gather
             w_data, w_scale = w._data, w._scale
@@ -179,19 +198,6 @@ class FP8BlockLinear(nn.Linear):
             master = getattr(w, "_tensor", w)  # FP8AllGatherWeight outside FSDP: its plain tensor
             w_data, w_scale = quantize_weight(master.detach(), pow2=self.scaling == "e8m0")
         w_hp = w
-        shape = x.shape
-        x2d = x.reshape(-1, shape[-1])
-        if x2d.stride(-1) != 1:
-            x2d = x2d.contiguous()
-        x_data = x_scale = None
-        if quantized is not None:
-            x_data, x_scale = quantized.tensor, quantized.dequant_scale
-            blocks = (x2d.shape[0], -(-x2d.shape[1] // 128))
-            if self.scaling == "e8m0" and quantized.meta.get("scale_format") != "e8m0":
-                raise ValueError("an e8m0 linear needs its quantized input with power-of-two scales")
-            if x_data.shape != x2d.shape or x_data.dtype != E4M3 or tuple(x_scale.shape) != blocks:
-                raise ValueError(f"quantized input must be e4m3 {tuple(x2d.shape)} with 1x128 scales {blocks}, got "
-                                 f"{x_data.dtype} {tuple(x_data.shape)} with {tuple(x_scale.shape)}")
         y = _FP8BlockLinearFn.apply(x2d, w_hp, w_data, w_scale, self.scaling == "e8m0", x_data, x_scale)
         y = y.reshape(*shape[:-1], y.shape[-1])
         if self.bias is not None:
