@@ -633,3 +633,65 @@ def test_gradients_of_sure_tokens(tokens, dtype):
         rest = dx.clone()
         rest[rows, target] = rest[rows, other] = 0.0
         assert int(rest.count_nonzero()) == 0
+
+
+@gpu
+def test_mean_loss_of_long_products():
+    """The tensor cores truncate as they add, which moves every logit towards zero and, since
+    the errors agree in sign, a mean loss with them.  Between two promotions (512 products, 32
+    additions of 16) each addition loses less than 2^-23 of the running sum, on average half of
+    that, of a sum that has on average come half of its way: 32 * 2^-23 / 4 < 1e-6 of a logit.
+    The loss is the difference of the target's logit and the expected one."""
+    tokens, vocab, dim = 2000, 4000, 4096
+    g = torch.Generator(device="cuda").manual_seed(21)
+    normal = lambda *shape: torch.randn(shape, generator=g, device="cuda")
+    weight = 0.02 * normal(vocab, dim)
+    target = torch.randint(0, vocab, (tokens,), generator=g, device="cuda")
+    lean = torch.rand((tokens, 1), generator=g, device="cuda") * 16.0 / (0.02 ** 2 * dim)
+    x, w = (normal(tokens, dim) + lean * weight[target]).bfloat16(), weight.bfloat16()
+    logits = x.double() @ w.double().t()
+    lse = torch.logsumexp(logits, 1)
+    at = logits.gather(1, target[:, None])[:, 0]
+    expected = (torch.exp(logits - lse[:, None]) * logits).sum(1)
+    loss = linear_cross_entropy(x, w, target).double()
+    off = (loss - (lse - at).mean()).abs()
+    bound = 1e-6 * (at - expected).abs().mean() + 2.0 ** -23 * (lse - at).mean()
+    assert bool(off <= bound), f"mean loss off by {off.item():.3e}, {(off / bound).item():.2f} of the bound"
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,dim,first,second", [
+    (60, 700, 136, 0.0, 0.3),  # single CTAs
+    (500, 3000, 256, 0.3, 0.0),
+    (2100, 8200, 4032, 0.1, 0.7),  # packed: another number of tiles
+    (2100, 8200, 4032, 0.5, 0.0),  # packed, then none left out
+])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_graph_of_both_passes_on_other_data(tokens, vocab, dim, first, second, reduction):
+    x, w, target = _inputs(tokens, vocab, dim, BF16, seed=22, ignored=first)
+    x.requires_grad_(), w.requires_grad_()
+    dloss = torch.rand(tokens if reduction == "none" else (), device="cuda") + 0.5
+
+    def step():
+        loss = linear_cross_entropy(x, w, target, reduction=reduction)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w), dloss))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed, ignored in ((23, second), (24, first)):
+        other = _inputs(tokens, vocab, dim, BF16, seed=seed, ignored=ignored)
+        with torch.no_grad():
+            x.copy_(other[0]), w.copy_(other[1]), target.copy_(other[2])
+        dloss.copy_(torch.rand_like(dloss) + 0.5)
+        for t in captured:
+            t.fill_(float("nan"))
+        graph.replay()
+        for a, b, name in zip(captured, step(), ("loss", "dx", "dw")):
+            assert torch.equal(a, b), name
+    assert _lib.device_error()[0] == 0

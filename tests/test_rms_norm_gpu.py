@@ -399,3 +399,75 @@ def test_entry_points_reject_bad_arguments_without_gpu():
     # the backward's workspace has to be there
     assert lib.pcb_rms_norm_bwd(16, 64, 16, 64, 2, 4, 64, None, 0, 16, 2, 16, 16, 64, 16, None, 0,
                                 None) == _lib.PCB_ERR_INVALID
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 512, 515, 4096, 4101, 16392, 20001])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_row_scales_of_zero_rows_and_non_finite_values(dim, dtype):
+    """A row's scale is that of its largest value: not a number where one of them is not."""
+    for residual in (False, True):
+        x, r, w = _inputs(7, dim, dtype, seed=3, residual=residual)
+        x[1] = 0
+        if residual:
+            r[1] = 0
+        x[2, 5], x[3, dim - 1], x[4, 0] = float("inf"), float("nan"), -float("inf")
+        for keep in (False, True):
+            res = rms_norm_quant(x, w, r, eps=EPS, quant="row", return_y=keep)
+            q, scale = res.quant.tensor.float(), res.quant.dequant_scale
+            assert int(q[1].count_nonzero()) == 0
+            _close(scale[1:2], torch.full((1,), 1e-12 / 448.0, device="cuda").double(), RTOL32, 0.0, "zero row scale")
+            for row in (2, 3, 4):  # an infinity's quotient is not a number
+                assert bool(torch.isnan(scale[row])) and bool(torch.isnan(q[row]).all())
+            assert not keep or bool(torch.isnan(res.y[3]).all())
+        good = [0, 5, 6]
+        _check_forward(x[good], None if r is None else r[good], w, "row", E4M3, what="rows beside them")
+
+
+@gpu
+@pytest.mark.parametrize("fp8", [E4M3, E5M2])
+def test_row_scales_feed_the_per_channel_product(fp8):
+    """The norm's QuantResult is one operand of the per-channel BMM as it is, but for the batch."""
+    from practice_cuda_b200.registry import QuantResult, get_bmm, get_quant
+    from tests._util import assert_bmm_close
+
+    x, r, w = _inputs(300, 512, BF16, seed=31)
+    res = rms_norm_quant(x, w, r, eps=EPS, quant="row", fp8_dtype=fp8, return_y=True)
+    a = QuantResult(res.quant.tensor[None], res.quant.dequant_scale[None], res.quant.impl, res.quant.granularity,
+                    res.quant.meta)
+    b = get_quant("b200_per_channel").fn(synthetic((1, 512, 384), std=0.05, seed=32).cuda(), channel_axis=-1, fp8_dtype=fp8)
+    out = get_bmm("b200_per_channel_a_k_b_n").fn(a, b)
+    expected = (res.quant.tensor.double() * res.quant.dequant_scale.double()[:, None]) @ (
+        b.tensor[0].double() * b.dequant_scale[0].double())
+    assert_bmm_close(out[0], expected, "norm into product")
+
+
+@gpu
+@pytest.mark.parametrize("rows,dim", [(300, 4096), (40, 515), (70, 8200)])
+def test_graph_of_both_passes_on_other_data(rows, dim):
+    x, r, w = _inputs(rows, dim, BF16, seed=33)
+    for t in (x, r, w):
+        t.requires_grad_()
+    dy, dh = torch.randn_like(x), torch.randn_like(x)
+
+    def step():
+        y, h, quant = rms_norm(x, w, r, quant="block")
+        return (y.detach(), h.detach(), quant.tensor.view(torch.uint8), quant.dequant_scale,
+                *torch.autograd.grad((y, h), (x, r, w), (dy, dh)))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    other = _inputs(rows, dim, BF16, seed=34)
+    with torch.no_grad():
+        for t, o in zip((x, r, w), other):
+            t.copy_(o)
+    dy.copy_(torch.randn_like(dy)), dh.copy_(torch.randn_like(dh))
+    graph.replay()
+    for a, b in zip(captured, step()):
+        assert torch.equal(a, b)
