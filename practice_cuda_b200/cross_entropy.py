@@ -22,12 +22,16 @@ from . import _lib
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _ALIGN = 8  # elements: 16 bytes, what a tensor map asks of a row
 _LINE = 64  # elements: 128 bytes
-# Rows that do not start on 128-byte lines are read with twice the requests,
-# which slows every product down.  With gradients wanted, from so many tokens on,
-# they are copied to rows that do (kept for the backward pass): on a B200 at 50001 x
-# 2056 fp16, loss and gradients of 512 tokens take 521 us as they are and 564 us
-# with the copy, of 1021 tokens 946 and 893 us, of 2048 tokens 1922 and 1752 us.
-# The loss alone does not gain from it (2048 tokens: 413 and 428 us).
+# Rows that do not start on 128-byte lines are read with twice the requests.  With
+# gradients wanted, x is copied to rows that do from so many tokens on (kept for the
+# backward pass), since every tile of all three products reads it again: on a B200 loss
+# and gradients of 1021 tokens of 50001 x 2056 fp16 take 720 us so and 811 us with x as
+# it is, 2048 tokens of 32000 x 4104 bf16 1558 and 1819 us, 4096 tokens of 32000 x 520
+# 619 and 646 us; 1021 tokens of 4001 x 264 70 and 68 us, and where tokens are left out
+# of large products, whose packed x lies on lines already, it costs up to 3 %.  Fewer
+# tokens would gain alike (512 of 50001 x 2056: 390 and 427 us).  The weight is not
+# worth its copy: with it those calls take 836, 1672 and 657 us, and 702 instead of 584
+# us with 30 % of the 1021 tokens left out.
 _LINES_FROM = 768
 
 
@@ -82,7 +86,7 @@ def _forward(x, weight, target, ignore_index, reduction, train):
     lib = _lib.lib()
     with _lib.on_device(device):
         lines = train and tokens >= _LINES_FROM
-        x2, w2 = _aligned_rows(x, lines), _aligned_rows(weight, lines)
+        x2, w2 = _aligned_rows(x, lines), _aligned_rows(weight, False)
         loss = x.new_empty((tokens,) if reduction == 0 else (), dtype=torch.float32)
         stats = x.new_empty((2 * tokens + 1,), dtype=torch.float32)  # [2, tokens], count
         if tokens == 0:

@@ -695,3 +695,19 @@ def test_graph_of_both_passes_on_other_data(tokens, vocab, dim, first, second, r
         for a, b, name in zip(captured, step(), ("loss", "dx", "dw")):
             assert torch.equal(a, b), name
     assert _lib.device_error()[0] == 0
+
+
+@gpu
+def test_the_weight_is_not_copied():
+    """Rows that suit TMA, if not whole lines: a copy of the weight would cost more than it gives, and stay until the
+    backward pass."""
+    x, w, target = _inputs(1024, 30000, 1032, BF16, seed=25)
+    w.requires_grad_()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    loss = linear_cross_entropy(x, w, target)
+    weight = w.numel() * w.element_size()
+    assert torch.cuda.max_memory_allocated() - before < weight // 2
+    dw, = torch.autograd.grad(loss, w)
+    assert dw.shape == w.shape
