@@ -140,7 +140,7 @@ void shape(loss::Problem& q, int64_t m, int64_t n, int64_t k, int splits, bool p
   q.n_blocks = (int)up(n, tile_n);
   q.k_stages = (int)up(k, loss::BK);
   const int target = pair ? loss::kChunkStages : loss::kChunkStagesSingle;
-  const int chunks = std::max(1, (q.k_stages + target / 2) / target);
+  const int chunks = (int)up(q.k_stages, target);
   q.chunk_stages = (int)up(q.k_stages, chunks);  // even chunks: a last one of a stage or two would stall the others
   q.a_rows = (int)std::min<int64_t>(loss::BM, up(m, 8) * 8);
   q.split_stages = (int)up(q.k_stages, splits);

@@ -42,7 +42,7 @@ constexpr int BM = 128;            // rows of the tile per CTA
 constexpr int TILE = 256;          // tile rows of the pair, and tile columns
 constexpr int BK = 64;             // K elements of a stage: one 128-byte swizzle atom of 16-bit values
 constexpr int UMMA_K = 16;
-// Stages between two promotions of a logit's accumulator, about.  On a B200 the
+// Stages between two promotions of a logit's accumulator, at most.  On a B200 the
 // mean loss of 4096 tokens (dim 4096) is 3.1e-7 off with 8 and takes 657 us, 2.2e-7
 // and 671 us with 6, 1.4e-7 and 694 us with 4.  (Longer first chunks, which run
 // while the epilogue finishes the tile before, take kGradient from 361 to 342 us at

@@ -711,3 +711,22 @@ def test_the_weight_is_not_copied():
     assert torch.cuda.max_memory_allocated() - before < weight // 2
     dw, = torch.autograd.grad(loss, w)
     assert dw.shape == w.shape
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("dim", [512, 576, 640, 704, 768, 1216, 4096])
+def test_logits_are_promoted_every_512_products(tokens, dim):
+    """A logit whose first 16 products make 2048 and whose further additions are each 15/16 of its last place: those of
+    the same 512 products may be lost, 31 of them, the others not.  The other logit is 2048 itself."""
+    x = torch.ones(tokens, dim, device="cuda", dtype=BF16)
+    w = torch.zeros(2, dim, device="cuda", dtype=BF16)
+    w[:, :16] = 128.0
+    place = 2.0 ** -12
+    w[0, 16:] = 15 / 256 * place
+    target = torch.zeros(tokens, device="cuda", dtype=torch.int64)
+    loss = linear_cross_entropy(x, w, target, reduction="none").double()
+    ahead = (dim - 16) * 15 / 256 * place  # of the first logit
+    # 31 additions that are lost, one rounding a promotion, and the loss's own (a slope of a half at most)
+    off = 0.5 * place * (31 * 15 / 16 + 0.5 * math.ceil(dim / 512)) + 2.0 ** -23
+    _within(loss, torch.full_like(loss, math.log1p(math.exp(-ahead))), off, "loss")
