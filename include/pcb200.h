@@ -399,8 +399,9 @@ int pcb_linear_ce_fwd(const void* x, int64_t sx, const void* weight, int64_t sw,
                       int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
                       float* loss, float* stats, float* count, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_bwd; piece as
- * there, want_dx and want_dw whether dx and dw are not NULL. */
+/* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_bwd, enough for
+ * pcb_linear_ce_packed_bwd too; piece as there, want_dx and want_dw whether dx
+ * and dw are not NULL. */
 int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx,
                                           int want_dw);
 
@@ -433,7 +434,8 @@ int pcb_linear_ce_packed_fwd(const void* x, int64_t sx, const void* weight, int6
                              int64_t vocab, int64_t dim, const int64_t* target, int64_t ignore_index, int reduction,
                              float* loss, float* stats, float* count, void* packed, int64_t packed_bytes,
                              void* workspace, int64_t workspace_bytes, void* stream);
-/* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_packed_bwd. */
+/* Device workspace (bytes, 256-byte aligned) of pcb_linear_ce_packed_bwd alone,
+ * which needs no copy of x for dw. */
 int64_t pcb_linear_ce_packed_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece,
                                                  int want_dx, int want_dw);
 int pcb_linear_ce_packed_bwd(const void* x, int64_t sx, const void* weight, int64_t sw, int dtype, int64_t tokens,

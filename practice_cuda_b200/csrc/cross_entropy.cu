@@ -555,7 +555,8 @@ int pcb_linear_ce_packed_fwd(const void* x, int64_t sx, const void* weight, int6
 int64_t pcb_linear_ce_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, int want_dx,
                                           int want_dw) {
   if (!has_workspace(tokens, vocab, dim)) return 0;
-  return BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0, false).bytes;
+  const int64_t plain = BwdPlan(tokens, vocab, dim, piece, want_dx != 0, want_dw != 0, false).bytes;
+  return std::max(plain, pcb_linear_ce_packed_bwd_workspace_bytes(tokens, vocab, dim, piece, want_dx, want_dw));
 }
 
 int64_t pcb_linear_ce_packed_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece,

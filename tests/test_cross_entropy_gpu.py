@@ -730,3 +730,15 @@ def test_logits_are_promoted_every_512_products(tokens, dim):
     # 31 additions that are lost, one rounding a promotion, and the loss's own (a slope of a half at most)
     off = 0.5 * place * (31 * 15 / 16 + 0.5 * math.ceil(dim / 512)) + 2.0 ** -23
     _within(loss, torch.full_like(loss, math.log1p(math.exp(-ahead))), off, "loss")
+
+
+def test_one_workspace_serves_either_backward_pass_without_gpu():
+    lib = _lib.lib()
+    for tokens in (1, 100, 515, 4096, 20000):
+        for vocab in (300, 8200, 16000, 32000, 50001, 128000):
+            for dim in (64, 1000, 4096):
+                for piece in (0, 256, 5000, 1 << 40):
+                    for want in ((1, 1), (1, 0), (0, 1)):
+                        args = (tokens, vocab, dim, piece, *want)
+                        packed = lib.pcb_linear_ce_packed_bwd_workspace_bytes(*args)
+                        assert 0 < packed <= lib.pcb_linear_ce_bwd_workspace_bytes(*args), args
