@@ -190,13 +190,13 @@ struct Cut {
 
 // Where the logits take about 90 us or more, tokens that are left out are packed
 // away.  Packed and as they are, on a B200, loss / loss and gradients in us: 1021
-// tokens of 50001 x 2056 fp16 with 30 % left out 154 / 760 and 216 / 889, with 60 %
-// 121 / 598 and 216 / 864, with none 204 / 809 and 199 / 802; 4096 tokens of 32000 x
-// 4096 with 30 % 668 / 2456 and 833 / 3150; 2048 tokens of 8192 x 4096 with 30 % 121 /
-// 384 and 136 / 469.  It costs three launches, 5 to 10 us, where no token is left
+// tokens of 50001 x 2056 fp16 with 30 % left out 125 / 583 and 179 / 700, with 60 %
+// 102 / 434 and 179 / 686, with none 183 / 716 and 177 / 710; 4096 tokens of 32000 x
+// 4096 with 30 % 565 / 2235 and 714 / 2872; 2048 tokens of 8192 x 4096 with 30 % 104 /
+// 342 and 116 / 425.  It costs three launches, about 6 us, where no token is left
 // out, and below this size that is more than most masks save.  The gain comes
-// in whole tiles of 256 tokens: 768 tokens with 30 % left out keep their three (180
-// / 653 and 177 / 671), hence no fewer than two of them.
+// in whole tiles of 256 tokens: 768 tokens of which 534 are left still fill three (123
+// / 522 and 138 / 553), hence no fewer than two of them.
 bool packs(int64_t tokens, int64_t vocab, int64_t dim) {
   return tokens >= 512 && (double)tokens * vocab * dim >= (double)(1ll << 36);
 }
@@ -240,7 +240,11 @@ struct FwdPlan {
 // writing and reading of their fp32 accumulators.  The shares are counted in
 // stages (0.27 us of the tensor cores) as the kernel hands them out: a tile's
 // epilogue is worth about six stages, a stage's time about 1.7 MB of traffic, and
-// the joining kernel about ten stages of its own.
+// the joining kernel about ten stages of its own.  Loss and gradients on a B200, in one
+// part, as this chooses and in the best of the ten numbers below: 8 tokens of 32000 x
+// 4096 435, 245 and 236 us, 256 tokens 447, 271 and 271, 512 tokens 526, 422 and 421; 64
+// tokens of 32000 x 1024 353, 105 and 105, 1024 tokens 410, 212 and 212; 8 tokens of 8192
+// x 4096 192, 145 and 125, the one of fifteen sizes where it is more than 4 % off.
 int split_of(int64_t tokens, int64_t vocab, int64_t dim, bool want_dw) {
   const int workers = std::max(1, device_info().sm_count / 2);
   const int64_t cols = up(dim, loss::WIDE), stages = up(vocab, loss::BK), halves = dim > loss::TILE ? 2 : 1;

@@ -20,7 +20,11 @@
 // logit.  The tensor cores truncate as they accumulate, which moves a logit of 4096
 // products by about 3e-6 of its size towards zero, and a mean loss with it; so
 // the logits' accumulators are added up in registers every 512 products (see
-// kChunkStages; 2.9e-6 without).
+// kChunkStages; 2.9e-6 without).  The products of G stay in the tensor cores: what
+// they lose is small beside the roundings of G and of the gradients to 16 bits.  On
+// 4096 tokens of 32000 x 4096 bf16, dX and dW are 1.7e-3 and 1.6e-3 of their norm off,
+// as rounding exact ones is; dW of 512 x 256 is 2.2e-3 off with 1024 tokens, 2.4e-3
+// with 16384 and 2.7e-3 with 262144.
 //
 // Tiles are 256 x 256 on a CTA pair (cta_group::2), fed by 64-deep stages of
 // 128-byte swizzled operands by TMA, with two accumulators of 256 fp32 columns in
@@ -398,7 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1) logits_kernel(const __grid_consta
   }
   gemm::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // The set-up above overlaps the previous kernel's tail; nothing global is
+  // Launched ahead of the previous kernel's end, which hides the launch (the kernels
+  // of this file let it start only once their CTAs have left); nothing global is
   // read or written before that kernel has completed.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (MODE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;

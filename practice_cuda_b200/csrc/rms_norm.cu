@@ -98,7 +98,7 @@ template <int XT, int LANES, int NV>
 int launch_norm_bwd(const norm::BwdArgs& p, int& parts, cudaStream_t s) {
   constexpr int threads = LANES > 256 ? LANES : 256, rows = threads / LANES;
   parts = norm_bwd_ctas(p.rows, rows, LANES > 256 ? 1 : 2);
-  const int smem = rows > 1 ? p.dim * 4 : 0;  // at most 1024 columns of fp32
+  const int smem = rows > 1 ? p.dim * 4 : 0;  // at most 2048 columns of fp32 (128 lanes of two units)
   norm::rms_norm_bwd_kernel<XT, LANES, NV><<<parts, threads, smem, s>>>(p);
   return check_launch("rms_norm_bwd_kernel");
 }
