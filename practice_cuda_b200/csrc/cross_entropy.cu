@@ -274,7 +274,7 @@ int split_of(int64_t tokens, int64_t vocab, int64_t dim, bool want_dw) {
 struct BwdPlan {
   int64_t cols, pieces, pitch;  // of G
   int splits;                   // parts of K of dX
-  int64_t g, acc, weight, alpha, x, pitch_x, bytes;
+  int64_t g, acc, weight, alpha, x, pitch_x, residue, first, next, bytes;
   bool copies;  // dW reads a copy of X without the rows of tokens that are left out
   BwdPlan(int64_t tokens, int64_t vocab, int64_t dim, int64_t piece, bool want_dx, bool want_dw, bool packed) {
     pitch_x = up(dim, 64) * 64;
@@ -299,6 +299,9 @@ struct BwdPlan {
     weight = c.take(tokens * 4);
     alpha = c.take(4);
     x = c.take(copy);
+    residue = c.take(tokens * 4);
+    first = c.take(want_dw ? vocab * 4 : 0);
+    next = c.take(want_dw ? tokens * 4 : 0);
     bytes = c.at;
   }
 };
@@ -430,6 +433,20 @@ int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtyp
                               count, (int)tokens, (int)dim, reinterpret_cast<uint16_t*>(ws + plan.x),
                               (long long)plan.pitch_x))
       return st;
+  base.residue = reinterpret_cast<float*>(ws + plan.residue);
+  base.x = static_cast<const uint16_t*>(x);
+  base.w = static_cast<const uint16_t*>(weight);
+  base.sx = sx;
+  base.sw = sw;
+  if (dw) {
+    int* first = reinterpret_cast<int*>(ws + plan.first);
+    int* next = reinterpret_cast<int*>(ws + plan.next);
+    if (int st = launch_after(loss::loss_tokens_of_targets_kernel, "loss_tokens_of_targets_kernel",
+                              up(tokens, loss::kListTokens), loss::kListThreads, s, base, first, next))
+      return st;
+    base.first = first;
+    base.next = next;
+  }
   for (int64_t i = 0; i < plan.pieces; ++i) {
     const int64_t col0 = i * plan.cols, cols = std::min(plan.cols, vocab - col0);
     const char* w = static_cast<const char*>(weight) + col0 * sw * 2;
@@ -453,6 +470,7 @@ int backward(const void* x, int64_t sx, const void* weight, int64_t sw, int dtyp
     if (int st = launch_logits<loss::kGradient>(p, pair, s)) return st;
 
     p = base;
+    p.col0 = (int)col0;
     int n = 0;
     if (dx) {
       loss::Problem& d = p.prob[n++];

@@ -742,3 +742,79 @@ def test_one_workspace_serves_either_backward_pass_without_gpu():
                         args = (tokens, vocab, dim, piece, *want)
                         packed = lib.pcb_linear_ce_packed_bwd_workspace_bytes(*args)
                         assert 0 < packed <= lib.pcb_linear_ce_bwd_workspace_bytes(*args), args
+
+
+@gpu
+@pytest.mark.parametrize("tokens,vocab,dim,piece,ignored", [
+    (1, 700, 2048, None, 0.0), (1, 5000, 771, None, 0.0), (7, 1500, 4096, 512, 0.0), (40, 3000, 1032, None, 0.3),
+    (128, 257, 2056, None, 0.0), (129, 9000, 1001, None, 0.0), (300, 4099, 2048, 1024, 0.2), (700, 24001, 4104, None, 0.5),
+    (2100, 8200, 4032, None, 0.0), (2100, 8200, 4032, 2048, 0.4),
+])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_of_gradients_are_not_moved_as_a_whole(tokens, vocab, dim, piece, ignored, dtype):
+    """G holds a token's own entry beyond 16 bits: the entry multiplies all of a row, so its rounding would move the row as
+    one, by up to 2^-9 (bf16).
+
+    k is a row's component along the exact one.  Rounding the result's elements moves it by the sum of
+    independent errors of at most UNIT, uniform at most (UNIT / sqrt(3) each); so do the roundings of the other
+    entries of G, through the part of their rows that lies along this one.  Seven times their root of
+    summed squares is allowed, and RTOL32 for the arithmetic between."""
+    x, w, target = _inputs(tokens, vocab, dim, dtype, seed=dim, ignored=ignored)
+    target[0] = 3
+    target[tokens // 2] = 3  # two tokens of one target
+    g = torch.Generator().manual_seed(26)
+    dloss = (torch.rand(tokens, generator=g) + 0.5).cuda() * (1.0 if dtype == BF16 else 64.0)
+    x.requires_grad_(), w.requires_grad_()
+    loss = linear_cross_entropy(x, w, target, reduction="none", vocab_piece=piece)
+    dx, dw = torch.autograd.grad(loss, (x, w), dloss)
+    x64, w64 = x.detach().double(), w.detach().double()
+    valid = target != IGNORE
+    at = torch.where(valid, target, 0)[:, None]
+    p = torch.softmax(x64 @ w64.t(), 1) * torch.where(valid, dloss.double(), 0.0)[:, None]
+    full = p.scatter_add(1, at, torch.where(valid, -dloss.double(), 0.0)[:, None])
+    p.scatter_(1, at, 0.0)  # the entries that are rounded
+    unit = UNIT[dtype] / math.sqrt(3.0)
+
+    def along(got, exact, entries, rows):
+        """k of each row, and how far it may be off, for exact = (entries and the own ones) @ rows."""
+        square = exact.square().sum(1)
+        k = (got.double() * exact).sum(1) / square - 1
+        rounded = exact.pow(4).sum(1)
+        others = (entries.square() * (exact @ rows.t()).square()).sum(1)
+        return k.abs(), 7 * unit * torch.sqrt(rounded + others) / square + RTOL32 + 2 * LOGIT
+
+    LOGIT = ((dim / 16 + 8) * 2.0 ** -23 * x64.norm(dim=1).max() * w64.norm(dim=1).max()).item()
+    k, off = along(dx, full @ w64, p, w64)
+    assert bool((k <= off)[valid].all()), f"dx moved by {k[valid].max().item():.2e}, {(k / off)[valid].max().item():.2f} of its bound"
+    rows = torch.unique(target[valid])
+    k, off = along(dw[rows], full.t()[rows] @ x64, p.t()[rows], x64)
+    assert bool((k <= off).all()), f"dw moved by {k.max().item():.2e}, {(k / off).max().item():.2f} of its bound"
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [5, 70, 1000, 9000])
+@pytest.mark.parametrize("pattern", ["one", "two in turn", "blocks", "random", "far apart"])
+def test_tokens_that_share_targets(tokens, pattern):
+    """Lists of a target's tokens: every length, neighbours, tokens that are thousands apart, ignore_index among the columns."""
+    vocab, dim = 301, 72
+    x, w, target = _inputs(tokens, vocab, dim, BF16, seed=27)
+    i = torch.arange(tokens, device="cuda")
+    if pattern == "one":
+        target[:] = 300
+    elif pattern == "two in turn":
+        target = i % 2 * 255
+    elif pattern == "blocks":
+        target = i // 9 % vocab
+    elif pattern == "far apart":
+        target = torch.where(i < tokens // 2, i % 150, 200 + i % 90)
+        target[0] = target[-1] = 299
+    first = _check(x, w, target, "mean", what=pattern)
+    for a, b in zip(_check(x, w, target, "mean", what=pattern), first):
+        assert torch.equal(a, b)
+    # A column may be what marks the tokens that are left out.
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = target == int(target[-1])
+    got = torch.autograd.grad(linear_cross_entropy(xg, wg, target, reduction="sum", ignore_index=int(target[-1])), (xg, wg))
+    want = torch.autograd.grad(linear_cross_entropy(xg, wg, target.masked_fill(out, IGNORE), reduction="sum"), (xg, wg))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
