@@ -25,12 +25,12 @@ _LINE = 64  # elements: 128 bytes
 # Rows that do not start on 128-byte lines are read with twice the requests.  With
 # gradients wanted, x is copied to rows that do from so many tokens on (kept for the
 # backward pass), since every tile of all three products reads it again: on a B200 loss
-# and gradients of 1021 tokens of 50001 x 2056 fp16 take 720 us so and 811 us with x as
-# it is, 2048 tokens of 32000 x 4104 bf16 1558 and 1819 us, 4096 tokens of 32000 x 520
-# 619 and 646 us; 1021 tokens of 4001 x 264 70 and 68 us, and where tokens are left out
+# and gradients of 1021 tokens of 50001 x 2056 fp16 take 749 us so and 786 us with x as
+# it is, 2048 tokens of 32000 x 4104 bf16 1656 and 1804 us, 4096 tokens of 32000 x 520
+# 676 and 685 us; 1021 tokens of 4001 x 264 78 and 76 us, and where tokens are left out
 # of large products, whose packed x lies on lines already, it costs up to 3 %.  Fewer
-# tokens would gain alike (512 of 50001 x 2056: 390 and 427 us).  The weight is not
-# worth its copy: with it those calls take 836, 1672 and 657 us, and 702 instead of 584
+# tokens would gain alike (512 of 50001 x 2056: 419 and 450 us).  The weight is not
+# worth its copy: with it those calls take 859, 1786 and 716 us, and 770 instead of 645
 # us with 30 % of the 1021 tokens left out.
 _LINES_FROM = 768
 

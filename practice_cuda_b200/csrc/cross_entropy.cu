@@ -190,13 +190,13 @@ struct Cut {
 
 // Where the logits take about 90 us or more, tokens that are left out are packed
 // away.  Packed and as they are, on a B200, loss / loss and gradients in us: 1021
-// tokens of 50001 x 2056 fp16 with 30 % left out 125 / 583 and 179 / 700, with 60 %
-// 102 / 434 and 179 / 686, with none 183 / 716 and 177 / 710; 4096 tokens of 32000 x
-// 4096 with 30 % 565 / 2235 and 714 / 2872; 2048 tokens of 8192 x 4096 with 30 % 104 /
-// 342 and 116 / 425.  It costs three launches, about 6 us, where no token is left
+// tokens of 50001 x 2056 fp16 with 30 % left out 126 / 627 and 179 / 729, with 60 %
+// 101 / 465 and 179 / 710, with none 183 / 741 and 177 / 735; 4096 tokens of 32000 x
+// 4096 with 30 % 549 / 2286 and 679 / 2885; 2048 tokens of 8192 x 4096 with 30 % 96 /
+// 381 and 106 / 457.  It costs three launches, about 6 us, where no token is left
 // out, and below this size that is more than most masks save.  The gain comes
-// in whole tiles of 256 tokens: 768 tokens of which 534 are left still fill three (123
-// / 522 and 138 / 553), hence no fewer than two of them.
+// in whole tiles of 256 tokens: 768 tokens of which 534 are left still fill three (131
+// / 564 and 146 / 590), hence no fewer than two of them.
 bool packs(int64_t tokens, int64_t vocab, int64_t dim) {
   return tokens >= 512 && (double)tokens * vocab * dim >= (double)(1ll << 36);
 }
@@ -242,9 +242,9 @@ struct FwdPlan {
 // epilogue is worth about six stages, a stage's time about 1.7 MB of traffic, and
 // the joining kernel about ten stages of its own.  Loss and gradients on a B200, in one
 // part, as this chooses and in the best of the ten numbers below: 8 tokens of 32000 x
-// 4096 435, 245 and 236 us, 256 tokens 447, 271 and 271, 512 tokens 526, 422 and 421; 64
-// tokens of 32000 x 1024 353, 105 and 105, 1024 tokens 410, 212 and 212; 8 tokens of 8192
-// x 4096 192, 145 and 125, the one of fifteen sizes where it is more than 4 % off.
+// 4096 441, 271 and 253 us, 256 tokens 451, 296 and 296, 512 tokens 534, 466 and 466; 64
+// tokens of 32000 x 1024 364, 122 and 118, 1024 tokens 431, 239 and 239; 8 tokens of 8192
+// x 4096 192, 152 and 138.  At fifteen sizes it is never more than 10 % off the best.
 int split_of(int64_t tokens, int64_t vocab, int64_t dim, bool want_dw) {
   const int workers = std::max(1, device_info().sm_count / 2);
   const int64_t cols = up(dim, loss::WIDE), stages = up(vocab, loss::BK), halves = dim > loss::TILE ? 2 : 1;

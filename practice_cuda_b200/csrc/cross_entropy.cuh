@@ -11,20 +11,22 @@
 //   logits_kernel<kGradient>  the logits of one piece of the vocabulary again,
 //              leaving as G in the operands' 16-bit type (the one rounding that a
 //              tensor-core product of G asks for; w_i and a are split so that it
-//              is of the order of 1 and the loss's scale stays in fp32).
+//              is of the order of 1 and the loss's scale stays in fp32); what that
+//              takes from each token's own entry is kept in fp32 (see fetch_rows).
 //   grad_products_kernel      dX += G W and dW = G^T X of that piece in one launch:
 //              the tiles of both share the grid, so neither leaves SMs idle at its
-//              end.
+//              end; its epilogue adds what the own entries lost.
 // Logits, softmax statistics and every sum are fp32.  m and log2 s are kept apart:
 // their sum would lose the small part of a sure token's probability beside a large
 // logit.  The tensor cores truncate as they accumulate, which moves a logit of 4096
 // products by about 3e-6 of its size towards zero, and a mean loss with it; so
 // the logits' accumulators are added up in registers every 512 products (see
 // kChunkStages; 2.9e-6 without).  The products of G stay in the tensor cores: what
-// they lose is small beside the roundings of G and of the gradients to 16 bits.  On
-// 4096 tokens of 32000 x 4096 bf16, dX and dW are 1.7e-3 and 1.6e-3 of their norm off,
-// as rounding exact ones is; dW of 512 x 256 is 2.2e-3 off with 1024 tokens, 2.4e-3
-// with 16384 and 2.7e-3 with 262144.
+// they lose is small beside the rounding of the gradients to 16 bits.  On 4096
+// tokens of 32000 x 4096 bf16, dX and dW are 1.7e-3 and 1.6e-3 of their norm off, as
+// rounding exact ones is.  Where a column is the target of many more tokens than
+// are corrected (kMostCorrected), what rounding G takes shows: dW of 512 x 256 is 1.7e-3
+// off with 4096 tokens, 2.1e-3 with 16384, 2.7e-3 with 262144.
 //
 // Tiles are 256 x 256 on a CTA pair (cta_group::2), fed by 64-deep stages of
 // 128-byte swizzled operands by TMA, with two accumulators of 256 fp32 columns in
@@ -242,8 +244,9 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // accumulators a thread, stay as they are without.  Of 160 drawn sizes (1 to 4096 tokens,
 // bf16 and fp16) the gradients' error is then 1.00 to 1.01 times that of fp32 products,
 // 0.9 to 2.1 times without.  Loss and gradients of 8 tokens of 32000 x 4096 take 272 us
-// so and 249 us without, of 256 tokens 300 and 278 us, of 1024 tokens 755 and 744 us, of
-// 4096 tokens 3320 and 3297 us.  (Added to the registers after the tensor memory is
+// so and 249 us without, of 256 tokens 296 and 278 us, of 1024 tokens 775 and 744 us, of
+// 4096 tokens 3286 and 3297 us; of 256 tokens of 8192 x 4096, whose rows of dW take a token
+// more often, 178 and 157 us.  (Added to the registers after the tensor memory is
 // given back: 355 us with 256 tokens, since they spill; loaded by each lane for
 // itself: 373 us.)
 constexpr int kFetched = 16;  // rows of 256 bytes: 4 KB
@@ -294,8 +297,9 @@ __device__ __forceinline__ void add_row(uint32_t taddr, uint32_t stg, int slot, 
   }
   tmem_wait_st();
 }
-// Tokens of one target that are corrected so in its row of dW: beyond a few of
-// them their roundings cancel as those of any sum do.
+// Tokens of one target that are corrected so in its row of dW, one after the other:
+// a column that thousands of tokens share must not hold its tile up for as many
+// fetches, and beyond a few tokens their roundings cancel for the most part.
 constexpr int kMostCorrected = 8;
 constexpr int kNoToken = 0x7fffffff;
 
