@@ -243,12 +243,13 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // memory, 32 columns at a time, so that the registers of the epilogue, which holds 128
 // accumulators a thread, stay as they are without.  Of 160 drawn sizes (1 to 4096 tokens,
 // bf16 and fp16) the gradients' error is then 1.00 to 1.01 times that of fp32 products,
-// 0.9 to 2.1 times without.  Loss and gradients of 8 tokens of 32000 x 4096 take 272 us
-// so and 249 us without, of 256 tokens 296 and 278 us, of 1024 tokens 775 and 744 us, of
-// 4096 tokens 3286 and 3297 us; of 256 tokens of 8192 x 4096, whose rows of dW take a token
-// more often, 178 and 157 us.  (Added to the registers after the tensor memory is
-// given back: 355 us with 256 tokens, since they spill; loaded by each lane for
-// itself: 373 us.)
+// 0.9 to 2.1 times without.  Loss and gradients of 8 tokens of 32000 x 4096 take 269 us
+// so and 248 us without, of 256 tokens 297 and 273 us, of 1024 tokens 765 and 726 us, of
+// 4096 tokens 3286 and 3297 us; of 512 tokens of 8192 x 4096, where nearly every tile of
+// dW has rows with two tokens, 200 and 148 us, of 2048 tokens 450 and 390 us.  (Added to
+// the registers after the tensor memory is given back: 355 us with 256 tokens of 32000 x
+// 4096, since they spill; loaded by each lane for itself: 373 us; up to three tokens of
+// a row fetched at once: 310 us, and 173 us with 512 of 8192 x 4096.)
 constexpr int kFetched = 16;  // rows of 256 bytes: 4 KB
 // `row` (16-byte aligned) of the lanes in `lanes`, `cols` elements of it at most.
 __device__ __forceinline__ void fetch_rows(const uint16_t* row, uint32_t lanes, int cols, uint32_t stg, int lane) {
